@@ -1,0 +1,244 @@
+// tms_kv.hip -- the paged cache's own moves: new tokens written to their slots
+// (tms_kv_append), and a cache cut down to the entries of the largest
+// accumulated attention weight (tms_kv_evict).
+#include <algorithm>
+
+#include "tms_cache.h"
+#include "tms_device.h"
+
+namespace tms {
+
+struct AppendParams {
+    CacheView c;
+    const char* k;
+    const char* v;
+    int64_t kt, kh, vt, vh;   // bytes between tokens, heads
+    int hv, tv;               // 16-byte pieces of a head's row and of a token's
+};
+
+// A thread moves 16 bytes of a key and of a value.  Bound by latency for a
+// decode step (length, table entry and data one after another), by memory for
+// a prompt.
+__global__ __launch_bounds__(256) void append_kernel(AppendParams a) {
+    const int b = blockIdx.y;
+    const SeqView sq = seq_view(a.c, b);
+    const int32_t* row = a.c.tables + (int64_t)b * a.c.tstride;
+    const int64_t all = (int64_t)sq.n * a.tv;
+    for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < all; x += (int64_t)gridDim.x * 256) {
+        const int i = (int)(x / a.tv), w = (int)(x - (int64_t)i * a.tv), h = w / a.hv, d = w - h * a.hv;
+        const int64_t tok = sq.q0 + i;
+        const uint4 kx = *(const uint4*)(a.k + tok * a.kt + h * a.kh + 16 * d);
+        const uint4 vx = *(const uint4*)(a.v + tok * a.vt + h * a.vh + 16 * d);
+        const int j = sq.p0 + i, page = page_of(a.c, row, j, sq.len);
+        if (page < 0) continue;
+        const int slot = j & a.c.smask;
+        *(uint4*)(a.c.k + (int64_t)page * a.c.kp + h * a.c.kh + (int64_t)slot * a.c.ks + 16 * d) = kx;
+        *(uint4*)(a.c.v + (int64_t)page * a.c.vp + h * a.c.vh + (int64_t)slot * a.c.vs + 16 * d) = vx;
+        if (d == 0 && a.c.scores) a.c.scores[(((int64_t)page * a.c.kv_heads + h) << a.c.shift) + slot] = 0.f;
+    }
+}
+
+struct EvictParams {
+    CacheView c;
+    const int32_t* dst;
+    int64_t dstride;
+    int budget, sinks, recent, max_kv;
+    int32_t* new_len;
+    int32_t* kept;
+};
+
+__device__ __forceinline__ int evict_len(const EvictParams& a, int b) {
+    const int64_t cap = a.c.tstride << a.c.shift;
+    const int L = min(max(a.c.kv_len[b], 0), a.max_kv);
+    return (int)(cap < L ? cap : L);
+}
+
+// A score's place in the order of eviction: larger is kept longer.  NaN, and
+// positions on unmapped pages, come first to go.
+__device__ __forceinline__ uint32_t evict_key(const EvictParams& a, const int32_t* row, int h, int j, int len) {
+    const int page = page_of(a.c, row, j, len);
+    if (page < 0) return 0u;
+    const float s = a.c.scores[(((int64_t)page * a.c.kv_heads + h) << a.c.shift) + (j & a.c.smask)];
+    return s == s ? okey(s) : 0u;
+}
+
+// One workgroup a sequence and head: the key of the last entry kept, by a
+// radix select over the order keys, 8 bits a pass; then each thread counts
+// the entries of its own stretch above it and tied with it, one scan gives
+// the counts before the stretch, and an entry's new position is
+// sinks + above + min(tied, those that still fit).
+__global__ __launch_bounds__(1024) void evict_select_kernel(EvictParams a) {
+    __shared__ uint32_t hist[16][256];
+    __shared__ uint32_t part[16][2];
+    __shared__ uint32_t pick[2];
+    const int b = blockIdx.x / a.c.kv_heads, h = blockIdx.x - b * a.c.kv_heads;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int L = evict_len(a, b);
+    const int32_t* row = a.c.tables + (int64_t)b * a.c.tstride;
+    int32_t* kept = a.kept + (int64_t)blockIdx.x * a.budget;
+    for (int i = min(L, a.budget) + t; i < a.budget; i += 1024) kept[i] = -1;
+    if (L <= a.budget) {
+        for (int i = t; i < L; i += 1024) kept[i] = i;
+        return;
+    }
+    const int lo = a.sinks, hi = L - a.recent, want = a.budget - a.sinks - a.recent;
+    for (int i = t; i < lo; i += 1024) kept[i] = i;
+    for (int i = t; i < a.recent; i += 1024) kept[a.budget - a.recent + i] = hi + i;
+    if (want == 0) return;
+
+    uint32_t prefix = 0, fixed = 0;
+    uint32_t left = (uint32_t)want;   // of the entries that share the prefix
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        for (int i = t; i < 16 * 256; i += 1024) ((uint32_t*)hist)[i] = 0;
+        __syncthreads();
+        for (int j = lo + t; j < hi; j += 1024) {
+            const uint32_t k = evict_key(a, row, h, j, L);
+            if ((k & fixed) == prefix) atomicAdd(&hist[wave][k >> shift & 255], 1u);
+        }
+        __syncthreads();
+        if (t < 256) {
+            uint32_t n = 0;
+            for (int w = 0; w < 16; ++w) n += hist[w][t];
+            hist[0][t] = n;
+        }
+        __syncthreads();
+        if (t < 64) {   // the highest digit with `left` entries at or above it
+            uint32_t n[4], mine = 0;
+            for (int i = 0; i < 4; ++i) mine += n[i] = hist[0][255 - (4 * t + i)];
+            uint32_t upto = mine;
+            for (int x = 1; x < 64; x <<= 1) {
+                const uint32_t y = __shfl_up(upto, x);
+                if (lane >= x) upto += y;
+            }
+            uint32_t above = upto - mine;
+            for (int i = 0; i < 4; ++i) {
+                if (above < left && above + n[i] >= left) {
+                    pick[0] = 255 - (4 * t + i);
+                    pick[1] = left - above;
+                }
+                above += n[i];
+            }
+        }
+        __syncthreads();
+        prefix |= pick[0] << shift;
+        fixed |= 255u << shift;
+        left = pick[1];
+        __syncthreads();
+    }
+
+    const int per = (hi - lo + 1023) / 1024, from = min(lo + t * per, hi), to = min(from + per, hi);
+    uint32_t above = 0, tied = 0;
+    for (int j = from; j < to; ++j) {
+        const uint32_t k = evict_key(a, row, h, j, L);
+        above += k > prefix;
+        tied += k == prefix;
+    }
+    uint32_t sa = above, st = tied;
+    for (int x = 1; x < 64; x <<= 1) {
+        const uint32_t ya = __shfl_up(sa, x), yt = __shfl_up(st, x);
+        if (lane >= x) {
+            sa += ya;
+            st += yt;
+        }
+    }
+    if (lane == 63) {
+        part[wave][0] = sa;
+        part[wave][1] = st;
+    }
+    __syncthreads();
+    sa -= above;
+    st -= tied;
+    for (int w = 0; w < wave; ++w) {
+        sa += part[w][0];
+        st += part[w][1];
+    }
+    for (int j = from; j < to; ++j) {
+        const uint32_t k = evict_key(a, row, h, j, L);
+        if (k > prefix || (k == prefix && st < left)) kept[lo + sa + min(st, left)] = j;
+        sa += k > prefix;
+        st += k == prefix;
+    }
+}
+
+// 16 bytes of a kept entry's key and value a thread, from its old slot to its
+// new one; the first piece's thread moves the score too.
+__global__ __launch_bounds__(256) void evict_copy_kernel(EvictParams a, int hv) {
+    const int b = blockIdx.x / a.c.kv_heads, h = blockIdx.x - b * a.c.kv_heads;
+    const int L = evict_len(a, b), n = min(L, a.budget);
+    if (h == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.new_len[b] = n;
+    const int32_t* row = a.c.tables + (int64_t)b * a.c.tstride;
+    const int32_t* dst = a.dst + (int64_t)b * a.dstride;
+    const int32_t* kept = a.kept + (int64_t)blockIdx.x * a.budget;
+    const int64_t all = (int64_t)n * hv;
+    for (int64_t x = (int64_t)blockIdx.y * 256 + threadIdx.x; x < all; x += (int64_t)gridDim.y * 256) {
+        const int i = (int)(x / hv), d = (int)(x - (int64_t)i * hv);
+        const int j = kept[i], from = page_of(a.c, row, j, L), to = dst[i >> a.c.shift];
+        if (from < 0 || (unsigned)to >= (unsigned)a.c.pages) continue;
+        const int64_t s0 = j & a.c.smask, s1 = i & a.c.smask;
+        const uint4 kx = *(const uint4*)(a.c.k + from * a.c.kp + h * a.c.kh + s0 * a.c.ks + 16 * d);
+        const uint4 vx = *(const uint4*)(a.c.v + from * a.c.vp + h * a.c.vh + s0 * a.c.vs + 16 * d);
+        *(uint4*)(a.c.k + to * a.c.kp + h * a.c.kh + s1 * a.c.ks + 16 * d) = kx;
+        *(uint4*)(a.c.v + to * a.c.vp + h * a.c.vh + s1 * a.c.vs + 16 * d) = vx;
+        if (d == 0)
+            a.c.scores[(((int64_t)to * a.c.kv_heads + h) << a.c.shift) + s1] =
+                a.c.scores[(((int64_t)from * a.c.kv_heads + h) << a.c.shift) + s0];
+    }
+}
+
+}  // namespace tms
+
+extern "C" int tms_kv_append(const tms_cache* cache, const tms_append_args* args, hipStream_t stream) {
+    using namespace tms;
+    const int rc = check_cache(cache, true, true);
+    if (rc != TMS_OK) return rc;
+    if (!args) return TMS_ERR_INVALID_ARG;
+    for (int i = 0; i < 2; ++i)
+        if (args->k_new_stride[i] < 0 || args->k_new_stride[i] % 8 || args->v_new_stride[i] < 0 || args->v_new_stride[i] % 8)
+            return TMS_ERR_INVALID_ARG;
+    if (cache->batch > 65535) return TMS_ERR_CAPACITY;
+    if (cache->batch == 0 || cache->tokens == 0 || cache->max_q == 0) return TMS_OK;
+    if (!args->k_new || !args->v_new || !aligned16(args->k_new) || !aligned16(args->v_new)) return TMS_ERR_INVALID_ARG;
+    AppendParams a;
+    a.c = view_of(cache);
+    a.k = (const char*)args->k_new;
+    a.v = (const char*)args->v_new;
+    a.kt = 2 * args->k_new_stride[0];
+    a.kh = 2 * args->k_new_stride[1];
+    a.vt = 2 * args->v_new_stride[0];
+    a.vh = 2 * args->v_new_stride[1];
+    a.hv = cache->head_dim / 8;
+    a.tv = a.hv * cache->kv_heads;
+    const int64_t blocks = ((int64_t)std::min(cache->max_q, cache->tokens) * a.tv + 255) / 256;
+    hipLaunchKernelGGL(append_kernel, dim3((unsigned)std::min<int64_t>(blocks, 1 << 20), cache->batch), dim3(256), 0, stream, a);
+    return hipGetLastError() == hipSuccess ? TMS_OK : TMS_ERR_HIP;
+}
+
+extern "C" int tms_kv_evict(const tms_cache* cache, const tms_evict_args* args, hipStream_t stream) {
+    using namespace tms;
+    const int rc = check_cache(cache, true, false);
+    if (rc != TMS_OK) return rc;
+    if (!args || args->reserved != 0 || args->budget < 1 || args->sinks < 0 || args->recent < 0 ||
+        (int64_t)args->sinks + args->recent > args->budget)
+        return TMS_ERR_INVALID_ARG;
+    if (cache->max_kv > TMS_EVICT_MAX_KV) return TMS_ERR_CAPACITY;
+    if (cache->batch == 0) return TMS_OK;
+    const int most = std::min(args->budget, cache->max_kv);
+    if (!cache->scores || !args->dst_tables || !args->new_len || !args->kept || args->dst_table_stride < 1 ||
+        args->dst_table_stride < (most + cache->page_size - 1) / cache->page_size)
+        return TMS_ERR_INVALID_ARG;
+    EvictParams a;
+    a.c = view_of(cache);
+    a.dst = args->dst_tables;
+    a.dstride = args->dst_table_stride;
+    a.budget = args->budget;
+    a.sinks = args->sinks;
+    a.recent = args->recent;
+    a.max_kv = cache->max_kv;
+    a.new_len = args->new_len;
+    a.kept = args->kept;
+    const int pairs = cache->batch * cache->kv_heads, hv = cache->head_dim / 8;
+    hipLaunchKernelGGL(evict_select_kernel, dim3(pairs), dim3(1024), 0, stream, a);
+    const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>(((int64_t)most * hv + 255) / 256, 65535));
+    hipLaunchKernelGGL(evict_copy_kernel, dim3(pairs, (unsigned)blocks), dim3(256), 0, stream, a, hv);
+    return hipGetLastError() == hipSuccess ? TMS_OK : TMS_ERR_HIP;
+}

@@ -27,7 +27,7 @@ ROWS_ANY, ROWS_TOPK, ROWS_SPARSE_MASK = 0, 1, 2
 ROW_OK, ROW_BAD_PARAMS, ROW_ALL_MASKED, ROW_NONFINITE, ROW_UNSUPPORTED = 0, 1, 2, 3, 4
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 
-# Every symbol include/tmsample_hip.h declares.
+# Every symbol include/*.h declares.
 EXPORTS = (
     "tms_abi_version",
     "tms_status_string",
@@ -92,6 +92,12 @@ EXPORTS = (
     "tms_token_slot_fill",
     "tms_token_slot_peek",
     "tms_embed_gather",
+    "tms_kv_append",
+    "tms_paged_attention_workspace",
+    "tms_paged_attention",
+    "tms_kv_add_scores",
+    "tms_kv_evict",
+    "tms_adjust_logits",
 )
 
 
