@@ -161,10 +161,13 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(EvictParams a) {
 }
 
 // 16 bytes of a kept entry's key and value a thread, from its old slot to its
-// new one; the first piece's thread moves the score too.
+// new one; the first piece's thread moves the score too.  new_len may be the
+// array kv_len: a length read here is the old or the new one, and both give
+// the same number of entries; where those lie is in `kept`.
 __global__ __launch_bounds__(256) void evict_copy_kernel(EvictParams a, int hv) {
     const int b = blockIdx.x / a.c.kv_heads, h = blockIdx.x - b * a.c.kv_heads;
-    const int L = evict_len(a, b), n = min(L, a.budget);
+    const int n = min(evict_len(a, b), a.budget);
+    const int end = (int)min(a.c.tstride << a.c.shift, (int64_t)kMaxLen);
     if (h == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.new_len[b] = n;
     const int32_t* row = a.c.tables + (int64_t)b * a.c.tstride;
     const int32_t* dst = a.dst + (int64_t)b * a.dstride;
@@ -172,7 +175,7 @@ __global__ __launch_bounds__(256) void evict_copy_kernel(EvictParams a, int hv) 
     const int64_t all = (int64_t)n * hv;
     for (int64_t x = (int64_t)blockIdx.y * 256 + threadIdx.x; x < all; x += (int64_t)gridDim.y * 256) {
         const int i = (int)(x / hv), d = (int)(x - (int64_t)i * hv);
-        const int j = kept[i], from = page_of(a.c, row, j, L), to = dst[i >> a.c.shift];
+        const int j = kept[i], from = page_of(a.c, row, j, end), to = dst[i >> a.c.shift];
         if (from < 0 || (unsigned)to >= (unsigned)a.c.pages) continue;
         const int64_t s0 = j & a.c.smask, s1 = i & a.c.smask;
         const uint4 kx = *(const uint4*)(a.c.k + from * a.c.kp + h * a.c.kh + s0 * a.c.ks + 16 * d);

@@ -45,7 +45,7 @@ __global__ __launch_bounds__(256) void score_kernel(AttnParams a) {
     // Rows that see a key of the wave's: from the first at or past its first
     // key to the last whose window still reaches its last key.
     const int t1 = min(t0 + 16 * KT, sq.len) - 1;
-    int first = max(t0 - sq.p0, 0), last = sq.n - 1;
+    int first = min(max(t0 - sq.p0, 0), sq.n), last = sq.n - 1;
     if (a.window > 0 && t0 >= a.sinks) last = min(last, t1 - sq.p0 + a.window - 1);
     for (int r = first * G / 16 * 16; r <= last * G + G - 1; r += 16) {
         const int rr = r + n16;
