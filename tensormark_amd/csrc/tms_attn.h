@@ -60,7 +60,8 @@ struct AttnParams {
     int64_t ot, oh;
     int group, q_heads;
     int window, sinks;     // window 0: none
-    float scale;           // times log2(e): exponentials are taken to base 2
+    float scale;           // above 0, times log2(e): exponentials are taken to base 2
+    uint32_t qand, qxor;   // a query's bits are taken through these: a scale below 0 flips its sign, 0 clears it
     int split_tiles;       // key tiles a split has
     int splits;
     int row_tiles;
@@ -86,6 +87,19 @@ struct TileList {
     }
     __device__ __forceinline__ int key(int i) const { return (i < sink ? i : i - sink + lo) * KT; }
 };
+
+// The scale of a call, split into one above 0 and what becomes of the query:
+// masked scores are -inf before the scale and stay so.
+inline void set_scale(AttnParams& a, float scale) {
+    a.qand = scale == 0.f ? 0u : ~0u;
+    a.qxor = scale < 0.f ? 0x80008000u : 0u;
+    a.scale = scale == 0.f ? 1.f : (scale < 0.f ? -scale : scale) * kLog2e;
+}
+
+constexpr int kChunkRows = 128;   // of a workgroup of the chunk kernel
+inline int chunk_keys(int head_dim) { return head_dim > 128 ? 32 : 64; }   // of its tile
+constexpr float kSlack = 8.f;
+void launch_attn_chunk(const AttnParams& a, bool bf16, dim3 grid, hipStream_t stream);
 
 __device__ __forceinline__ bool sees(int j, int p, int window, int sinks) {
     return j <= p && (window <= 0 || j > p - window || j < sinks);

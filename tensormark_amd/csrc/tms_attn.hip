@@ -17,6 +17,7 @@
 #include <stddef.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "tms_attn.h"
 
@@ -64,7 +65,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnParams a) {
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int d = s * 32 + g4 * 8;
-            qf[rt][s] = in && d < D ? *(const u32x4*)(src + 2 * d) : (u32x4){0, 0, 0, 0};
+            qf[rt][s] = in && d < D ? (*(const u32x4*)(src + 2 * d) & a.qand) ^ a.qxor : (u32x4){0, 0, 0, 0};
         }
     }
 
@@ -384,7 +385,14 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams a, int rm) {
 
 // ---- host ---------------------------------------------------------------------------------------
 
+// The chunk kernel's offsets: a page's stride and what its slots span in 32
+// bits, and of 8 slots below 2^31.
+static bool short_strides(const tms_cache* c, const int64_t* stride) {
+    return 2 * stride[0] < (int64_t)1 << 32 && stride[2] < 1 << 26 && 2 * stride[2] * c->page_size < (int64_t)1 << 32;
+}
+
 struct AttnPlan {
+    bool chunk;        // the chunk kernel
     int rm;            // rows a workgroup
     int row_tiles;
     int tiles;         // most key tiles of a row tile
@@ -395,7 +403,7 @@ struct AttnPlan {
 static int check_attention(const tms_cache* c, const tms_attention_args* a) {
     const int rc = check_cache(c, true, true);
     if (rc != TMS_OK) return rc;
-    if (!a || a->q_heads < 1 || a->q_heads % c->kv_heads || a->sinks < 0 || !(a->scale == a->scale)) return TMS_ERR_INVALID_ARG;
+    if (!a || a->q_heads < 1 || a->q_heads % c->kv_heads || a->sinks < 0 || !std::isfinite(a->scale)) return TMS_ERR_INVALID_ARG;
     for (int i = 0; i < 2; ++i)
         if (a->q_stride[i] < 0 || a->q_stride[i] % 8 || a->out_stride[i] < 0 || a->out_stride[i] % 8) return TMS_ERR_INVALID_ARG;
     if ((int64_t)c->max_q * (a->q_heads / c->kv_heads) > (1 << 24)) return TMS_ERR_CAPACITY;
@@ -407,19 +415,27 @@ static int check_attention(const tms_cache* c, const tms_attention_args* a) {
 static AttnPlan plan_attention(const tms_cache* c, const tms_attention_args* a) {
     AttnPlan p;
     const int rows = min(c->max_q, c->tokens) * (a->q_heads / c->kv_heads);
+    p.chunk = rows > 64 && short_strides(c, c->k_stride) && short_strides(c, c->v_stride);
     const int rt = rows <= 16 || c->head_dim > 128 ? 1 : 2;
-    p.rm = 16 * rt;
+    p.rm = p.chunk ? kChunkRows : 16 * rt;
     p.row_tiles = (rows + p.rm - 1) / p.rm;
     int64_t keys = min(c->max_kv, kMaxLen);
-    if (a->window > 0) keys = std::min<int64_t>(keys, (int64_t)a->window + p.rm + a->sinks + 64);
-    p.tiles = (int)((keys + 31) / 32);
+    if (a->window > 0) keys = std::min<int64_t>(keys, (int64_t)a->window + p.rm + a->sinks + 128);
+    const int kt = p.chunk ? chunk_keys(c->head_dim) : 32;
+    p.tiles = (int)((keys + kt - 1) / kt);
     const int64_t items = (int64_t)c->batch * c->kv_heads * p.row_tiles;
+    if (p.chunk) {
+        // Workgroups enough for two a CU, with 16 tiles each at least.
+        const int64_t want = std::max<int64_t>(1, 512 / std::max<int64_t>(items, 1));
+        p.split_tiles = (int)std::max<int64_t>((p.tiles + want - 1) / want, 16);
+    } else {
     // Workgroups enough for four a CU, with 16 tiles each at least (four a wave).
     const int64_t want = std::max<int64_t>(1, 1024 / std::max<int64_t>(items, 1));
     int split = std::max<int64_t>((p.tiles + want - 1) / want, 16);
     if (split > 64) split = 64;
     if ((p.tiles + split - 1) / split > 256) split = (p.tiles + 255) / 256;
     p.split_tiles = (split + 3) / 4 * 4;
+    }
     p.splits = std::max(1, (p.tiles + p.split_tiles - 1) / p.split_tiles);
     const size_t parts = p.splits > 1 ? (size_t)items * p.splits * p.rm : 0;
     p.o_bytes = parts * c->head_dim * 4;
@@ -442,7 +458,8 @@ template <typename T>
 static void launch_attention(const AttnPlan& p, const AttnParams& a, hipStream_t stream) {
     const int D = a.c.head_dim;
     const dim3 grid(a.c.batch * a.c.kv_heads, p.row_tiles, p.splits);
-    if (D <= 64) launch_rows<T, 2, 4>(p, a, grid, stream);
+    if (p.chunk) launch_attn_chunk(a, std::is_same<T, Bf16>::value, grid, stream);
+    else if (D <= 64) launch_rows<T, 2, 4>(p, a, grid, stream);
     else if (D <= 96) launch_rows<T, 3, 8>(p, a, grid, stream);
     else if (D <= 128) launch_rows<T, 4, 8>(p, a, grid, stream);
     else launch_rows<T, 8, 16>(p, a, grid, stream);
@@ -483,7 +500,7 @@ extern "C" int tms_paged_attention(const tms_cache* cache, const tms_attention_a
     a.group = args->q_heads / cache->kv_heads;
     a.window = args->window > 0 && args->window < kMaxLen ? args->window : 0;
     a.sinks = std::min(args->sinks, kMaxLen);
-    a.scale = args->scale * kLog2e;
+    set_scale(a, args->scale);
     a.split_tiles = p.split_tiles;
     a.splits = p.splits;
     a.row_tiles = p.row_tiles;

@@ -1,0 +1,332 @@
+// tms_attn_chunk.hip -- attention over the paged cache for many rows a key
+// head: chunks of a prompt, long drafts (tms_paged_attention).
+//
+// The same mathematics as tms_attn.hip's: S^T = K Q^T, weights 2^(s - m), O^T
+// = V^T P^T, m and the sum of weights running per row.  128 rows of one key
+// head a workgroup, 32 a wave, on 32x32x16 instructions; a tile of 64 keys and
+// values goes to LDS once for the four waves.
+#include <type_traits>
+
+#include "tms_attn.h"
+
+namespace tms {
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+// A tile lies in LDS by rows of `ROWB` bytes, a key's (value's) 16-byte pieces
+// permuted within its row so that the reads of the matrix operands fall on
+// different banks: the key operand takes one piece of 32 rows, the value
+// operand (transposed on the way, ds_read_b64_tr_b16) 64 bytes of 4 rows.
+template <int ROWB> __device__ __forceinline__ int key_swizzle(int row) { return ROWB == 128 ? row >> 1 & 7 : row & 15; }
+template <int ROWB> __device__ __forceinline__ int value_swizzle(int row) { return ROWB == 128 ? (row >> 1 & 1) << 2 : (row & 3) << 2; }
+
+// 16 bytes a lane from `off` of the resource to LDS at `lds` (wave-uniform) +
+// 16 * lane; zeros where the resource ends before.  Counted by vmcnt only:
+// the loop waits for it, the compiler does not know of it.
+__device__ __forceinline__ void load_lds16(u32x4 rsrc, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc) : "memory");
+}
+
+// The resource of the last + 1 slots at `p`, none of them where `last` < 0.
+__device__ __forceinline__ u32x4 slots_rsrc(const char* p, int last, uint32_t stride, int bytes) {
+    const uint64_t at = (uint64_t)p;
+    return (u32x4){(uint32_t)at, (uint32_t)(at >> 32) & 0xFFFF, last < 0 ? 0u : (uint32_t)(last * stride + bytes), 0x00020000u};
+}
+
+template <typename T, int ROWB, int KS, int DT, int NK>
+__global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(AttnParams a) {
+    constexpr int KT = 32 * NK, RM = kChunkRows;
+    constexpr int C = ROWB / 16, RPI = 64 / C, NI = KT / (4 * RPI);   // pieces a row; rows a load; loads a wave
+    constexpr uint32_t ALL = (1u << KT / 8) - 1;
+    __shared__ __attribute__((aligned(128))) char sm[2][2][KT * ROWB];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n32 = lane & 31, hh = lane >> 5;
+    const int pair = blockIdx.x, tile = a.row_tiles - 1 - blockIdx.y, split = blockIdx.z;
+    const int b = pair / a.c.kv_heads, h = pair - b * a.c.kv_heads;
+    const SeqView sq = seq_view(a.c, b);
+    const int G = a.group, rows = sq.n * G, r0 = tile * RM;
+    if (r0 >= rows) return;
+    const int D = a.c.head_dim;
+    const int gfirst = sq.p0 + r0 / G, glast = sq.p0 + (min(r0 + RM, rows) - 1) / G;   // positions of the workgroup's rows
+    const TileList<KT> tl(a.window, a.sinks, gfirst, glast, sq.len);
+    const int v0 = split * a.split_tiles, v1 = a.splits == split + 1 ? tl.n : min(tl.n, v0 + a.split_tiles);
+
+    // The wave's rows, and the lane's: its query and its position.
+    const int w0 = r0 + wave * 32, r = w0 + n32;
+    const bool in = r < rows;
+    const int pfirst = sq.p0 + w0 / G, plast = w0 < rows ? sq.p0 + (min(w0 + 32, rows) - 1) / G : -1;
+    const int tok = in ? r / G : 0, hd = in ? r - tok * G : 0;
+    const int pos = in ? sq.p0 + tok : -1;
+    u32x4 qf[KS];
+    {
+        const char* src = a.q + (int64_t)(sq.q0 + tok) * a.qt + (int64_t)(h * G + hd) * a.qh;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = s * 16 + hh * 8;
+            qf[s] = in && d < D ? (*(const u32x4*)(src + 2 * d) & a.qand) ^ a.qxor : (u32x4){0, 0, 0, 0};
+        }
+    }
+
+    // Loads into LDS: an instruction moves 64 pieces, RPI whole rows, of 8
+    // keys that share a resource.  That ends with the last of them that exists,
+    // and a page that does not has none: what lies past is written as zeros,
+    // and so are the pieces past head_dim.
+    const int32_t* row = a.c.tables + (int64_t)b * a.c.tstride;
+    const char* kbase = a.c.k + (int64_t)h * a.c.kh;
+    const char* vbase = a.c.v + (int64_t)h * a.c.vh;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)&sm[0][0][0];
+    const uint32_t kslot = (uint32_t)a.c.ks, vslot = (uint32_t)a.c.vs, kpage = (uint32_t)a.c.kp, vpage = (uint32_t)a.c.vp;
+    uint32_t koff[NI], voff[NI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        const int rr = (wave * NI + i) * RPI + lane / C, lc = lane % C;
+        const int ck = lc ^ key_swizzle<ROWB>(rr), cv = lc ^ value_swizzle<ROWB>(rr);
+        koff[i] = ck * 8 < D ? (rr & 7) * kslot + ck * 16 : 0x80000000u;
+        voff[i] = cv * 8 < D ? (rr & 7) * vslot + cv * 16 : 0x80000000u;
+    }
+    // Table entries of the tile's groups of 8 keys, a lane each; -1 past the end.
+    auto entries = [&](int v) {
+        const int j = tl.key(v) + 8 * (lane & 7);
+        return (unsigned)j < (unsigned)sq.len ? row[j >> a.c.shift] : -1;
+    };
+    auto load = [&](int v, int buf, int pg) {
+        const int t0 = tl.key(v);
+#pragma unroll
+        for (int g = 0; g < NI * RPI / 8; ++g) {
+            const int at = wave * NI * RPI + 8 * g, j = t0 + at;
+            const uint32_t entry = __builtin_amdgcn_readlane(pg, at / 8);
+            const bool ok = entry < (uint32_t)a.c.pages;
+            const uint32_t page = ok ? entry : 0, slot = ok ? j & a.c.smask : 0;
+            const int last = ok ? min(8, sq.len - j) - 1 : -1;
+            const u32x4 kres = slots_rsrc(kbase + (uint64_t)page * kpage + slot * kslot, last, kslot, 2 * D);
+            const u32x4 vres = slots_rsrc(vbase + (uint64_t)page * vpage + slot * vslot, last, vslot, 2 * D);
+#pragma unroll
+            for (int i = g * 8 / RPI; i < (g + 1) * 8 / RPI; ++i) {
+                const uint32_t to = lds0 + buf * 2 * KT * ROWB + (wave * NI + i) * RPI * ROWB;
+                load_lds16(kres, koff[i], to);
+                load_lds16(vres, voff[i], to + KT * ROWB);
+            }
+        }
+    };
+
+    f32x16 o[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
+    float m = -__builtin_huge_valf(), l = 0.f;
+
+    // One tile.  EDGE: some row of the workgroup does not see all of it.
+    auto step = [&](auto edge, int t0, int buf, uint32_t there) __attribute__((always_inline)) {
+        constexpr bool EDGE = decltype(edge)::value;
+        const char* sk = sm[buf][0];
+        char* sv = sm[buf][1];
+        bool odd = false;
+        if constexpr (EDGE) {
+            // Some row has a weight of zero: does the tile hold an infinity or NaN?
+#pragma unroll
+            for (int i = 0; i < KT * ROWB / 1024; ++i) {
+                const u32x4 x = *(const u32x4*)(sv + i * 1024 + lane * 16);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) odd |= (x[w] & T::kExp) == T::kExp || (x[w] >> 16 & T::kExp) == T::kExp;
+            }
+            odd = __any(odd);
+            const bool none = t0 > plast || (a.window > 0 && t0 + KT <= pfirst - a.window + 1 && t0 >= a.sinks);
+            if (none && !odd) return;
+        }
+        f32x16 s[NK];
+#pragma unroll
+        for (int kt = 0; kt < NK; ++kt) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[kt][i] = 0.f;
+            const int key = kt * 32 + n32;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const u32x4 kf = *(const u32x4*)(sk + key * ROWB + 16 * ((2 * ks + hh) ^ key_swizzle<ROWB>(key)));
+                s[kt] = T::mfma32(kf, qf[ks], s[kt]);
+            }
+        }
+        if constexpr (EDGE) {
+#pragma unroll
+            for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int j = t0 + 32 * kt + 8 * (i / 4) + 4 * hh + (i & 3);
+                    const bool on = (there >> (4 * kt + i / 4) & 1) && j < sq.len && sees(j, pos, a.window, a.sinks);
+                    s[kt][i] = on ? s[kt][i] : -__builtin_huge_valf();
+                }
+        }
+        float top = -__builtin_huge_valf();
+#pragma unroll
+        for (int e = 0; e < 16 * NK; ++e) top = fmaxf(top, s[e / 16][e % 16]);
+        top *= a.scale;
+        // The reference point follows the maximum once some row's has grown by
+        // 2^kSlack: weights stay below that, which neither type minds.
+        if (__any(top > m + kSlack)) {
+            top = fmaxf(top, __shfl_xor(top, 32));
+            top = fmaxf(top, m);
+            const float f = __builtin_amdgcn_exp2f(m - (top == -__builtin_huge_valf() ? 0.f : top));
+            m = top;
+            l *= f;
+#pragma unroll
+            for (int t = 0; t < DT; ++t) o[t] *= f;
+        }
+        const float base = m == -__builtin_huge_valf() ? 0.f : m;
+        u32x4 pf[2 * NK];
+#pragma unroll
+        for (int e = 0; e < 16 * NK; ++e) {
+            const float x = __builtin_amdgcn_exp2f(fmaf(s[e / 16][e % 16], a.scale, -base));
+            s[e / 16][e % 16] = x;
+            l += x;
+        }
+#pragma unroll
+        for (int t = 0; t < 2 * NK; ++t)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) pf[t][w] = T::pack(s[t / 2][8 * (t & 1) + 2 * w], s[t / 2][8 * (t & 1) + 2 * w + 1]);
+
+        if constexpr (EDGE) {
+            // A weight of zero times an infinity or NaN would reach rows that
+            // do not see the value: such values go, key by key, to the rows whose
+            // weight is not zero, and are zero in the product.
+            if (odd) {
+#pragma unroll 1
+                for (int e = 0; e < 16 * NK; ++e) {
+                    float x = s[0][0];
+#pragma unroll
+                    for (int q = 1; q < 16 * NK; ++q) x = e == q ? s[q / 16][q % 16] : x;
+                    const float y = __shfl_xor(x, 32);
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) {
+                        const float w = hh == half ? x : y;
+                        const int key = 32 * (e / 16) + 8 * (e % 16 / 4) + 4 * half + (e & 3);
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                const u32x2 val =
+                                    *(const u32x2*)(sv + key * ROWB + 16 * ((4 * dt + c) ^ value_swizzle<ROWB>(key)) + 8 * hh);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const uint32_t bits = val[i / 2] >> 16 * (i & 1) & 0xFFFF;
+                                    if (w != 0.f && (bits & T::kExp) == T::kExp) o[dt][4 * c + i] = fmaf(w, T::up(bits), o[dt][4 * c + i]);
+                                }
+                            }
+                    }
+                }
+                __syncthreads();
+                for (int i = threadIdx.x; i < KT * ROWB / 16; i += 256) {
+                    u32x4 x = *(const u32x4*)(sv + 16 * i);
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        if ((x[w] & T::kExp) == T::kExp) x[w] &= 0xFFFF0000u;
+                        if ((x[w] >> 16 & T::kExp) == T::kExp) x[w] &= 0x0000FFFFu;
+                    }
+                    *(u32x4*)(sv + 16 * i) = x;
+                }
+                __syncthreads();
+            }
+        }
+
+        // Value operand: the lane's value column, keys 16t + 4hh + 0..3 and 8 more on.
+        const int q16 = lane & 15, colg = lane >> 4 & 1;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int t = 0; t < 2 * NK; ++t) {
+                u32x4 vf;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int key = 16 * t + 8 * u + 4 * hh + (q16 >> 2);
+                    const int ch = 4 * dt + 2 * colg + (q16 >> 1 & 1);
+                    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (lds_s16x4*)(sv + key * ROWB + 16 * (ch ^ value_swizzle<ROWB>(key)) + 8 * (q16 & 1)));
+                    const u32x2 y = __builtin_bit_cast(u32x2, x);
+                    vf[2 * u] = y[0];
+                    vf[2 * u + 1] = y[1];
+                }
+                o[dt] = T::mfma32(vf, pf[t], o[dt]);
+            }
+    };
+
+    int pg = v0 < v1 ? entries(v0) : -1, ahead = v0 + 1 < v1 ? entries(v0 + 1) : -1;
+    uint32_t there = (uint32_t)__ballot((unsigned)pg < (unsigned)a.c.pages) & ALL;
+    if (v0 < v1) load(v0, 0, pg);
+    int v = v0;
+    // Takes tile v when it has come: the wave's loads are in, and after the
+    // barrier all are and the other buffer is free for the next tile's.
+    uint32_t now = 0;
+    auto arrive = [&]() __attribute__((always_inline)) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        pg = ahead;
+        now = there;
+        there = (uint32_t)__ballot((unsigned)pg < (unsigned)a.c.pages) & ALL;
+        __syncthreads();
+        if (v + 1 < v1) load(v + 1, v + 1 - v0 & 1, pg);
+        if (v + 2 < v1) ahead = entries(v + 2);
+    };
+    auto is_edge = [&](int t0, uint32_t bits) {
+        return bits != ALL || t0 + KT > sq.len || t0 + KT - 1 > gfirst || (a.window > 0 && t0 <= glast - a.window && t0 + KT > a.sinks);
+    };
+    while (v < v1) {
+        while (v < v1 && !is_edge(tl.key(v), there)) {
+            arrive();
+            step(std::false_type(), tl.key(v), v - v0 & 1, now);
+            ++v;
+        }
+        while (v < v1 && is_edge(tl.key(v), there)) {
+            arrive();
+            step(std::true_type(), tl.key(v), v - v0 & 1, now);
+            ++v;
+        }
+    }
+    l += __shfl_xor(l, 32);
+    if (!in) return;
+
+    if (a.splits > 1) {
+        const int64_t at = (((int64_t)pair * a.row_tiles + tile) * a.splits + split) * RM + (r - r0);
+        if (hh == 0) {
+            a.part_ml[2 * at] = m;
+            a.part_ml[2 * at + 1] = l;
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int d = 32 * dt + 8 * c + 4 * hh;
+                if (d < D)
+                    *(f32x4*)(a.part_o + at * D + d) =
+                        (f32x4){o[dt][4 * c], o[dt][4 * c + 1], o[dt][4 * c + 2], o[dt][4 * c + 3]};
+            }
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;   // (a NaN sum stays one)
+    if (a.lse && hh == 0) a.lse[(int64_t)(sq.q0 + tok) * a.q_heads + h * G + hd] = (m + log2f(l)) * kLn2;
+    char* dst = a.out + (int64_t)(sq.q0 + tok) * a.ot + (int64_t)(h * G + hd) * a.oh;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int d = 32 * dt + 8 * c + 4 * hh;
+            if (d < D)
+                *(u32x2*)(dst + 2 * d) = (u32x2){T::pack(o[dt][4 * c] * inv, o[dt][4 * c + 1] * inv),
+                                                 T::pack(o[dt][4 * c + 2] * inv, o[dt][4 * c + 3] * inv)};
+        }
+}
+
+template <typename T>
+static void launch_chunk_type(const AttnParams& a, dim3 grid, hipStream_t stream) {
+    const int D = a.c.head_dim;
+    if (D <= 64) hipLaunchKernelGGL((attn_chunk_kernel<T, 128, 4, 2, 2>), grid, dim3(256), 0, stream, a);
+    else if (D <= 96) hipLaunchKernelGGL((attn_chunk_kernel<T, 256, 6, 3, 2>), grid, dim3(256), 0, stream, a);
+    else if (D <= 128) hipLaunchKernelGGL((attn_chunk_kernel<T, 256, 8, 4, 2>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((attn_chunk_kernel<T, 512, 16, 8, 1>), grid, dim3(256), 0, stream, a);
+}
+
+void launch_attn_chunk(const AttnParams& a, bool bf16, dim3 grid, hipStream_t stream) {
+    if (bf16) launch_chunk_type<Bf16>(a, grid, stream);
+    else launch_chunk_type<F16>(a, grid, stream);
+}
+
+}  // namespace tms

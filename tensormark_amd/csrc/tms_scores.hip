@@ -4,6 +4,7 @@
 // between workgroups: a wave keeps its keys in registers and passes over the
 // rows that see them, so a key's sum is one lane group's, in row order.
 #include <algorithm>
+#include <cmath>
 
 #include "tms_attn.h"
 
@@ -59,7 +60,7 @@ __global__ __launch_bounds__(256) void score_kernel(AttnParams a) {
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int d = s * 32 + g4 * 8;
-            qf[s] = in && d < D ? *(const u32x4*)(src + 2 * d) : (u32x4){0, 0, 0, 0};
+            qf[s] = in && d < D ? (*(const u32x4*)(src + 2 * d) & a.qand) ^ a.qxor : (u32x4){0, 0, 0, 0};
         }
         const int pfirst = sq.p0 + r / G, plast = sq.p0 + (r + 15) / G;
         const bool edge = r + 15 >= rows || t0 + 16 * KT - 1 > pfirst ||
@@ -119,7 +120,7 @@ extern "C" int tms_kv_add_scores(const tms_cache* cache, const tms_score_args* a
     const int rc = check_cache(cache, false, true);
     if (rc != TMS_OK) return rc;
     if (!args || !cache->scores || args->q_heads < 1 || args->q_heads % cache->kv_heads || args->sinks < 0 ||
-        !(args->scale == args->scale) || args->q_stride[0] < 0 || args->q_stride[0] % 8 || args->q_stride[1] < 0 ||
+        !std::isfinite(args->scale) || args->q_stride[0] < 0 || args->q_stride[0] % 8 || args->q_stride[1] < 0 ||
         args->q_stride[1] % 8 || ((uintptr_t)args->out & 15) || ((uintptr_t)args->lse & 3))
         return TMS_ERR_INVALID_ARG;
     if (cache->max_kv > 4 * 1024 * 1024 || (int64_t)cache->max_q * (args->q_heads / cache->kv_heads) > (1 << 24))
@@ -137,7 +138,7 @@ extern "C" int tms_kv_add_scores(const tms_cache* cache, const tms_score_args* a
     a.group = args->q_heads / cache->kv_heads;
     a.window = args->window > 0 && args->window < kMaxLen ? args->window : 0;
     a.sinks = std::min(args->sinks, kMaxLen);
-    a.scale = args->scale * kLog2e;
+    set_scale(a, args->scale);
     if (cache->dtype == TMS_DTYPE_BF16) launch_scores<Bf16>(a, cache->max_kv, cache->max_q, stream);
     else launch_scores<F16>(a, cache->max_kv, cache->max_q, stream);
     return hipGetLastError() == hipSuccess ? TMS_OK : TMS_ERR_HIP;
