@@ -62,11 +62,12 @@ struct AttnParams {
     int window, sinks;     // window 0: none
     float scale;           // above 0, times log2(e): exponentials are taken to base 2
     uint32_t qand, qxor;   // a query's bits are taken through these: a scale below 0 flips its sign, 0 clears it
-    int split_tiles;       // key tiles a split has
-    int splits;
+    int split_tiles;       // chunk kernel: key tiles a split has; rows kernel: the least that a share has
+    int splits;            // chunk kernel
     int row_tiles;
-    float* part_o;         // [pairs * row_tiles][splits][rows a tile][head_dim]
-    float* part_ml;        // [pairs * row_tiles][splits][rows a tile][2]: maximum, sum
+    float* part_o;         // parts of rows, [part][rows a tile][head_dim]
+    float* part_ml;        // [part][rows a tile][2]: maximum, sum
+    int2* item_parts;      // rows kernel, [pairs * row_tiles]: the first share and the number of shares with a part
 };
 
 // The key tiles of `KT` keys that the rows at positions [pmin, pmax] see, as
@@ -87,6 +88,67 @@ struct TileList {
     }
     __device__ __forceinline__ int key(int i) const { return (i < sink ? i : i - sink + lo) * KT; }
 };
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+// A tile lies in LDS by rows of `ROWB` bytes, a key's (value's) 16-byte pieces
+// permuted within its row so that the reads of the matrix operands fall on
+// different banks: the key operand takes one piece of 32 rows, the value
+// operand (transposed on the way, ds_read_b64_tr_b16) 64 bytes of 4 rows.
+template <int ROWB> __device__ __forceinline__ int key_swizzle(int row) { return ROWB == 128 ? row >> 1 & 7 : row & 15; }
+template <int ROWB> __device__ __forceinline__ int value_swizzle(int row) { return ROWB == 128 ? (row >> 1 & 1) << 2 : (row & 3) << 2; }
+
+// 16 bytes a lane from `off` of the resource to LDS at `lds` (wave-uniform) +
+// 16 * lane; zeros where the resource ends before.  Counted by vmcnt only:
+// the loop waits for it, the compiler does not know of it.  (A wait state
+// lies between m0's write and the load that reads it.)
+__device__ __forceinline__ void load_lds16(u32x4 rsrc, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc) : "memory");
+}
+
+// The resource of the last + 1 slots at `p`, none of them where `last` < 0.
+__device__ __forceinline__ u32x4 slots_rsrc(const char* p, int last, uint32_t stride, int bytes) {
+    const uint64_t at = (uint64_t)p;
+    return (u32x4){(uint32_t)at, (uint32_t)(at >> 32) & 0xFFFF, last < 0 ? 0u : (uint32_t)(last * stride + bytes), 0x00020000u};
+}
+
+// A row's 8 values from dimension d on as the operand of the scores, zeros
+// past head_dim and for a row that is none (`src` is some row in any case:
+// loads without a branch between them are in flight together).
+__device__ __forceinline__ u32x4 query_operand(const AttnParams& a, const char* src, int d, bool in) {
+    const bool is = in && d < a.c.head_dim;
+    const u32x4 x = *(const u32x4*)(src + 2 * (d < a.c.head_dim ? d : 0));
+    u32x4 y;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) y[w] = is ? (x[w] & a.qand) ^ a.qxor : 0u;
+    return y;
+}
+
+// The operand of S^T = K Q^T: 32 keys from `tile` on, dimensions 16 ks...
+template <int ROWB> __device__ __forceinline__ u32x4 key_operand(const char* sk, int lane, int tile, int ks) {
+    const int key = tile * 32 + (lane & 31);
+    return *(const u32x4*)(sk + key * ROWB + 16 * ((2 * ks + (lane >> 5)) ^ key_swizzle<ROWB>(key)));
+}
+
+// The operand of O^T = V^T P^T: value columns 32 dt..., the keys of weights
+// 8 t .. 8 t + 7 of a lane, which are 16 t + 4 (lane / 32) + 0..3 and 8 more on.
+template <int ROWB> __device__ __forceinline__ u32x4 value_operand(const char* sv, int lane, int dt, int t) {
+    const int q16 = lane & 15;
+    u32x4 vf;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int key = 16 * t + 8 * u + 4 * (lane >> 5) + (q16 >> 2);
+        const int piece = 4 * dt + 2 * (lane >> 4 & 1) + (q16 >> 1 & 1);
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_s16x4*)(sv + key * ROWB + 16 * (piece ^ value_swizzle<ROWB>(key)) + 8 * (q16 & 1)));
+        const u32x2 y = __builtin_bit_cast(u32x2, x);
+        vf[2 * u] = y[0];
+        vf[2 * u + 1] = y[1];
+    }
+    return vf;
+}
 
 // The scale of a call, split into one above 0 and what becomes of the query:
 // masked scores are -inf before the scale and stay so.

@@ -10,7 +10,7 @@
 //
 // Both products are matrix instructions on transposed tiles: S^T = K Q^T and
 // O^T = V^T P^T.  A lane then holds one row's scores for several keys (row =
-// lane % 16): the softmax needs no exchange but two shuffles for a maximum,
+// lane % 32): the softmax needs no exchange but one shuffle for a maximum,
 // and the weights are already where the second product wants its right
 // operand, since the order of its inner index (the keys) is free as long as
 // V^T's is the same.
@@ -18,338 +18,385 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "tms_attn.h"
 
 namespace tms {
 
-// ---- few rows: keys spread over waves ------------------------------------------------------------
+// ---- few rows: the keys of all sequences in equal shares ---------------------------------------
 //
-// 16 * RT rows of one key head a workgroup.  Its four waves take the key
-// tiles (32 keys) of the workgroup's split in turn, each with its own running
-// maximum and sum, and join at the end.  Keys and values go from memory to
-// registers, in the matrix instructions' layout, without LDS: nothing is
-// shared between the waves.  A lane reads 16 bytes of a key (lane % 16 the
-// key, 64 bytes of a row together), and 8 values' rows at the 16 bytes
-// lane % 16; v_perm pairs those rows' halves into the left operand, one
-// instruction for two values.  Value row piece `c` of 8 then is rows
-// {8c + t} of O^T in its tile t, so a lane ends with 8 neighbouring values of
-// its row.
-template <typename T, int KS, int VB, int RT>
-__global__ __launch_bounds__(256) void attn_rows_kernel(AttnParams a) {
-    constexpr int RM = 16 * RT, VP = VB / 8 ? VB / 8 : 1, VW = VB >= 8 ? 4 : 2;   // pieces, words a piece
-    __shared__ float sm_o[2][VB * RT * 4 * 64];
-    __shared__ float sm_m[2][RM], sm_l[2][RM];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int n16 = lane & 15, g4 = lane >> 4;
-    const int pair = blockIdx.x, tile = blockIdx.y, split = blockIdx.z;
-    const int b = pair / a.c.kv_heads, h = pair - b * a.c.kv_heads;
+// Bound by memory: the keys and values of a call are read once.  All items
+// (sequence, row tile, key head) lie behind each other on one axis of key
+// tiles, and each workgroup takes an equal share of it, whatever the lengths;
+// an item that its share holds whole is written out, the two at its ends go
+// to the workspace as parts, which a second launch joins.
+//
+// Within an item the four waves take the tiles (32 keys) in turn, each with
+// its own running maximum and sum and its own piece of LDS: a tile's keys are
+// loaded there while the values of the one before are used, and its values
+// while its keys are, so that 8 waves a CU keep some 100 KB on the way without
+// a register for it.  No wave waits for another before the item's end.
+template <int RM>
+__device__ __forceinline__ int item_tiles(const AttnParams& a, int combo) {
+    const int b = combo / a.row_tiles, tile = combo - b * a.row_tiles;
     const SeqView sq = seq_view(a.c, b);
     const int G = a.group, rows = sq.n * G, r0 = tile * RM;
-    if (r0 >= rows) return;
-    const int D = a.c.head_dim;
-    const int rlast = min(r0 + RM, rows) - 1;
-    const TileList<32> tl(a.window, a.sinks, sq.p0 + r0 / G, sq.p0 + rlast / G, sq.len);
-    const int v0 = split * a.split_tiles, v1 = a.splits == split + 1 ? tl.n : min(tl.n, v0 + a.split_tiles);
+    if (r0 >= rows) return 0;
+    // (rows that see nothing have an output all the same)
+    return max(TileList<32>(a.window, a.sinks, sq.p0 + r0 / G, sq.p0 + (min(r0 + RM, rows) - 1) / G, sq.len).n, 1);
+}
 
-    // This lane's row of each 16: its query and its position.
-    u32x4 qf[RT][KS];
-    int pos[RT];
+__device__ __forceinline__ int64_t share_of(const AttnParams& a, int64_t total, int shares) {
+    return max((total + shares - 1) / shares, (int64_t)a.split_tiles);
+}
+
+template <typename T, int ROWB, int KS, int DT, int RT>
+__global__ __launch_bounds__(256, ROWB > 256 || (ROWB > 128 && RT > 1) ? 1 : 2) void attn_rows_kernel(AttnParams a) {
+    constexpr int RM = 32 * RT, KT = 32, NL = KT * ROWB / 1024, RPI = 1024 / ROWB, PAD = 33;
+    constexpr int MERGE = 4 * DT * 32 * PAD * 4, RING = 4 * 2 * KT * ROWB;
+    __shared__ __attribute__((aligned(128))) char sm[MERGE > RING ? MERGE : RING];
+    __shared__ float sm_ml[RT][4][32][2];
+    __shared__ int64_t wsum[4], start_at;
+    __shared__ int start_combo;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int n32 = lane & 31, hh = lane >> 5;
+    const int H = a.c.kv_heads, G = a.group, D = a.c.head_dim;
+    const int combos = a.c.batch * a.row_tiles;
+
+    // The share: [x, end) of the axis, which starts in `combo` (a sequence's
+    // row tile, all key heads one after another) at `at`.
+    const int per = (combos + 255) / 256, c0 = min(t * per, combos), c1 = min(c0 + per, combos);
+    int64_t mine = 0;
+    for (int c = c0; c < c1; ++c) mine += item_tiles<RM>(a, c);
+    int64_t upto = mine;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int r = r0 + rt * 16 + n16;
-        const bool in = r < rows;
-        const int tok = in ? r / G : 0, hd = in ? r - tok * G : 0;
-        pos[rt] = in ? sq.p0 + tok : -1;
-        const char* src = a.q + (int64_t)(sq.q0 + tok) * a.qt + (int64_t)(h * G + hd) * a.qh;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const int d = s * 32 + g4 * 8;
-            qf[rt][s] = in && d < D ? (*(const u32x4*)(src + 2 * d) & a.qand) ^ a.qxor : (u32x4){0, 0, 0, 0};
-        }
+    for (int d = 1; d < 64; d <<= 1) {
+        const int64_t y = __shfl_up(upto, d);
+        if (lane >= d) upto += y;
     }
-
-    const int32_t* row = a.c.tables + (int64_t)b * a.c.tstride;
-    const char* kbase = a.c.k + (int64_t)h * a.c.kh;
-    const char* vbase = a.c.v + (int64_t)h * a.c.vh;
-    u32x4 kr[2][KS];
-    uint32_t vr[2][4][VP][VW];
-    int kp[2], vp[2];
-
-    auto pages = [&](int v) {
-        const int t0 = tl.key(v);
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-            kp[kt] = page_of(a.c, row, t0 + 16 * kt + n16, sq.len);
-            vp[kt] = page_of(a.c, row, t0 + 16 * kt + 4 * g4, sq.len);
-        }
-    };
-    // A key that does not exist is read from the first slot of the pool, and masked.
-    auto load_k = [&](int v) {
-        const int t0 = tl.key(v);
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-            const int j = t0 + 16 * kt + n16;
-            const char* src = kbase + (kp[kt] < 0 ? 0 : (int64_t)kp[kt] * a.c.kp + (int64_t)(j & a.c.smask) * a.c.ks);
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                const int d = s * 32 + g4 * 8;
-                kr[kt][s] = d < D ? *(const u32x4*)(src + 2 * d) : (u32x4){0, 0, 0, 0};
+    if (lane == 63) wsum[wave] = upto;
+    __syncthreads();
+    int64_t total = 0, before = upto - mine;
+    for (int w = 0; w < 4; ++w) {
+        before += w < wave ? wsum[w] : 0;
+        total += wsum[w];
+    }
+    const int64_t share = share_of(a, total * H, gridDim.x);
+    int64_t x = blockIdx.x * share;
+    const int64_t end = min(x + share, total * H);
+    if (x >= end) return;
+    if (x >= before * H && x < (before + mine) * H)
+        for (int c = c0;; ++c) {
+            const int n = item_tiles<RM>(a, c);
+            if (x < (before + n) * H) {
+                start_combo = c;
+                start_at = before * H;
+                break;
             }
+            before += n;
         }
-    };
-    auto load_v = [&](int v) {
-        const int t0 = tl.key(v);
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-            const int j = (t0 + 16 * kt + 4 * g4) & a.c.smask;
-            const char* src = vbase + (vp[kt] < 0 ? 0 : (int64_t)vp[kt] * a.c.vp + (int64_t)j * a.c.vs);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int p = 0; p < VP; ++p) {
-                    const int d = p * 128 + n16 * (2 * VW);
-                    const char* at = src + (vp[kt] < 0 ? 0 : i * a.c.vs) + 2 * (d < D ? d : 0);
-                    if constexpr (VW == 4) {
-                        const u32x4 x = *(const u32x4*)at;
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) vr[kt][i][p][w] = x[w];
-                    } else {
-                        const u32x2 x = *(const u32x2*)at;
-                        vr[kt][i][p][0] = x[0];
-                        vr[kt][i][p][1] = x[1];
-                    }
-                }
-        }
-    };
+    __syncthreads();
+    int combo = __builtin_amdgcn_readfirstlane(start_combo);
+    int64_t at = start_at;
 
-    f32x4 o[RT][VB];
-    float m[RT], l[RT];
+    char* ring = sm + wave * 2 * KT * ROWB;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)ring;
+    const uint32_t kslot = (uint32_t)a.c.ks, vslot = (uint32_t)a.c.vs;
+    uint32_t koff[NL], voff[NL];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        m[rt] = -__builtin_huge_valf();
-        l[rt] = 0.f;
-#pragma unroll
-        for (int t = 0; t < VB; ++t) o[rt][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < NL; ++i) {
+        const int rr = i * RPI + lane / (ROWB / 16), lc = lane % (ROWB / 16);
+        const int ck = lc ^ key_swizzle<ROWB>(rr), cv = lc ^ value_swizzle<ROWB>(rr);
+        koff[i] = ck * 8 < D ? (rr & 7) * kslot + ck * 16 : 0x80000000u;
+        voff[i] = cv * 8 < D ? (rr & 7) * vslot + cv * 16 : 0x80000000u;
     }
 
-    int v = v0 + wave;
-    if (v < v1) {
-        pages(v);
-        load_k(v);
-        load_v(v);
-    }
-    for (; v < v1; v += 4) {
-        const int t0 = tl.key(v);
-        // Which of this lane's 8 keys of S^T (and value rows) are there.
+    while (x < end) {
+        const int b = combo / a.row_tiles, tile = combo - b * a.row_tiles;
+        const SeqView sq = seq_view(a.c, b);
+        const int rows = sq.n * G, r0 = tile * RM;
+        if (r0 >= rows) {
+            ++combo;
+            continue;
+        }
+        const int nr = min(RM, rows - r0);
+        const int pfirst = sq.p0 + r0 / G, plast = sq.p0 + (r0 + nr - 1) / G;
+        const TileList<KT> tl(a.window, a.sinks, pfirst, plast, sq.len);
+        const int n = max(tl.n, 1);
+        if (x >= at + (int64_t)n * H) {
+            at += (int64_t)n * H;
+            ++combo;
+            continue;
+        }
+        const int h = (int)((x - at) / n);
+        const int64_t item = at + (int64_t)h * n;
+        const int k0 = (int)(x - item), k1 = (int)min((int64_t)n, end - item), kend = min(k1, tl.n);
+
+        int pos[RT];
+        u32x4 qf[RT][KS];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const int r = r0 + 32 * rt + n32;
+            const bool in = r < rows;
+            const int tok = in ? r / G : 0, hd = in ? r - tok * G : 0;
+            pos[rt] = in ? sq.p0 + tok : -1;
+            const char* src = a.q + (int64_t)(sq.q0 + tok) * a.qt + (int64_t)(h * G + hd) * a.qh;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) qf[rt][s] = query_operand(a, src, s * 16 + hh * 8, in);
+        }
+        // Table entries of a tile's groups of 8 keys: by the scalar cache, whose
+        // counter the loads into LDS do not share.
+        typedef const __attribute__((address_space(4))) int32_t* scalar_ptr;
+        const scalar_ptr row = (scalar_ptr)(uintptr_t)(a.c.tables + (int64_t)b * a.c.tstride);
+        const char* kbase = a.c.k + (int64_t)h * a.c.kh;
+        const char* vbase = a.c.v + (int64_t)h * a.c.vh;
+        int page[4], next[4];
+        auto entries = [&](int v) __attribute__((always_inline)) {
+            const int t0 = tl.key(v);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) next[g] = row[min(t0 + 8 * g, sq.len - 1) >> a.c.shift];
+        };
+        auto take = [&](int v) __attribute__((always_inline)) {   // bit g: group g of 8 keys is there
+            const int t0 = tl.key(v);
+            uint32_t there = 0;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const bool ok = t0 + 8 * g < sq.len && (uint32_t)next[g] < (uint32_t)a.c.pages;
+                page[g] = ok ? next[g] : -1;
+                there |= ok ? 1u << g : 0u;
+            }
+            return there;
+        };
+        auto load = [&](int v, const char* base, int64_t pstride, uint32_t slot, const uint32_t* off, uint32_t to) __attribute__((always_inline)) {
+            const int t0 = tl.key(v);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int j = t0 + 8 * g;
+                const uint32_t p = max(page[g], 0), sl = page[g] < 0 ? 0 : j & a.c.smask;
+                const u32x4 res = slots_rsrc(base + p * pstride + (uint64_t)sl * slot, page[g] < 0 ? -1 : min(8, sq.len - j) - 1, slot, 2 * D);
+#pragma unroll
+                for (int i = g * 8 / RPI; i < (g + 1) * 8 / RPI; ++i) load_lds16(res, off[i], to + i * 1024);
+            }
+        };
+
+        f32x16 o[RT][DT];
+        float m[RT], l[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            m[rt] = -__builtin_huge_valf();
+            l[rt] = 0.f;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[rt][dt][i] = 0.f;
+        }
+        int v = k0 + wave;
         uint32_t there = 0;
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                there |= (uint32_t)(vp[kt] >= 0 && t0 + 16 * kt + 4 * g4 + i < sq.len) << (4 * kt + i);
-        const bool more = v + 4 < v1;
-        f32x4 s[RT][2];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-                s[rt][kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) s[rt][kt] = T::mfma16(kr[kt][ks], qf[rt][ks], s[rt][kt]);
-            }
-        int vpn[2];
-        if (more) {
-            vpn[0] = vp[0];
-            vpn[1] = vp[1];
-            pages(v + 4);
-            load_k(v + 4);
+        if (v < kend) {
+            entries(v);
+            there = take(v);
+            __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): what went before is not counted below
+            load(v, kbase, a.c.kp, kslot, koff, lds0);
+            load(v, vbase, a.c.vp, vslot, voff, lds0 + KT * ROWB);
+            if (v + 4 < kend) entries(v + 4);
         }
-        // A tile that some row sees in part: rows' own bounds, and values of
-        // keys that are not there set to zero.
-        const int pfirst = sq.p0 + r0 / G, plast = sq.p0 + rlast / G;
-        const bool edge = __any(there != 0xFF) || t0 + 31 > pfirst ||
-                          (a.window > 0 && t0 <= plast - a.window && t0 + 32 > a.sinks);
-        bool odd = false;   // a value that is no finite number in such a tile
-        if (edge) {
+        for (; v < kend; v += 4) {
+            const bool more = v + 4 < kend;
+            const int t0 = tl.key(v);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");   // the keys; the values may be on the way
+            f32x16 s[RT];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
+                for (int i = 0; i < 16; ++i) s[rt][i] = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int j = t0 + 16 * kt + 4 * g4 + i;
-                        const bool on = (there >> (4 * kt + i) & 1) && sees(j, pos[rt], a.window, a.sinks);
-                        s[rt][kt][i] = on ? s[rt][kt][i] : -__builtin_huge_valf();
-                    }
+            for (int ks = 0; ks < KS; ++ks) {
+                const u32x4 kf = key_operand<ROWB>(ring, lane, 0, ks);
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
+                for (int rt = 0; rt < RT; ++rt) s[rt] = T::mfma32(kf, qf[rt][ks], s[rt]);
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the keys are read: their place is free
+            const uint32_t now = there;
+            int pnow[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+            for (int g = 0; g < 4; ++g) pnow[g] = page[g];
+            if (more) {
+                there = take(v + 4);
+                load(v + 4, kbase, a.c.kp, kslot, koff, lds0);
+                if (v + 8 < kend) entries(v + 8);
+            }
+            const bool edge = now != 15 || t0 + KT > sq.len || t0 + KT - 1 > pfirst ||
+                              (a.window > 0 && t0 <= plast - a.window && t0 + KT > a.sinks);
+            if (edge) {
 #pragma unroll
-                    for (int p = 0; p < VP; ++p)
+                for (int i = 0; i < 16; ++i) {
+                    const int j = t0 + 8 * (i / 4) + 4 * hh + (i & 3);
+                    const bool is = (now >> (i / 4) & 1) && j < sq.len;
 #pragma unroll
-                        for (int w = 0; w < VW; ++w) {
-                            uint32_t& x = vr[kt][i][p][w];
-                            x = (there >> (4 * kt + i) & 1) ? x : 0u;
-                            odd |= (x & T::kExp) == T::kExp || (x >> 16 & T::kExp) == T::kExp;
+                    for (int rt = 0; rt < RT; ++rt)
+                        s[rt][i] = is && sees(j, pos[rt], a.window, a.sinks) ? s[rt][i] : -__builtin_huge_valf();
+                }
+            }
+            u32x4 pf[RT][2];
+            uint32_t some[RT];   // weights that are not zero, a bit each
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                float top = -__builtin_huge_valf();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) top = fmaxf(top, s[rt][e]);
+                top *= a.scale;
+                if (__any(top > m[rt] + kSlack)) {   // (as in the chunk kernel)
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    top = fmaxf(top, m[rt]);
+                    const float f = __builtin_amdgcn_exp2f(m[rt] - (top == -__builtin_huge_valf() ? 0.f : top));
+                    m[rt] = top;
+                    l[rt] *= f;
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= f;
+                }
+                const float base = m[rt] == -__builtin_huge_valf() ? 0.f : m[rt];
+                some[rt] = 0;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    s[rt][e] = __builtin_amdgcn_exp2f(fmaf(s[rt][e], a.scale, -base));
+                    l[rt] += s[rt][e];
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) pf[rt][u][w] = T::pack(s[rt][8 * u + 2 * w], s[rt][8 * u + 2 * w + 1]);
+                if (edge) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) some[rt] |= s[rt][e] != 0.f ? 1u << e : 0u;
+                }
+            }
+            if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");   // the values; the next keys may be on the way
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            char* sv = ring + KT * ROWB;
+            if (edge) {
+                // A weight of zero times an infinity or NaN would reach rows that
+                // do not see the value: such values go, key by key, to the rows
+                // whose weight is not zero (which weight does not matter), and are
+                // zero in the product.
+                bool odd = false;
+#pragma unroll
+                for (int i = 0; i < NL; ++i) {
+                    const u32x4 y = *(const u32x4*)(sv + i * 1024 + lane * 16);
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) odd |= (y[w] & T::kExp) == T::kExp || (y[w] >> 16 & T::kExp) == T::kExp;
+                }
+                if (__any(odd)) {
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        const uint32_t other = __shfl_xor(some[rt], 32);
+#pragma unroll 1
+                        for (int key = 0; key < KT; ++key) {
+                            const uint32_t w = (key >> 2 & 1) == hh ? some[rt] : other;
+                            if (!(w >> (key / 8 * 4 + (key & 3)) & 1)) continue;
+#pragma unroll
+                            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                                for (int c = 0; c < 4; ++c) {
+                                    const u32x2 val = *(const u32x2*)(sv + key * ROWB + 16 * ((4 * dt + c) ^ value_swizzle<ROWB>(key)) + 8 * hh);
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) {
+                                        const uint32_t bits = val[i / 2] >> 16 * (i & 1) & 0xFFFF;
+                                        o[rt][dt][4 * c + i] += (bits & T::kExp) == T::kExp ? T::up(bits) : 0.f;
+                                    }
+                                }
                         }
-            odd = __any(odd);
+                    }
+#pragma unroll 1
+                    for (int i = 0; i < NL; ++i) {
+                        u32x4 y = *(const u32x4*)(sv + i * 1024 + lane * 16);
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            if ((y[w] & T::kExp) == T::kExp) y[w] &= 0xFFFF0000u;
+                            if ((y[w] >> 16 & T::kExp) == T::kExp) y[w] &= 0x0000FFFFu;
+                        }
+                        *(u32x4*)(sv + i * 1024 + lane * 16) = y;
+                    }
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                }
+            }
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const u32x4 vf = value_operand<ROWB>(sv, lane, dt, u);
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) o[rt][dt] = T::mfma32(vf, pf[rt][u], o[rt][dt]);
+                }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (more) load(v + 4, vbase, a.c.vp, vslot, voff, lds0 + KT * ROWB);
         }
-        u32x4 pb[RT];
-        float pw[RT][8];
+
+        // The four waves' shares of the item's rows, by way of LDS: 32 rows a
+        // pass, row by row contiguous in a wave's array [dimension][row].
+        const bool whole = k0 == 0 && k1 == n;
+        const int64_t part = 2 * (int64_t)blockIdx.x + (k0 == 0 ? 1 : 0);
+        const int item_id = combo * H + h;
+        if (k0 == 0 && t == 0 && a.item_parts)
+            a.item_parts[item_id] = make_int2(blockIdx.x, whole ? 0 : (int)((item + n - 1) / share) - (int)blockIdx.x + 1);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            float x[8], top = -__builtin_huge_valf();
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[e] = s[rt][e >> 2][e & 3] * a.scale;
-                top = fmaxf(top, x[e]);
+            l[rt] += __shfl_xor(l[rt], 32);
+            __syncthreads();
+            if (hh == 0) {
+                sm_ml[rt][wave][n32][0] = m[rt];
+                sm_ml[rt][wave][n32][1] = l[rt];
             }
-            if (__any(top > m[rt])) {   // (most tiles leave every row's maximum where it was)
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                top = fmaxf(top, m[rt]);
-                const float f = __builtin_amdgcn_exp2f(m[rt] - (top == -__builtin_huge_valf() ? 0.f : top));
-                m[rt] = top;
-                l[rt] *= f;
+            float* to = (float*)sm + wave * DT * 32 * PAD;
 #pragma unroll
-                for (int t = 0; t < VB; ++t) o[rt][t] *= f;
-            }
-            const float base = m[rt] == -__builtin_huge_valf() ? 0.f : m[rt];
+            for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                pw[rt][e] = __builtin_amdgcn_exp2f(x[e] - base);
-                l[rt] += pw[rt][e];
-            }
+                for (int i = 0; i < 16; ++i) to[(32 * dt + 8 * (i / 4) + 4 * hh + (i & 3)) * PAD + n32] = o[rt][dt][i];
+            __syncthreads();
+            const int nrt = min(nr - 32 * rt, 32), quads = D / 4;
+            for (int e = t; e < nrt * quads; e += 256) {
+                const int rr = e / quads, d = 4 * (e - rr * quads), r = r0 + 32 * rt + rr;
+                float M = -__builtin_huge_valf(), L = 0.f;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) pb[rt][w] = T::pack(pw[rt][2 * w], pw[rt][2 * w + 1]);
-        }
-        if (!odd) {
+                for (int w = 0; w < 4; ++w) M = fmaxf(M, sm_ml[rt][w][rr][0]);
+                const float base = M == -__builtin_huge_valf() ? 0.f : M;
+                f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int t = 0; t < VB; ++t) {
-                const int p = t / 8, w = (t & 7) >> 1;
-                const uint32_t sel = t & 1 ? 0x07060302u : 0x05040100u;
-                u32x4 av;
+                for (int w = 0; w < 4; ++w) {
+                    const float f = __builtin_amdgcn_exp2f(sm_ml[rt][w][rr][0] - base), lw = sm_ml[rt][w][rr][1];
+                    if (lw == 0.f) continue;   // the wave's keys gave the row nothing
+                    L += lw * f;
+                    const float* from = (const float*)sm + (w * DT * 32 + d) * PAD + rr;
 #pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    av[x] = __builtin_amdgcn_perm(vr[x >> 1][2 * (x & 1) + 1][p][w], vr[x >> 1][2 * (x & 1)][p][w], sel);
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) o[rt][t] = T::mfma16(av, pb[rt], o[rt][t]);
-            }
-        } else {
-            // A weight of zero times an infinity or NaN would reach rows that
-            // do not see the key: key by key, only where the weight is not zero.
-            const int32_t vpc[2] = {more ? vpn[0] : vp[0], more ? vpn[1] : vp[1]};
-            for (int key = 0; key < 32; ++key) {
-                const int from = n16 + 16 * ((key & 15) >> 2);   // the lane that has this row's weight
-                const int page = __shfl(key < 16 ? vpc[0] : vpc[1], from);
-                const char* src = vbase + (int64_t)max(page, 0) * a.c.vp + (int64_t)((t0 + key) & a.c.smask) * a.c.vs;
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    float w = 0.f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float x = __shfl(pw[rt][e], from);
-                        if (e == (key >> 4) * 4 + (key & 3)) w = x;
+                    for (int i = 0; i < 4; ++i) acc[i] += from[i * PAD] * f;
+                }
+                if (!whole) {
+                    const int64_t to_row = part * RM + 32 * rt + rr;
+                    *(f32x4*)(a.part_o + to_row * D + d) = acc;
+                    if (d == 0) {
+                        a.part_ml[2 * to_row] = M;
+                        a.part_ml[2 * to_row + 1] = L;
                     }
-                    if (w == 0.f || page < 0) continue;
-#pragma unroll
-                    for (int t = 0; t < VB; ++t)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int d = (t / 8) * 128 + (g4 * 4 + i) * (2 * VW) + (t & 7);
-                            if (d < D) o[rt][t][i] = fmaf(w, T::up(*(const uint16_t*)(src + 2 * d)), o[rt][t][i]);
-                        }
+                    continue;
                 }
-            }
-        }
-        if (more) load_v(v + 4);
-    }
-
-    // The waves' shares to wave 0, in pairs: 2 and 3 into 0 and 1, 1 into 0.
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        l[rt] += __shfl_xor(l[rt], 16);
-        l[rt] += __shfl_xor(l[rt], 32);
-    }
-    for (int half = 2; half >= 1; half >>= 1) {
-        if (wave >= half && wave < 2 * half) {
-            const int w = wave - half;
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                if (g4 == 0) {
-                    sm_m[w][rt * 16 + n16] = m[rt];
-                    sm_l[w][rt * 16 + n16] = l[rt];
-                }
-#pragma unroll
-                for (int t = 0; t < VB; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sm_o[w][((rt * VB + t) * 4 + i) * 64 + lane] = o[rt][t][i];
+                const int tok = r / G, hd = h * G + r - tok * G;
+                const float inv = L == 0.f ? 0.f : 1.0f / L;   // (a NaN sum stays one)
+                if (a.lse && d == 0) a.lse[(int64_t)(sq.q0 + tok) * a.q_heads + hd] = (M + log2f(L)) * kLn2;
+                *(u32x2*)(a.out + (int64_t)(sq.q0 + tok) * a.ot + (int64_t)hd * a.oh + 2 * d) =
+                    (u32x2){T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv)};
             }
         }
         __syncthreads();
-        if (wave < half) {
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                const float m2 = sm_m[wave][rt * 16 + n16], top = fmaxf(m[rt], m2);
-                const float base = top == -__builtin_huge_valf() ? 0.f : top;
-                const float f1 = __builtin_amdgcn_exp2f(m[rt] - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
-                m[rt] = top;
-                l[rt] = l[rt] * f1 + sm_l[wave][rt * 16 + n16] * f2;
-#pragma unroll
-                for (int t = 0; t < VB; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        o[rt][t][i] = o[rt][t][i] * f1 + sm_o[wave][((rt * VB + t) * 4 + i) * 64 + lane] * f2;
-            }
-        }
-        __syncthreads();
-    }
-    if (wave != 0) return;
-
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int r = r0 + rt * 16 + n16;
-        if (r >= rows) continue;
-        if (a.splits > 1) {
-            const int64_t at = (((int64_t)pair * a.row_tiles + tile) * a.splits + split) * RM + rt * 16 + n16;
-            if (g4 == 0) {
-                a.part_ml[2 * at] = m[rt];
-                a.part_ml[2 * at + 1] = l[rt];
-            }
-#pragma unroll
-            for (int t = 0; t < VB; t += 4)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int d = (t / 8) * 128 + (g4 * 4 + i) * (2 * VW) + (t & 7);
-                    if (d < D)
-                        *(f32x4*)(a.part_o + at * D + d) =
-                            (f32x4){o[rt][t][i], o[rt][t + 1][i], o[rt][t + 2][i], o[rt][t + 3][i]};
-                }
-            continue;
-        }
-        const int tok = r / G, hd = h * G + r - tok * G;
-        const float inv = l[rt] == 0.f ? 0.f : 1.0f / l[rt];   // (a NaN sum stays one)
-        if (a.lse && g4 == 0)
-            a.lse[(int64_t)(sq.q0 + tok) * a.q_heads + hd] = (m[rt] + log2f(l[rt])) * kLn2;
-        char* dst = a.out + (int64_t)(sq.q0 + tok) * a.ot + (int64_t)hd * a.oh;
-#pragma unroll
-        for (int t = 0; t < VB; t += 4)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int d = (t / 8) * 128 + (g4 * 4 + i) * (2 * VW) + (t & 7);
-                if (d < D)
-                    *(u32x2*)(dst + 2 * d) = (u32x2){T::pack(o[rt][t][i] * inv, o[rt][t + 1][i] * inv),
-                                                     T::pack(o[rt][t + 2][i] * inv, o[rt][t + 3][i] * inv)};
-            }
+        x = item + k1;
     }
 }
 
-// ---- the splits' shares of a row ---------------------------------------------------------------
+// ---- the parts of a row --------------------------------------------------------------------------
 //
 // A wave a row: out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), the
-// splits in order.  A split whose sum is zero saw nothing.
+// parts in order.  A part whose sum is zero saw nothing.  The rows kernel
+// leaves a list: its first part lies at the end of a share, the others at the
+// beginning of the shares that follow.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams a, int rm) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -358,14 +405,27 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams a, int rm) {
     const int G = a.group, rows = sq.n * G, D = a.c.head_dim;
     const int in = blockIdx.z * 4 + wave, r = tile * rm + in;
     if (in >= rm || r >= rows) return;
-    const int64_t base = ((int64_t)pair * a.row_tiles + tile) * a.splits;
+    int64_t base, first;   // the part before the second one, and the first
+    int parts;
+    if (a.item_parts) {
+        const int2 ip = a.item_parts[((int64_t)b * a.row_tiles + tile) * a.c.kv_heads + h];
+        parts = ip.y;
+        if (parts == 0) return;   // written by one workgroup
+        base = 2 * (int64_t)ip.x;
+        first = base + 1;
+    } else {
+        parts = a.splits;
+        base = first = ((int64_t)pair * a.row_tiles + tile) * a.splits;
+    }
+    const int step = a.item_parts ? 2 : 1;
+    auto place = [&](int s) { return (s == 0 ? first : base + (int64_t)s * step) * rm + in; };
     float M = -__builtin_huge_valf();
-    for (int s = lane; s < a.splits; s += 64) M = fmaxf(M, a.part_ml[2 * ((base + s) * rm + in)]);
+    for (int s = lane; s < parts; s += 64) M = fmaxf(M, a.part_ml[2 * place(s)]);
     for (int x = 32; x; x >>= 1) M = fmaxf(M, __shfl_xor(M, x));
     const float ref = M == -__builtin_huge_valf() ? 0.f : M;
     float L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.splits; ++s) {
-        const int64_t at = (base + s) * rm + in;
+    for (int s = 0; s < parts; ++s) {
+        const int64_t at = place(s);
         const float l = a.part_ml[2 * at + 1], f = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - ref);
         if (l == 0.f) continue;
         L += l * f;
@@ -385,19 +445,19 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams a, int rm) {
 
 // ---- host ---------------------------------------------------------------------------------------
 
-// The chunk kernel's offsets: a page's stride and what its slots span in 32
-// bits, and of 8 slots below 2^31.
+// A page's stride and what its slots span in 32 bits: the chunk kernel's offsets.
 static bool short_strides(const tms_cache* c, const int64_t* stride) {
-    return 2 * stride[0] < (int64_t)1 << 32 && stride[2] < 1 << 26 && 2 * stride[2] * c->page_size < (int64_t)1 << 32;
+    return 2 * stride[0] < (int64_t)1 << 32 && 2 * stride[2] * c->page_size < (int64_t)1 << 32;
 }
 
 struct AttnPlan {
     bool chunk;        // the chunk kernel
     int rm;            // rows a workgroup
     int row_tiles;
-    int tiles;         // most key tiles of a row tile
     int split_tiles, splits;
-    size_t o_bytes, ml_bytes;
+    int shares;        // workgroups of the rows kernel
+    bool join;
+    size_t o_bytes, ml_bytes, item_bytes;
 };
 
 static int check_attention(const tms_cache* c, const tms_attention_args* a) {
@@ -416,55 +476,57 @@ static AttnPlan plan_attention(const tms_cache* c, const tms_attention_args* a) 
     AttnPlan p;
     const int rows = min(c->max_q, c->tokens) * (a->q_heads / c->kv_heads);
     p.chunk = rows > 64 && short_strides(c, c->k_stride) && short_strides(c, c->v_stride);
-    const int rt = rows <= 16 || c->head_dim > 128 ? 1 : 2;
-    p.rm = p.chunk ? kChunkRows : 16 * rt;
+    p.rm = p.chunk ? kChunkRows : rows <= 32 || c->head_dim > 128 ? 32 : 64;
     p.row_tiles = (rows + p.rm - 1) / p.rm;
     int64_t keys = min(c->max_kv, kMaxLen);
     if (a->window > 0) keys = std::min<int64_t>(keys, (int64_t)a->window + p.rm + a->sinks + 128);
-    const int kt = p.chunk ? chunk_keys(c->head_dim) : 32;
-    p.tiles = (int)((keys + kt - 1) / kt);
     const int64_t items = (int64_t)c->batch * c->kv_heads * p.row_tiles;
+    int64_t parts;
+    p.splits = p.shares = 0;
+    p.item_bytes = 0;
     if (p.chunk) {
         // Workgroups enough for two a CU, with 16 tiles each at least.
+        const int kt = chunk_keys(c->head_dim);
+        const int tiles = (int)((keys + kt - 1) / kt);
         const int64_t want = std::max<int64_t>(1, 512 / std::max<int64_t>(items, 1));
-        p.split_tiles = (int)std::max<int64_t>((p.tiles + want - 1) / want, 16);
+        p.split_tiles = (int)std::max<int64_t>((tiles + want - 1) / want, 16);
+        p.splits = std::max(1, (tiles + p.split_tiles - 1) / p.split_tiles);
+        p.join = p.splits > 1;
+        parts = p.join ? items * p.splits : 0;
     } else {
-    // Workgroups enough for four a CU, with 16 tiles each at least (four a wave).
-    const int64_t want = std::max<int64_t>(1, 1024 / std::max<int64_t>(items, 1));
-    int split = std::max<int64_t>((p.tiles + want - 1) / want, 16);
-    if (split > 64) split = 64;
-    if ((p.tiles + split - 1) / split > 256) split = (p.tiles + 255) / 256;
-    p.split_tiles = (split + 3) / 4 * 4;
+        const int64_t tiles = std::max<int64_t>((keys + 31) / 32, 1) * items;
+        p.split_tiles = 16;
+        p.shares = (int)std::min<int64_t>(c->head_dim > 128 ? 256 : 512, std::max<int64_t>(1, (tiles + p.split_tiles - 1) / p.split_tiles));
+        p.join = true;
+        parts = 2 * (int64_t)p.shares;
+        p.item_bytes = (size_t)(items * 8 + 15) / 16 * 16;
     }
-    p.splits = std::max(1, (p.tiles + p.split_tiles - 1) / p.split_tiles);
-    const size_t parts = p.splits > 1 ? (size_t)items * p.splits * p.rm : 0;
-    p.o_bytes = parts * c->head_dim * 4;
-    p.ml_bytes = parts * 8;
+    p.o_bytes = (size_t)parts * p.rm * c->head_dim * 4;
+    p.ml_bytes = (size_t)parts * p.rm * 8;
     return p;
 }
 
-template <typename T, int KS, int VB>
-static void launch_rows(const AttnPlan& p, const AttnParams& a, dim3 grid, hipStream_t stream) {
-    if constexpr (VB <= 8) {
-        if (p.rm == 32) {
-            hipLaunchKernelGGL((attn_rows_kernel<T, KS, VB, 2>), grid, dim3(256), 0, stream, a);
+template <typename T, int ROWB, int KS, int DT>
+static void launch_rows(const AttnPlan& p, const AttnParams& a, hipStream_t stream) {
+    if constexpr (ROWB <= 256) {
+        if (p.rm == 64) {
+            hipLaunchKernelGGL((attn_rows_kernel<T, ROWB, KS, DT, 2>), dim3(p.shares), dim3(256), 0, stream, a);
             return;
         }
     }
-    hipLaunchKernelGGL((attn_rows_kernel<T, KS, VB, 1>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((attn_rows_kernel<T, ROWB, KS, DT, 1>), dim3(p.shares), dim3(256), 0, stream, a);
 }
 
 template <typename T>
 static void launch_attention(const AttnPlan& p, const AttnParams& a, hipStream_t stream) {
-    const int D = a.c.head_dim;
-    const dim3 grid(a.c.batch * a.c.kv_heads, p.row_tiles, p.splits);
-    if (p.chunk) launch_attn_chunk(a, std::is_same<T, Bf16>::value, grid, stream);
-    else if (D <= 64) launch_rows<T, 2, 4>(p, a, grid, stream);
-    else if (D <= 96) launch_rows<T, 3, 8>(p, a, grid, stream);
-    else if (D <= 128) launch_rows<T, 4, 8>(p, a, grid, stream);
-    else launch_rows<T, 8, 16>(p, a, grid, stream);
-    if (p.splits > 1)
-        hipLaunchKernelGGL((attn_join_kernel<T>), dim3(grid.x, p.row_tiles, (p.rm + 3) / 4), dim3(256), 0, stream, a, p.rm);
+    const int D = a.c.head_dim, pairs = a.c.batch * a.c.kv_heads;
+    if (p.chunk) launch_attn_chunk(a, std::is_same<T, Bf16>::value, dim3(pairs, p.row_tiles, p.splits), stream);
+    else if (D <= 64) launch_rows<T, 128, 4, 2>(p, a, stream);
+    else if (D <= 96) launch_rows<T, 256, 6, 3>(p, a, stream);
+    else if (D <= 128) launch_rows<T, 256, 8, 4>(p, a, stream);
+    else launch_rows<T, 512, 16, 8>(p, a, stream);
+    if (p.join)
+        hipLaunchKernelGGL((attn_join_kernel<T>), dim3(pairs, p.row_tiles, (p.rm + 3) / 4), dim3(256), 0, stream, a, p.rm);
 }
 
 }  // namespace tms
@@ -473,7 +535,7 @@ extern "C" int64_t tms_paged_attention_workspace(const tms_cache* cache, const t
     const int rc = tms::check_attention(cache, args);
     if (rc != TMS_OK) return rc;
     const tms::AttnPlan p = tms::plan_attention(cache, args);
-    return (int64_t)(p.o_bytes + p.ml_bytes);
+    return (int64_t)(p.o_bytes + p.ml_bytes + p.item_bytes);
 }
 
 extern "C" int tms_paged_attention(const tms_cache* cache, const tms_attention_args* args, hipStream_t stream) {
@@ -483,8 +545,8 @@ extern "C" int tms_paged_attention(const tms_cache* cache, const tms_attention_a
     if (cache->batch == 0 || cache->tokens == 0 || cache->max_q == 0) return TMS_OK;
     const AttnPlan p = plan_attention(cache, args);
     if (p.row_tiles > 65535) return TMS_ERR_CAPACITY;
-    if (args->workspace_bytes < p.o_bytes + p.ml_bytes ||
-        (p.splits > 1 && (!args->workspace || !aligned16(args->workspace))))
+    if (args->workspace_bytes < p.o_bytes + p.ml_bytes + p.item_bytes ||
+        (p.join && (!args->workspace || !aligned16(args->workspace))))
         return TMS_ERR_INVALID_ARG;
     AttnParams a;
     a.c = view_of(cache);
@@ -506,6 +568,7 @@ extern "C" int tms_paged_attention(const tms_cache* cache, const tms_attention_a
     a.row_tiles = p.row_tiles;
     a.part_o = (float*)args->workspace;
     a.part_ml = (float*)((char*)args->workspace + p.o_bytes);
+    a.item_parts = p.chunk ? nullptr : (int2*)((char*)args->workspace + p.o_bytes + p.ml_bytes);
     if (cache->dtype == TMS_DTYPE_BF16) launch_attention<Bf16>(p, a, stream);
     else launch_attention<F16>(p, a, stream);
     return hipGetLastError() == hipSuccess ? TMS_OK : TMS_ERR_HIP;

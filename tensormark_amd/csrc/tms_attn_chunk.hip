@@ -11,30 +11,6 @@
 
 namespace tms {
 
-typedef __attribute__((address_space(3))) void lds_void;
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-
-// A tile lies in LDS by rows of `ROWB` bytes, a key's (value's) 16-byte pieces
-// permuted within its row so that the reads of the matrix operands fall on
-// different banks: the key operand takes one piece of 32 rows, the value
-// operand (transposed on the way, ds_read_b64_tr_b16) 64 bytes of 4 rows.
-template <int ROWB> __device__ __forceinline__ int key_swizzle(int row) { return ROWB == 128 ? row >> 1 & 7 : row & 15; }
-template <int ROWB> __device__ __forceinline__ int value_swizzle(int row) { return ROWB == 128 ? (row >> 1 & 1) << 2 : (row & 3) << 2; }
-
-// 16 bytes a lane from `off` of the resource to LDS at `lds` (wave-uniform) +
-// 16 * lane; zeros where the resource ends before.  Counted by vmcnt only:
-// the loop waits for it, the compiler does not know of it.
-__device__ __forceinline__ void load_lds16(u32x4 rsrc, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc) : "memory");
-}
-
-// The resource of the last + 1 slots at `p`, none of them where `last` < 0.
-__device__ __forceinline__ u32x4 slots_rsrc(const char* p, int last, uint32_t stride, int bytes) {
-    const uint64_t at = (uint64_t)p;
-    return (u32x4){(uint32_t)at, (uint32_t)(at >> 32) & 0xFFFF, last < 0 ? 0u : (uint32_t)(last * stride + bytes), 0x00020000u};
-}
-
 template <typename T, int ROWB, int KS, int DT, int NK>
 __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(AttnParams a) {
     constexpr int KT = 32 * NK, RM = kChunkRows;
@@ -63,10 +39,7 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
     {
         const char* src = a.q + (int64_t)(sq.q0 + tok) * a.qt + (int64_t)(h * G + hd) * a.qh;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const int d = s * 16 + hh * 8;
-            qf[s] = in && d < D ? (*(const u32x4*)(src + 2 * d) & a.qand) ^ a.qxor : (u32x4){0, 0, 0, 0};
-        }
+        for (int s = 0; s < KS; ++s) qf[s] = query_operand(a, src, s * 16 + hh * 8, in);
     }
 
     // Loads into LDS: an instruction moves 64 pieces, RPI whole rows, of 8
@@ -141,10 +114,9 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
         for (int kt = 0; kt < NK; ++kt) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[kt][i] = 0.f;
-            const int key = kt * 32 + n32;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                const u32x4 kf = *(const u32x4*)(sk + key * ROWB + 16 * ((2 * ks + hh) ^ key_swizzle<ROWB>(key)));
+                const u32x4 kf = key_operand<ROWB>(sk, lane, kt, ks);
                 s[kt] = T::mfma32(kf, qf[ks], s[kt]);
             }
         }
@@ -189,31 +161,28 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
         if constexpr (EDGE) {
             // A weight of zero times an infinity or NaN would reach rows that
             // do not see the value: such values go, key by key, to the rows whose
-            // weight is not zero, and are zero in the product.
+            // weight is not zero (which weight does not matter), and are zero in
+            // the product.
             if (odd) {
+                uint32_t mine = 0;
+#pragma unroll
+                for (int e = 0; e < 16 * NK; ++e) mine |= s[e / 16][e % 16] != 0.f ? 1u << e : 0u;
+                const uint32_t other = __shfl_xor(mine, 32);
 #pragma unroll 1
-                for (int e = 0; e < 16 * NK; ++e) {
-                    float x = s[0][0];
+                for (int key = 0; key < KT; ++key) {
+                    const uint32_t w = (key >> 2 & 1) == hh ? mine : other;
+                    if (!(w >> (key / 8 * 4 + (key & 3)) & 1)) continue;
 #pragma unroll
-                    for (int q = 1; q < 16 * NK; ++q) x = e == q ? s[q / 16][q % 16] : x;
-                    const float y = __shfl_xor(x, 32);
-#pragma unroll 1
-                    for (int half = 0; half < 2; ++half) {
-                        const float w = hh == half ? x : y;
-                        const int key = 32 * (e / 16) + 8 * (e % 16 / 4) + 4 * half + (e & 3);
+                    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                        for (int dt = 0; dt < DT; ++dt)
+                        for (int c = 0; c < 4; ++c) {
+                            const u32x2 val = *(const u32x2*)(sv + key * ROWB + 16 * ((4 * dt + c) ^ value_swizzle<ROWB>(key)) + 8 * hh);
 #pragma unroll
-                            for (int c = 0; c < 4; ++c) {
-                                const u32x2 val =
-                                    *(const u32x2*)(sv + key * ROWB + 16 * ((4 * dt + c) ^ value_swizzle<ROWB>(key)) + 8 * hh);
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    const uint32_t bits = val[i / 2] >> 16 * (i & 1) & 0xFFFF;
-                                    if (w != 0.f && (bits & T::kExp) == T::kExp) o[dt][4 * c + i] = fmaf(w, T::up(bits), o[dt][4 * c + i]);
-                                }
+                            for (int i = 0; i < 4; ++i) {
+                                const uint32_t bits = val[i / 2] >> 16 * (i & 1) & 0xFFFF;
+                                o[dt][4 * c + i] += (bits & T::kExp) == T::kExp ? T::up(bits) : 0.f;
                             }
-                    }
+                        }
                 }
                 __syncthreads();
                 for (int i = threadIdx.x; i < KT * ROWB / 16; i += 256) {
@@ -229,25 +198,10 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
             }
         }
 
-        // Value operand: the lane's value column, keys 16t + 4hh + 0..3 and 8 more on.
-        const int q16 = lane & 15, colg = lane >> 4 & 1;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int t = 0; t < 2 * NK; ++t) {
-                u32x4 vf;
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int key = 16 * t + 8 * u + 4 * hh + (q16 >> 2);
-                    const int ch = 4 * dt + 2 * colg + (q16 >> 1 & 1);
-                    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (lds_s16x4*)(sv + key * ROWB + 16 * (ch ^ value_swizzle<ROWB>(key)) + 8 * (q16 & 1)));
-                    const u32x2 y = __builtin_bit_cast(u32x2, x);
-                    vf[2 * u] = y[0];
-                    vf[2 * u + 1] = y[1];
-                }
-                o[dt] = T::mfma32(vf, pf[t], o[dt]);
-            }
+            for (int t = 0; t < 2 * NK; ++t) o[dt] = T::mfma32(value_operand<ROWB>(sv, lane, dt, t), pf[t], o[dt]);
     };
 
     int pg = v0 < v1 ? entries(v0) : -1, ahead = v0 + 1 < v1 ? entries(v0 + 1) : -1;
