@@ -24,6 +24,8 @@
 
 namespace tms {
 
+constexpr int kShareRows = 32;   // of a workgroup of the rows kernel
+
 // ---- few rows: the keys of all sequences in equal shares ---------------------------------------
 //
 // Bound by memory: the keys and values of a call are read once.  All items
@@ -32,73 +34,89 @@ namespace tms {
 // an item that its share holds whole is written out, the two at its ends go
 // to the workspace as parts, which a second launch joins.
 //
-// Within an item the four waves take the tiles (32 keys) in turn, each with
+// Within an item the waves take the tiles (32 keys) in turn, each with
 // its own running maximum and sum and its own piece of LDS: a tile's keys are
 // loaded there while the values of the one before are used, and its values
 // while its keys are, so that 8 waves a CU keep some 100 KB on the way without
 // a register for it.  No wave waits for another before the item's end.
-template <int RM>
 __device__ __forceinline__ int item_tiles(const AttnParams& a, int combo) {
     const int b = combo / a.row_tiles, tile = combo - b * a.row_tiles;
     const SeqView sq = seq_view(a.c, b);
-    const int G = a.group, rows = sq.n * G, r0 = tile * RM;
+    const int G = a.group, rows = sq.n * G, r0 = tile * kShareRows;
     if (r0 >= rows) return 0;
     // (rows that see nothing have an output all the same)
-    return max(TileList<32>(a.window, a.sinks, sq.p0 + r0 / G, sq.p0 + (min(r0 + RM, rows) - 1) / G, sq.len).n, 1);
+    return max(TileList<32>(a.window, a.sinks, sq.p0 + r0 / G, sq.p0 + (min(r0 + kShareRows, rows) - 1) / G, sq.len).n, 1);
 }
 
 __device__ __forceinline__ int64_t share_of(const AttnParams& a, int64_t total, int shares) {
     return max((total + shares - 1) / shares, (int64_t)a.split_tiles);
 }
 
-template <typename T, int ROWB, int KS, int DT, int RT>
-__global__ __launch_bounds__(256, ROWB > 256 || (ROWB > 128 && RT > 1) ? 1 : 2) void attn_rows_kernel(AttnParams a) {
-    constexpr int RM = 32 * RT, KT = 32, NL = KT * ROWB / 1024, RPI = 1024 / ROWB, PAD = 33;
-    constexpr int MERGE = 4 * DT * 32 * PAD * 4, RING = 4 * 2 * KT * ROWB;
-    __shared__ __attribute__((aligned(128))) char sm[MERGE > RING ? MERGE : RING];
-    __shared__ float sm_ml[RT][4][32][2];
-    __shared__ int64_t wsum[4], start_at;
-    __shared__ int start_combo;
+// Four values of a row's output from dimension d on, and its lse.
+template <typename T>
+__device__ __forceinline__ void write_row(const AttnParams& a, const SeqView& sq, int h, int r, int d, float m, float l, f32x4 o) {
+    const int tok = r / a.group, hd = h * a.group + r - tok * a.group;
+    const float inv = l == 0.f ? 0.f : 1.0f / l;   // (a NaN sum stays one)
+    if (a.lse && d == 0) a.lse[(int64_t)(sq.q0 + tok) * a.q_heads + hd] = (m + log2f(l)) * kLn2;
+    *(u32x2*)(a.out + (int64_t)(sq.q0 + tok) * a.ot + (int64_t)hd * a.oh + 2 * d) =
+        (u32x2){T::pack(o[0] * inv, o[1] * inv), T::pack(o[2] * inv, o[3] * inv)};
+}
+
+template <typename T, int ROWB, int KS, int DT, int NW>
+__global__ __launch_bounds__(64 * NW, ROWB > 256 ? 1 : 2) void attn_rows_kernel(AttnParams a) {
+    constexpr int RM = kShareRows, KT = 32, NL = KT * ROWB / 1024, RPI = 1024 / ROWB, PAD = 33;
+    // LDS: the waves' pieces, and at an item's end their outputs, maxima and sums.
+    constexpr int RING = NW * 2 * KT * ROWB;
+    constexpr int MERGE = NW * DT * 32 * PAD * 4, ML = NW * 32 * 2 * 4;
+    __shared__ __attribute__((aligned(128))) char sm[MERGE + ML > RING ? MERGE + ML : RING];
+    float* const sm_ml = (float*)(sm + MERGE);   // [wave][row][maximum, sum]
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int n32 = lane & 31, hh = lane >> 5;
     const int H = a.c.kv_heads, G = a.group, D = a.c.head_dim;
     const int combos = a.c.batch * a.row_tiles;
 
     // The share: [x, end) of the axis, which starts in `combo` (a sequence's
-    // row tile, all key heads one after another) at `at`.
-    const int per = (combos + 255) / 256, c0 = min(t * per, combos), c1 = min(c0 + per, combos);
-    int64_t mine = 0;
-    for (int c = c0; c < c1; ++c) mine += item_tiles<RM>(a, c);
-    int64_t upto = mine;
+    // row tile, all key heads one after another) at `at`.  Without shares, an
+    // item a workgroup.
+    int64_t share = 0, x = 0, end = 1, at = 0;
+    int combo = blockIdx.x / H;
+    if (a.split_tiles > 0) {
+        int64_t* const wsum = (int64_t*)sm;   // [NW], then where the share starts
+        const int per = (combos + 64 * NW - 1) / (64 * NW), c0 = min(t * per, combos), c1 = min(c0 + per, combos);
+        int64_t mine = 0;
+        for (int c = c0; c < c1; ++c) mine += item_tiles(a, c);
+        int64_t upto = mine;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int64_t y = __shfl_up(upto, d);
-        if (lane >= d) upto += y;
-    }
-    if (lane == 63) wsum[wave] = upto;
-    __syncthreads();
-    int64_t total = 0, before = upto - mine;
-    for (int w = 0; w < 4; ++w) {
-        before += w < wave ? wsum[w] : 0;
-        total += wsum[w];
-    }
-    const int64_t share = share_of(a, total * H, gridDim.x);
-    int64_t x = blockIdx.x * share;
-    const int64_t end = min(x + share, total * H);
-    if (x >= end) return;
-    if (x >= before * H && x < (before + mine) * H)
-        for (int c = c0;; ++c) {
-            const int n = item_tiles<RM>(a, c);
-            if (x < (before + n) * H) {
-                start_combo = c;
-                start_at = before * H;
-                break;
-            }
-            before += n;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int64_t y = __shfl_up(upto, d);
+            if (lane >= d) upto += y;
         }
-    __syncthreads();
-    int combo = __builtin_amdgcn_readfirstlane(start_combo);
-    int64_t at = start_at;
+        if (lane == 63) wsum[wave] = upto;
+        __syncthreads();
+        int64_t total = 0, before = upto - mine;
+        for (int w = 0; w < NW; ++w) {
+            before += w < wave ? wsum[w] : 0;
+            total += wsum[w];
+        }
+        share = share_of(a, total * H, gridDim.x);
+        x = blockIdx.x * share;
+        end = min(x + share, total * H);
+        if (x >= end) return;
+        if (x >= before * H && x < (before + mine) * H)
+            for (int c = c0;; ++c) {
+                const int n = item_tiles(a, c);
+                if (x < (before + n) * H) {
+                    wsum[NW] = c;
+                    wsum[NW + 1] = before * H;
+                    break;
+                }
+                before += n;
+            }
+        __syncthreads();
+        combo = __builtin_amdgcn_readfirstlane((int)wsum[NW]);
+        at = wsum[NW + 1];
+        __syncthreads();
+    }
 
     char* ring = sm + wave * 2 * KT * ROWB;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)ring;
@@ -117,6 +135,7 @@ __global__ __launch_bounds__(256, ROWB > 256 || (ROWB > 128 && RT > 1) ? 1 : 2) 
         const SeqView sq = seq_view(a.c, b);
         const int rows = sq.n * G, r0 = tile * RM;
         if (r0 >= rows) {
+            if (a.split_tiles == 0) return;
             ++combo;
             continue;
         }
@@ -124,7 +143,11 @@ __global__ __launch_bounds__(256, ROWB > 256 || (ROWB > 128 && RT > 1) ? 1 : 2) 
         const int pfirst = sq.p0 + r0 / G, plast = sq.p0 + (r0 + nr - 1) / G;
         const TileList<KT> tl(a.window, a.sinks, pfirst, plast, sq.len);
         const int n = max(tl.n, 1);
-        if (x >= at + (int64_t)n * H) {
+        if (a.split_tiles == 0) {
+            x = at = (int64_t)(blockIdx.x - combo * H) * n;   // (only this item, by its own axis)
+            at = 0;
+            end = x + n;
+        } else if (x >= at + (int64_t)n * H) {
             at += (int64_t)n * H;
             ++combo;
             continue;
@@ -133,17 +156,15 @@ __global__ __launch_bounds__(256, ROWB > 256 || (ROWB > 128 && RT > 1) ? 1 : 2) 
         const int64_t item = at + (int64_t)h * n;
         const int k0 = (int)(x - item), k1 = (int)min((int64_t)n, end - item), kend = min(k1, tl.n);
 
-        int pos[RT];
-        u32x4 qf[RT][KS];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const int r = r0 + 32 * rt + n32;
-            const bool in = r < rows;
-            const int tok = in ? r / G : 0, hd = in ? r - tok * G : 0;
-            pos[rt] = in ? sq.p0 + tok : -1;
+        const int r = r0 + n32;
+        const bool in = r < rows;
+        const int tok = in ? r / G : 0, hd = in ? r - tok * G : 0;
+        const int pos = in ? sq.p0 + tok : -1;
+        u32x4 qf[KS];
+        {
             const char* src = a.q + (int64_t)(sq.q0 + tok) * a.qt + (int64_t)(h * G + hd) * a.qh;
 #pragma unroll
-            for (int s = 0; s < KS; ++s) qf[rt][s] = query_operand(a, src, s * 16 + hh * 8, in);
+            for (int s = 0; s < KS; ++s) qf[s] = query_operand(a, src, s * 16 + hh * 8, in);
         }
         // Table entries of a tile's groups of 8 keys: by the scalar cache, whose
         // counter the loads into LDS do not share.
@@ -180,17 +201,12 @@ __global__ __launch_bounds__(256, ROWB > 256 || (ROWB > 128 && RT > 1) ? 1 : 2) 
             }
         };
 
-        f32x16 o[RT][DT];
-        float m[RT], l[RT];
+        f32x16 o[DT];
+        float m = -__builtin_huge_valf(), l = 0.f;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            m[rt] = -__builtin_huge_valf();
-            l[rt] = 0.f;
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[rt][dt][i] = 0.f;
-        }
+            for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
         int v = k0 + wave;
         uint32_t there = 0;
         if (v < kend) {
@@ -199,32 +215,23 @@ __global__ __launch_bounds__(256, ROWB > 256 || (ROWB > 128 && RT > 1) ? 1 : 2) 
             __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): what went before is not counted below
             load(v, kbase, a.c.kp, kslot, koff, lds0);
             load(v, vbase, a.c.vp, vslot, voff, lds0 + KT * ROWB);
-            if (v + 4 < kend) entries(v + 4);
+            if (v + NW < kend) entries(v + NW);
         }
-        for (; v < kend; v += 4) {
-            const bool more = v + 4 < kend;
+        for (; v < kend; v += NW) {
+            const bool more = v + NW < kend;
             const int t0 = tl.key(v);
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");   // the keys; the values may be on the way
-            f32x16 s[RT];
+            f32x16 s;
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
+            for (int i = 0; i < 16; ++i) s[i] = 0.f;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[rt][i] = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const u32x4 kf = key_operand<ROWB>(ring, lane, 0, ks);
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) s[rt] = T::mfma32(kf, qf[rt][ks], s[rt]);
-            }
+            for (int ks = 0; ks < KS; ++ks) s = T::mfma32(key_operand<ROWB>(ring, lane, 0, ks), qf[ks], s);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the keys are read: their place is free
             const uint32_t now = there;
-            int pnow[4];
-#pragma unroll
-            for (int g = 0; g < 4; ++g) pnow[g] = page[g];
             if (more) {
-                there = take(v + 4);
-                load(v + 4, kbase, a.c.kp, kslot, koff, lds0);
-                if (v + 8 < kend) entries(v + 8);
+                there = take(v + NW);
+                load(v + NW, kbase, a.c.kp, kslot, koff, lds0);
+                if (v + 2 * NW < kend) entries(v + 2 * NW);
             }
             const bool edge = now != 15 || t0 + KT > sq.len || t0 + KT - 1 > pfirst ||
                               (a.window > 0 && t0 <= plast - a.window && t0 + KT > a.sinks);
@@ -232,45 +239,34 @@ __global__ __launch_bounds__(256, ROWB > 256 || (ROWB > 128 && RT > 1) ? 1 : 2) 
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int j = t0 + 8 * (i / 4) + 4 * hh + (i & 3);
-                    const bool is = (now >> (i / 4) & 1) && j < sq.len;
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
-                        s[rt][i] = is && sees(j, pos[rt], a.window, a.sinks) ? s[rt][i] : -__builtin_huge_valf();
+                    const bool on = (now >> (i / 4) & 1) && j < sq.len && sees(j, pos, a.window, a.sinks);
+                    s[i] = on ? s[i] : -__builtin_huge_valf();
                 }
             }
-            u32x4 pf[RT][2];
-            uint32_t some[RT];   // weights that are not zero, a bit each
+            float top = -__builtin_huge_valf();
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                float top = -__builtin_huge_valf();
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, s[e]);
+            top *= a.scale;
+            if (__any(top > m + kSlack)) {   // (as in the chunk kernel)
+                top = fmaxf(top, __shfl_xor(top, 32));
+                top = fmaxf(top, m);
+                const float f = __builtin_amdgcn_exp2f(m - (top == -__builtin_huge_valf() ? 0.f : top));
+                m = top;
+                l *= f;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) top = fmaxf(top, s[rt][e]);
-                top *= a.scale;
-                if (__any(top > m[rt] + kSlack)) {   // (as in the chunk kernel)
-                    top = fmaxf(top, __shfl_xor(top, 32));
-                    top = fmaxf(top, m[rt]);
-                    const float f = __builtin_amdgcn_exp2f(m[rt] - (top == -__builtin_huge_valf() ? 0.f : top));
-                    m[rt] = top;
-                    l[rt] *= f;
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= f;
-                }
-                const float base = m[rt] == -__builtin_huge_valf() ? 0.f : m[rt];
-                some[rt] = 0;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    s[rt][e] = __builtin_amdgcn_exp2f(fmaf(s[rt][e], a.scale, -base));
-                    l[rt] += s[rt][e];
-                }
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) pf[rt][u][w] = T::pack(s[rt][8 * u + 2 * w], s[rt][8 * u + 2 * w + 1]);
-                if (edge) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) some[rt] |= s[rt][e] != 0.f ? 1u << e : 0u;
-                }
+                for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
             }
+            const float base = m == -__builtin_huge_valf() ? 0.f : m;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale, -base));
+                l += s[e];
+            }
+            u32x4 pf[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) pf[u][w] = T::pack(s[8 * u + 2 * w], s[8 * u + 2 * w + 1]);
             if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");   // the values; the next keys may be on the way
             else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             char* sv = ring + KT * ROWB;
@@ -287,25 +283,25 @@ __global__ __launch_bounds__(256, ROWB > 256 || (ROWB > 128 && RT > 1) ? 1 : 2) 
                     for (int w = 0; w < 4; ++w) odd |= (y[w] & T::kExp) == T::kExp || (y[w] >> 16 & T::kExp) == T::kExp;
                 }
                 if (__any(odd)) {
+                    uint32_t mine = 0;
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) {
-                        const uint32_t other = __shfl_xor(some[rt], 32);
+                    for (int e = 0; e < 16; ++e) mine |= s[e] != 0.f ? 1u << e : 0u;
+                    const uint32_t other = __shfl_xor(mine, 32);
 #pragma unroll 1
-                        for (int key = 0; key < KT; ++key) {
-                            const uint32_t w = (key >> 2 & 1) == hh ? some[rt] : other;
-                            if (!(w >> (key / 8 * 4 + (key & 3)) & 1)) continue;
+                    for (int key = 0; key < KT; ++key) {
+                        const uint32_t w = (key >> 2 & 1) == hh ? mine : other;
+                        if (!(w >> (key / 8 * 4 + (key & 3)) & 1)) continue;
 #pragma unroll
-                            for (int dt = 0; dt < DT; ++dt)
+                        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                                for (int c = 0; c < 4; ++c) {
-                                    const u32x2 val = *(const u32x2*)(sv + key * ROWB + 16 * ((4 * dt + c) ^ value_swizzle<ROWB>(key)) + 8 * hh);
+                            for (int c = 0; c < 4; ++c) {
+                                const u32x2 val = *(const u32x2*)(sv + key * ROWB + 16 * ((4 * dt + c) ^ value_swizzle<ROWB>(key)) + 8 * hh);
 #pragma unroll
-                                    for (int i = 0; i < 4; ++i) {
-                                        const uint32_t bits = val[i / 2] >> 16 * (i & 1) & 0xFFFF;
-                                        o[rt][dt][4 * c + i] += (bits & T::kExp) == T::kExp ? T::up(bits) : 0.f;
-                                    }
+                                for (int i = 0; i < 4; ++i) {
+                                    const uint32_t bits = val[i / 2] >> 16 * (i & 1) & 0xFFFF;
+                                    o[dt][4 * c + i] += (bits & T::kExp) == T::kExp ? T::up(bits) : 0.f;
                                 }
-                        }
+                            }
                     }
 #pragma unroll 1
                     for (int i = 0; i < NL; ++i) {
@@ -323,69 +319,58 @@ __global__ __launch_bounds__(256, ROWB > 256 || (ROWB > 128 && RT > 1) ? 1 : 2) 
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const u32x4 vf = value_operand<ROWB>(sv, lane, dt, u);
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) o[rt][dt] = T::mfma32(vf, pf[rt][u], o[rt][dt]);
-                }
+                for (int u = 0; u < 2; ++u) o[dt] = T::mfma32(value_operand<ROWB>(sv, lane, dt, u), pf[u], o[dt]);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (more) load(v + 4, vbase, a.c.vp, vslot, voff, lds0 + KT * ROWB);
+            if (more) load(v + NW, vbase, a.c.vp, vslot, voff, lds0 + KT * ROWB);
         }
 
-        // The four waves' shares of the item's rows, by way of LDS: 32 rows a
-        // pass, row by row contiguous in a wave's array [dimension][row].
+        // The waves' shares of the item's rows, by way of LDS: an array
+        // [dimension][row] a wave.
         const bool whole = k0 == 0 && k1 == n;
         const int64_t part = 2 * (int64_t)blockIdx.x + (k0 == 0 ? 1 : 0);
         const int item_id = combo * H + h;
-        if (k0 == 0 && t == 0 && a.item_parts)
+        if (k0 == 0 && t == 0 && a.split_tiles > 0)
             a.item_parts[item_id] = make_int2(blockIdx.x, whole ? 0 : (int)((item + n - 1) / share) - (int)blockIdx.x + 1);
+        l += __shfl_xor(l, 32);
+        __syncthreads();
+        if (hh == 0) {
+            sm_ml[(wave * 32 + n32) * 2] = m;
+            sm_ml[(wave * 32 + n32) * 2 + 1] = l;
+        }
+        float* to = (float*)sm + wave * DT * 32 * PAD;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            l[rt] += __shfl_xor(l[rt], 32);
-            __syncthreads();
-            if (hh == 0) {
-                sm_ml[rt][wave][n32][0] = m[rt];
-                sm_ml[rt][wave][n32][1] = l[rt];
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) to[(32 * dt + 8 * (i / 4) + 4 * hh + (i & 3)) * PAD + n32] = o[dt][i];
+        __syncthreads();
+        const int quads = D / 4;
+        for (int e = t; e < nr * quads; e += 64 * NW) {
+            const int rr = e / quads, d = 4 * (e - rr * quads);
+            float M = -__builtin_huge_valf(), L = 0.f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) M = fmaxf(M, sm_ml[(w * 32 + rr) * 2]);
+            const float ref = M == -__builtin_huge_valf() ? 0.f : M;
+            f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                const float f = __builtin_amdgcn_exp2f(sm_ml[(w * 32 + rr) * 2] - ref);
+                L += sm_ml[(w * 32 + rr) * 2 + 1] * f;
+                const float* from = (const float*)sm + (w * DT * 32 + d) * PAD + rr;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[i] += from[i * PAD] * f;
             }
-            float* to = (float*)sm + wave * DT * 32 * PAD;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) to[(32 * dt + 8 * (i / 4) + 4 * hh + (i & 3)) * PAD + n32] = o[rt][dt][i];
-            __syncthreads();
-            const int nrt = min(nr - 32 * rt, 32), quads = D / 4;
-            for (int e = t; e < nrt * quads; e += 256) {
-                const int rr = e / quads, d = 4 * (e - rr * quads), r = r0 + 32 * rt + rr;
-                float M = -__builtin_huge_valf(), L = 0.f;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) M = fmaxf(M, sm_ml[rt][w][rr][0]);
-                const float base = M == -__builtin_huge_valf() ? 0.f : M;
-                f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const float f = __builtin_amdgcn_exp2f(sm_ml[rt][w][rr][0] - base), lw = sm_ml[rt][w][rr][1];
-                    if (lw == 0.f) continue;   // the wave's keys gave the row nothing
-                    L += lw * f;
-                    const float* from = (const float*)sm + (w * DT * 32 + d) * PAD + rr;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[i] += from[i * PAD] * f;
+            if (!whole) {
+                const int64_t row_at = part * RM + rr;
+                *(f32x4*)(a.part_o + row_at * D + d) = acc;
+                if (d == 0) {
+                    a.part_ml[2 * row_at] = M;
+                    a.part_ml[2 * row_at + 1] = L;
                 }
-                if (!whole) {
-                    const int64_t to_row = part * RM + 32 * rt + rr;
-                    *(f32x4*)(a.part_o + to_row * D + d) = acc;
-                    if (d == 0) {
-                        a.part_ml[2 * to_row] = M;
-                        a.part_ml[2 * to_row + 1] = L;
-                    }
-                    continue;
-                }
-                const int tok = r / G, hd = h * G + r - tok * G;
-                const float inv = L == 0.f ? 0.f : 1.0f / L;   // (a NaN sum stays one)
-                if (a.lse && d == 0) a.lse[(int64_t)(sq.q0 + tok) * a.q_heads + hd] = (M + log2f(L)) * kLn2;
-                *(u32x2*)(a.out + (int64_t)(sq.q0 + tok) * a.ot + (int64_t)hd * a.oh + 2 * d) =
-                    (u32x2){T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv)};
+            } else {
+                write_row<T>(a, sq, h, r0 + rr, d, M, L, acc);
             }
         }
+        if (a.split_tiles == 0) return;
         __syncthreads();
         x = item + k1;
     }
@@ -393,54 +378,91 @@ __global__ __launch_bounds__(256, ROWB > 256 || (ROWB > 128 && RT > 1) ? 1 : 2) 
 
 // ---- the parts of a row --------------------------------------------------------------------------
 //
-// A wave a row: out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), the
-// parts in order.  A part whose sum is zero saw nothing.  The rows kernel
-// leaves a list: its first part lies at the end of a share, the others at the
+// out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M).  LPR lanes (4 dimensions
+// each) take a part; `sub` such groups take a row's parts in turn, each with
+// its own maximum, and meet in LDS, so a long list is some loads deep and a
+// workgroup has several rows where the lists are short.  The rows kernel
+// leaves lists: the first part lies at the end of a share, the others at the
 // beginning of the shares that follow.
-template <typename T>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnParams a, int rm) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+template <typename T, int LPR>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnParams a, int rm, int sub) {
+    __shared__ float sm[256 / LPR][4 * LPR + 2];
+    const int g = threadIdx.x / LPR, lane = threadIdx.x % LPR, sg = g % sub;
     const int pair = blockIdx.x, tile = blockIdx.y, b = pair / a.c.kv_heads, h = pair - b * a.c.kv_heads;
     const SeqView sq = seq_view(a.c, b);
-    const int G = a.group, rows = sq.n * G, D = a.c.head_dim;
-    const int in = blockIdx.z * 4 + wave, r = tile * rm + in;
-    if (in >= rm || r >= rows) return;
+    const int rows = sq.n * a.group, D = a.c.head_dim, n_in = 256 / LPR / sub;
+    const int in = blockIdx.z * n_in + g / sub, r = tile * rm + in;
+    if (tile * rm + (int)blockIdx.z * n_in >= rows) return;
     int64_t base, first;   // the part before the second one, and the first
-    int parts;
+    int parts, step;
     if (a.item_parts) {
         const int2 ip = a.item_parts[((int64_t)b * a.row_tiles + tile) * a.c.kv_heads + h];
         parts = ip.y;
         if (parts == 0) return;   // written by one workgroup
         base = 2 * (int64_t)ip.x;
         first = base + 1;
+        step = 2;
     } else {
         parts = a.splits;
         base = first = ((int64_t)pair * a.row_tiles + tile) * a.splits;
+        step = 1;
     }
-    const int step = a.item_parts ? 2 : 1;
+    const bool on = in < rm && r < rows;
     auto place = [&](int s) { return (s == 0 ? first : base + (int64_t)s * step) * rm + in; };
-    float M = -__builtin_huge_valf();
-    for (int s = lane; s < parts; s += 64) M = fmaxf(M, a.part_ml[2 * place(s)]);
-    for (int x = 32; x; x >>= 1) M = fmaxf(M, __shfl_xor(M, x));
-    const float ref = M == -__builtin_huge_valf() ? 0.f : M;
-    float L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < parts; ++s) {
-        const int64_t at = place(s);
-        const float l = a.part_ml[2 * at + 1], f = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - ref);
-        if (l == 0.f) continue;
-        L += l * f;
-        if (4 * lane < D) {
-            const f32x4 o = *(const f32x4*)(a.part_o + at * D + 4 * lane);
+    float M = -__builtin_huge_valf(), L = 0.f;
+    f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
+    const int d = 4 * lane < D ? 4 * lane : 0;
+    for (int s0 = sg; on && s0 < parts; s0 += sub * LPR) {   // LPR parts: a lane has one's maximum and sum
+        const int s = s0 + sub * lane, count = min((parts - s0 + sub - 1) / sub, LPR);
+        const float2 ml = lane < count ? *(const float2*)(a.part_ml + 2 * place(s)) : make_float2(-__builtin_huge_valf(), 0.f);
+        float top = ml.x;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i] += o[i] * f;
+        for (int x = LPR / 2; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, LPR));
+        top = fmaxf(top, M);
+        const float ref = top == -__builtin_huge_valf() ? 0.f : top;
+        const float f0 = __builtin_amdgcn_exp2f(M - ref), f = __builtin_amdgcn_exp2f(ml.x - ref);
+        M = top;
+        L *= f0;
+        acc *= f0;
+        float sum = ml.y * f;
+#pragma unroll
+        for (int x = LPR / 2; x; x >>= 1) sum += __shfl_xor(sum, x, LPR);
+        L += sum;
+        for (int i = 0; i < count; i += 4) {
+            f32x4 o[4];
+            float w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int at = min(i + k, count - 1);
+                w[k] = __shfl(f, at, LPR);
+                o[k] = *(const f32x4*)(a.part_o + place(s0 + sub * at) * D + d);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (i + k < count) acc += o[k] * w[k];
         }
     }
-    const int tok = r / G, hd = h * G + r - tok * G;
-    const float inv = L == 0.f ? 0.f : 1.0f / L;
-    if (a.lse && lane == 0) a.lse[(int64_t)(sq.q0 + tok) * a.q_heads + hd] = (M + log2f(L)) * kLn2;
-    if (4 * lane < D)
-        *(u32x2*)(a.out + (int64_t)(sq.q0 + tok) * a.ot + (int64_t)hd * a.oh + 8 * lane) =
-            (u32x2){T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv)};
+    if (sub > 1) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sm[g][4 * lane + e] = acc[e];
+        if (lane == 0) {
+            sm[g][4 * LPR] = M;
+            sm[g][4 * LPR + 1] = L;
+        }
+        __syncthreads();
+        if (sg != 0) return;
+        for (int i = 1; i < sub; ++i) M = fmaxf(M, sm[g + i][4 * LPR]);
+        const float ref = M == -__builtin_huge_valf() ? 0.f : M;
+        L = 0.f;
+        acc = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < sub; ++i) {
+            const float f = __builtin_amdgcn_exp2f(sm[g + i][4 * LPR] - ref);
+            L += sm[g + i][4 * LPR + 1] * f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] += sm[g + i][4 * lane + e] * f;
+        }
+    }
+    if (on && 4 * lane < D) write_row<T>(a, sq, h, r, 4 * lane, M, L, acc);
 }
 
 // ---- host ---------------------------------------------------------------------------------------
@@ -450,13 +472,17 @@ static bool short_strides(const tms_cache* c, const int64_t* stride) {
     return 2 * stride[0] < (int64_t)1 << 32 && 2 * stride[2] * c->page_size < (int64_t)1 << 32;
 }
 
+constexpr int kWholeTiles = 32;
+
 struct AttnPlan {
     bool chunk;        // the chunk kernel
     int rm;            // rows a workgroup
     int row_tiles;
     int split_tiles, splits;
     int shares;        // workgroups of the rows kernel
+    int waves;         // of one of them
     bool join;
+    int rows, most_parts;   // bounds: of a sequence and key head, and of a row's parts
     size_t o_bytes, ml_bytes, item_bytes;
 };
 
@@ -474,9 +500,9 @@ static int check_attention(const tms_cache* c, const tms_attention_args* a) {
 
 static AttnPlan plan_attention(const tms_cache* c, const tms_attention_args* a) {
     AttnPlan p;
-    const int rows = min(c->max_q, c->tokens) * (a->q_heads / c->kv_heads);
-    p.chunk = rows > 64 && short_strides(c, c->k_stride) && short_strides(c, c->v_stride);
-    p.rm = p.chunk ? kChunkRows : rows <= 32 || c->head_dim > 128 ? 32 : 64;
+    const int rows = p.rows = min(c->max_q, c->tokens) * (a->q_heads / c->kv_heads);
+    p.chunk = rows > kShareRows && short_strides(c, c->k_stride) && short_strides(c, c->v_stride);
+    p.rm = p.chunk ? kChunkRows : kShareRows;
     p.row_tiles = (rows + p.rm - 1) / p.rm;
     int64_t keys = min(c->max_kv, kMaxLen);
     if (a->window > 0) keys = std::min<int64_t>(keys, (int64_t)a->window + p.rm + a->sinks + 128);
@@ -485,21 +511,24 @@ static AttnPlan plan_attention(const tms_cache* c, const tms_attention_args* a) 
     p.splits = p.shares = 0;
     p.item_bytes = 0;
     if (p.chunk) {
-        // Workgroups enough for two a CU, with 16 tiles each at least.
+        // Workgroups enough for two a CU, with 4 tiles each at least.
         const int kt = chunk_keys(c->head_dim);
         const int tiles = (int)((keys + kt - 1) / kt);
         const int64_t want = std::max<int64_t>(1, 512 / std::max<int64_t>(items, 1));
-        p.split_tiles = (int)std::max<int64_t>((tiles + want - 1) / want, 16);
+        p.split_tiles = (int)std::max<int64_t>((tiles + want - 1) / want, 4);
         p.splits = std::max(1, (tiles + p.split_tiles - 1) / p.split_tiles);
         p.join = p.splits > 1;
+        p.most_parts = p.splits;
         parts = p.join ? items * p.splits : 0;
     } else {
-        const int64_t tiles = std::max<int64_t>((keys + 31) / 32, 1) * items;
-        p.split_tiles = 16;
-        p.shares = (int)std::min<int64_t>(c->head_dim > 128 ? 256 : 512, std::max<int64_t>(1, (tiles + p.split_tiles - 1) / p.split_tiles));
-        p.join = true;
-        parts = 2 * (int64_t)p.shares;
-        p.item_bytes = (size_t)(items * 8 + 15) / 16 * 16;
+        const int64_t tiles = std::max<int64_t>((keys + 31) / 32, 1);
+        p.waves = c->head_dim <= 128 && tiles <= kWholeTiles ? 8 : 4;
+        p.join = p.waves == 4;
+        p.split_tiles = p.join ? 16 : 0;
+        p.shares = (int)(p.join ? std::min<int64_t>(c->head_dim > 128 ? 256 : 512, (tiles * items + p.split_tiles - 1) / p.split_tiles) : items);
+        parts = p.join ? 2 * (int64_t)p.shares : 0;
+        p.most_parts = (int)std::min<int64_t>(tiles / 16 + 2, p.shares);
+        p.item_bytes = p.join ? (size_t)(items * 8 + 15) / 16 * 16 : 0;
     }
     p.o_bytes = (size_t)parts * p.rm * c->head_dim * 4;
     p.ml_bytes = (size_t)parts * p.rm * 8;
@@ -509,12 +538,21 @@ static AttnPlan plan_attention(const tms_cache* c, const tms_attention_args* a) 
 template <typename T, int ROWB, int KS, int DT>
 static void launch_rows(const AttnPlan& p, const AttnParams& a, hipStream_t stream) {
     if constexpr (ROWB <= 256) {
-        if (p.rm == 64) {
-            hipLaunchKernelGGL((attn_rows_kernel<T, ROWB, KS, DT, 2>), dim3(p.shares), dim3(256), 0, stream, a);
+        if (p.waves == 8) {
+            hipLaunchKernelGGL((attn_rows_kernel<T, ROWB, KS, DT, 8>), dim3(p.shares), dim3(512), 0, stream, a);
             return;
         }
     }
-    hipLaunchKernelGGL((attn_rows_kernel<T, ROWB, KS, DT, 1>), dim3(p.shares), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((attn_rows_kernel<T, ROWB, KS, DT, 4>), dim3(p.shares), dim3(256), 0, stream, a);
+}
+
+template <typename T, int LPR>
+static void launch_join(const AttnPlan& p, const AttnParams& a, int pairs, hipStream_t stream) {
+    int sub = 1;
+    while (sub < 256 / LPR && sub < p.most_parts) sub *= 2;
+    const int n_in = 256 / LPR / sub;
+    hipLaunchKernelGGL((attn_join_kernel<T, LPR>), dim3(pairs, p.row_tiles, (std::min(p.rm, p.rows) + n_in - 1) / n_in), dim3(256), 0, stream, a,
+                       p.rm, sub);
 }
 
 template <typename T>
@@ -525,8 +563,10 @@ static void launch_attention(const AttnPlan& p, const AttnParams& a, hipStream_t
     else if (D <= 96) launch_rows<T, 256, 6, 3>(p, a, stream);
     else if (D <= 128) launch_rows<T, 256, 8, 4>(p, a, stream);
     else launch_rows<T, 512, 16, 8>(p, a, stream);
-    if (p.join)
-        hipLaunchKernelGGL((attn_join_kernel<T>), dim3(pairs, p.row_tiles, (p.rm + 3) / 4), dim3(256), 0, stream, a, p.rm);
+    if (!p.join) return;
+    if (D <= 64) launch_join<T, 16>(p, a, pairs, stream);
+    else if (D <= 128) launch_join<T, 32>(p, a, pairs, stream);
+    else launch_join<T, 64>(p, a, pairs, stream);
 }
 
 }  // namespace tms
