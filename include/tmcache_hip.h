@@ -39,6 +39,8 @@ extern "C" {
 #define TMS_CACHE_MAX_HEAD_DIM 256
 #define TMS_CACHE_MIN_PAGE 8
 #define TMS_CACHE_MAX_PAGE 65536
+#define TMS_ATTENTION_MAX_SLOT_STRIDE 67108864   /* elements; tms_paged_attention */
+#define TMS_ATTENTION_MAX_ROWS 2097152           /* max_q times query heads a key head */
 
 /* The pools, page tables and lengths of one call. */
 typedef struct tms_cache {
@@ -89,7 +91,7 @@ int tms_kv_append(const tms_cache* cache, const tms_append_args* args, hipStream
  *   s_j = scale * q . k_j,  lse = log(sum_j exp(s_j)),
  *   out = sum_j exp(s_j - lse) v_j.
  * A row that sees nothing (or every s_j = -inf) gives out = 0, lse = -inf.
- * Sums and products are held in fp32; the weights are rounded once to the
+ * scale is any finite number.  Sums and products are held in fp32; the weights are rounded once to the
  * cache's dtype for the product with v, the output once at the end.  The
  * same inputs give the same bits on every call.
  */
@@ -185,8 +187,10 @@ typedef struct tms_adjust_args {
     int64_t out_stride;
     const tms_row_params* params;   /* device, [seqs]; nullable: no penalties */
     const int32_t* recent;    /* device, [seqs][recent_stride], nullable */
-    const int32_t* n_recent;  /* device, [seqs], nullable: all recent_stride */
-    int64_t recent_stride;
+    const int32_t* n_recent;  /* device, [seqs], nullable: all n_history */
+    int64_t recent_stride;    /* >= n_history */
+    int32_t n_history;        /* ids that a sequence's row of `recent` holds */
+    int32_t reserved;         /* must be 0 */
     const int32_t* drafts;    /* device, [seqs][steps - 1], nullable: none counted */
     const int32_t* bias_ids;  /* device, [seqs][n_bias], nullable with n_bias = 0 */
     const float* bias_values; /* device, [seqs][n_bias] */

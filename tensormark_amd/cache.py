@@ -17,6 +17,7 @@ refuses; there is no fallback.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 from typing import Optional
@@ -82,7 +83,7 @@ class AdjustArgs(C.Structure):
         ("logits", C.c_void_p), ("out", C.c_void_p), ("dtype", C.c_int32), ("out_dtype", C.c_int32),
         ("seqs", C.c_int32), ("steps", C.c_int32), ("vocab", C.c_int32), ("n_bias", C.c_int32),
         ("row_stride", C.c_int64), ("out_stride", C.c_int64), ("params", C.c_void_p),
-        ("recent", C.c_void_p), ("n_recent", C.c_void_p), ("recent_stride", C.c_int64),
+        ("recent", C.c_void_p), ("n_recent", C.c_void_p), ("recent_stride", C.c_int64), ("n_history", C.c_int32), ("reserved", C.c_int32),
         ("drafts", C.c_void_p), ("bias_ids", C.c_void_p), ("bias_values", C.c_void_p),
         ("mask", C.c_void_p), ("mask_stride", C.c_int64),
     ]
@@ -108,10 +109,24 @@ def _fns():
     return _FNS
 
 
-def _stream(stream, t) -> C.c_void_p:
+def _stream(stream, device: int):
+    """The stream to run on, as an address."""
+    if stream is not None:
+        return stream
     import torch
 
-    return C.c_void_p(stream if stream is not None else torch.cuda.current_stream(t.device).cuda_stream)
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+class _On:
+    """Allocations within are ordered with the work of the caller's `stream`."""
+
+    def __new__(cls, stream, device: int):
+        import torch
+
+        if stream is None:
+            return contextlib.nullcontext()
+        return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device))
 
 
 def _want(ok: bool, what: str) -> None:
@@ -119,65 +134,72 @@ def _want(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def _ints(t, shape, what, like):
-    """A contiguous int32 tensor of that shape on the pool's device; its address."""
+def _ints(t, shape, what, device: int):
+    """The address of a contiguous int32 tensor of that shape on the device."""
     import torch
 
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != like.device:
-        raise ValueError(f"{what}: a contiguous int32 tensor {list(shape)} on {like.device}, not {t.dtype} {list(t.shape)} on {t.device}")
+    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous() or t.get_device() != device:
+        raise ValueError(f"{what}: a contiguous int32 tensor {list(shape)} on cuda:{device}, not {t.dtype} {list(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _cache(k, v, scores, tables, kv_len, q_start, tokens, max_q, max_kv) -> CacheArgs:
+# Only addresses, sizes and strides are read here, once each: a decode step is
+# short enough for its calls' host time to count.
+def _cache(k, v, scores, tables, kv_len, q_start, tokens, max_q, max_kv):
+    """The call's tms_cache and its device's index."""
     import torch
 
-    _want(k.dim() == 4 and k.shape[0] >= 1, "k_cache: [pages, kv_heads, page_size, head_dim]")
-    _want(k.dtype in (torch.bfloat16, torch.float16), f"k_cache: bfloat16 or float16, not {k.dtype}")
-    _want(k.is_cuda, "k_cache: a device tensor")
-    _want(k.stride(3) == 1, "k_cache: the last stride must be 1")
-    c = CacheArgs()
-    c.k, c.dtype = k.data_ptr(), DTYPE_BF16 if k.dtype == torch.bfloat16 else DTYPE_F16
-    c.pages, c.kv_heads, c.page_size, c.head_dim = k.shape
-    c.k_stride[0], c.k_stride[1], c.k_stride[2] = k.stride()[:3]
+    device, dtype, shape, stride = k.get_device(), k.dtype, k.shape, k.stride()
+    _want(len(shape) == 4 and shape[0] >= 1, "k_cache: [pages, kv_heads, page_size, head_dim]")
+    code = DTYPE_BF16 if dtype == torch.bfloat16 else DTYPE_F16
+    if dtype != torch.bfloat16 and dtype != torch.float16:
+        raise ValueError(f"k_cache: bfloat16 or float16, not {dtype}")
+    _want(device >= 0, "k_cache: a device tensor")
+    _want(stride[3] == 1, "k_cache: the last stride must be 1")
+    vp, vs = None, (0, 0, 0)
     if v is not None:
-        _want(v.shape == k.shape and v.dtype == k.dtype and v.device == k.device and v.stride(3) == 1,
-              "v_cache: like k_cache")
-        c.v = v.data_ptr()
-        c.v_stride[0], c.v_stride[1], c.v_stride[2] = v.stride()[:3]
+        vs = v.stride()
+        _want(v.shape == shape and v.dtype == dtype and v.get_device() == device and vs[3] == 1, "v_cache: like k_cache")
+        vp, vs = v.data_ptr(), vs[:3]
+    sp = None
     if scores is not None:
-        _want(scores.dtype == torch.float32 and scores.shape == k.shape[:3] and scores.is_contiguous() and
-              scores.device == k.device, "scores: contiguous float32 [pages, kv_heads, page_size]")
-        c.scores = scores.data_ptr()
-    _want(tables.dim() == 2 and tables.dtype == torch.int32 and tables.device == k.device and
-          (tables.stride(1) == 1 or tables.shape[1] <= 1) and tables.shape[1] >= 1, "tables: int32 [batch, entries], rows contiguous")
-    c.batch, c.tables = tables.shape[0], tables.data_ptr()
-    _want(tables.shape[0] <= 1 or tables.stride(0) == tables.shape[1], "tables: contiguous")
-    c.table_stride = tables.shape[1]
-    c.kv_len = _ints(kv_len, (c.batch,), "kv_len", k)
-    if q_start is not None:
-        c.q_start = _ints(q_start, (c.batch + 1,), "q_start", k)
-    c.tokens, c.max_q, c.max_kv = tokens, max_q, max_kv
-    return c
+        _want(scores.dtype == torch.float32 and scores.shape == shape[:3] and scores.is_contiguous() and
+              scores.get_device() == device, "scores: contiguous float32 [pages, kv_heads, page_size]")
+        sp = scores.data_ptr()
+    _want(tables.dtype == torch.int32 and tables.get_device() == device and tables.dim() == 2 and tables.is_contiguous() and
+          tables.shape[1] >= 1, "tables: contiguous int32 [batch, entries]")
+    batch, entries = tables.shape
+    return CacheArgs(k.data_ptr(), vp, sp, stride[:3], vs, code, *shape[:3], shape[3], batch, tables.data_ptr(), entries,
+                     _ints(kv_len, (batch,), "kv_len", device),
+                     None if q_start is None else _ints(q_start, (batch + 1,), "q_start", device), tokens, max_q, max_kv, 0), device
 
 
 def _rows(t, k, what):
-    """[tokens, heads, head_dim] rows of the cache's type; its token and head strides."""
-    _want(t.dim() == 3 and t.dtype == k.dtype and t.device == k.device and t.shape[2] == k.shape[3] and
-          (t.stride(2) == 1 or t.shape[2] == 1), f"{what}: [tokens, heads, {k.shape[3]}] of {k.dtype} on {k.device}, last stride 1")
-    return t.stride(0), t.stride(1)
+    """The token and head strides of [tokens, heads, head_dim] rows of the cache's type."""
+    D, st = k.shape[-1], t.stride()
+    if len(st) != 3 or t.dtype != k.dtype or t.get_device() != k.get_device() or t.shape[2] != D or st[2] != 1:
+        raise ValueError(f"{what}: [tokens, heads, {D}] of {k.dtype} on {k.device}, last stride 1")
+    return st[:2]
+
+
+def _f32_rows(t, rows, what, device: int):
+    """The address of a contiguous float32 [tokens, q_heads]."""
+    import torch
+
+    if t.dtype != torch.float32 or t.shape != rows or not t.is_contiguous() or t.get_device() != device:
+        raise ValueError(f"{what}: contiguous float32 [tokens, q_heads]")
+    return t.data_ptr()
 
 
 def kv_append(k_new, v_new, k_cache, v_cache, tables, kv_len, q_start, *, max_q: int, scores=None, stream=None) -> None:
     """Write new tokens' keys and values (``[tokens, kv_heads, head_dim]``) to
     their slots, the last positions of each sequence's ``kv_len``; their slots' scores
     become 0.  Tokens without a mapped slot are dropped."""
-    c = _cache(k_cache, v_cache, scores, tables, kv_len, q_start, k_new.shape[0], max_q, 0)
-    a = AppendArgs()
-    a.k_new_stride[0], a.k_new_stride[1] = _rows(k_new, k_cache, "k_new")
-    a.v_new_stride[0], a.v_new_stride[1] = _rows(v_new, k_cache, "v_new")
+    c, device = _cache(k_cache, v_cache, scores, tables, kv_len, q_start, k_new.shape[0], max_q, 0)
+    ks, vs = _rows(k_new, k_cache, "k_new"), _rows(v_new, k_cache, "v_new")
     _want(k_new.shape == v_new.shape and k_new.shape[1] == k_cache.shape[1], "k_new, v_new: one row a key head")
-    a.k_new, a.v_new = k_new.data_ptr(), v_new.data_ptr()
-    _check(_fns().tms_kv_append(C.byref(c), C.byref(a), _stream(stream, k_cache)), "tms_kv_append")
+    a = AppendArgs(k_new.data_ptr(), v_new.data_ptr(), ks, vs)
+    _check(_fns().tms_kv_append(C.byref(c), C.byref(a), _stream(stream, device)), "tms_kv_append")
 
 
 def paged_attention(q, k_cache, v_cache, tables, kv_len, q_start, *, max_q: int, max_kv: int, window: int = 0,
@@ -189,30 +211,25 @@ def paged_attention(q, k_cache, v_cache, tables, kv_len, q_start, *, max_q: int,
     out 0, where a row sees nothing).  ``scale`` is 1 / sqrt(head_dim) by default."""
     import torch
 
-    c = _cache(k_cache, v_cache, None, tables, kv_len, q_start, q.shape[0], max_q, max_kv)
-    a = AttentionArgs()
-    a.q_stride[0], a.q_stride[1] = _rows(q, k_cache, "q")
+    qs = _rows(q, k_cache, "q")
     T, H, D = q.shape
-    if out is None:
-        out = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
-    a.out_stride[0], a.out_stride[1] = _rows(out, k_cache, "out")
-    if lse is None:
-        lse = torch.empty((T, H), dtype=torch.float32, device=q.device)
-    _want(out.shape == q.shape, "out: like q")
-    _want(lse.dtype == torch.float32 and lse.shape == (T, H) and lse.is_contiguous() and lse.device == q.device,
-          "lse: contiguous float32 [tokens, q_heads]")
-    a.q, a.out, a.lse, a.q_heads = q.data_ptr(), out.data_ptr(), lse.data_ptr(), H
-    a.window, a.sinks, a.scale = max(window, 0), sinks, 1.0 / math.sqrt(D) if scale is None else scale
-    lib = _fns()
-    need = lib.tms_paged_attention_workspace(C.byref(c), C.byref(a))
-    if need < 0:
-        _check(int(need), "tms_paged_attention")
-    if need > 0:
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), need
-        if stream is not None:
-            ws.record_stream(torch.cuda.ExternalStream(stream, device=q.device))
-    _check(lib.tms_paged_attention(C.byref(c), C.byref(a), _stream(stream, q)), "tms_paged_attention")
+    c, device = _cache(k_cache, v_cache, None, tables, kv_len, q_start, T, max_q, max_kv)
+    with _On(stream, device):
+        if out is None:
+            out = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
+        if lse is None:
+            lse = torch.empty((T, H), dtype=torch.float32, device=q.device)
+        _want(out.shape == q.shape, "out: like q")
+        a = AttentionArgs(q.data_ptr(), out.data_ptr(), _f32_rows(lse, (T, H), "lse", device), qs, _rows(out, k_cache, "out"), H,
+                          max(window, 0), sinks, 1.0 / math.sqrt(D) if scale is None else scale, None, 0)
+        lib = _fns()
+        need = lib.tms_paged_attention_workspace(C.byref(c), C.byref(a))
+        if need < 0:
+            _check(need, "tms_paged_attention")
+        if need > 0:
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), need
+        _check(lib.tms_paged_attention(C.byref(c), C.byref(a), _stream(stream, device)), "tms_paged_attention")
     return out, lse
 
 
@@ -223,21 +240,16 @@ def kv_add_scores(q, lse, k_cache, scores, tables, kv_len, q_start, *, max_q: in
     ``lse``, ``window``, ``sinks`` and ``scale`` are those of the paged_attention call.
     ``out`` (like ``scores``, default ``scores`` itself) is returned; every mapped position
     is written there, nothing else."""
-    import torch
-
     _want(scores is not None, "scores: needed")
-    c = _cache(k_cache, None, scores, tables, kv_len, q_start, q.shape[0], max_q, max_kv)
-    a = ScoreArgs()
-    a.q_stride[0], a.q_stride[1] = _rows(q, k_cache, "q")
-    _want(lse.dtype == torch.float32 and lse.shape == q.shape[:2] and lse.is_contiguous() and lse.device == q.device,
-          "lse: contiguous float32 [tokens, q_heads]")
+    qs, (T, H, D) = _rows(q, k_cache, "q"), q.shape
+    c, device = _cache(k_cache, None, scores, tables, kv_len, q_start, T, max_q, max_kv)
     if out is None:
         out = scores
-    _want(out.dtype == torch.float32 and out.shape == scores.shape and out.is_contiguous() and out.device == q.device,
+    _want(out.dtype == scores.dtype and out.shape == scores.shape and out.is_contiguous() and out.get_device() == device,
           "out: like scores")
-    a.q, a.lse, a.out, a.q_heads = q.data_ptr(), lse.data_ptr(), out.data_ptr(), q.shape[1]
-    a.window, a.sinks, a.scale = max(window, 0), sinks, 1.0 / math.sqrt(q.shape[2]) if scale is None else scale
-    _check(_fns().tms_kv_add_scores(C.byref(c), C.byref(a), _stream(stream, q)), "tms_kv_add_scores")
+    a = ScoreArgs(q.data_ptr(), _f32_rows(lse, (T, H), "lse", device), out.data_ptr(), qs, H, max(window, 0), sinks,
+                  1.0 / math.sqrt(D) if scale is None else scale)
+    _check(_fns().tms_kv_add_scores(C.byref(c), C.byref(a), _stream(stream, device)), "tms_kv_add_scores")
     return out
 
 
@@ -251,19 +263,18 @@ def kv_evict(k_cache, v_cache, scores, tables, kv_len, dst_tables, *, budget: in
     import torch
 
     _want(scores is not None, "scores: needed")
-    c = _cache(k_cache, v_cache, scores, tables, kv_len, None, 0, 0, max_kv)
-    _want(dst_tables.dim() == 2 and dst_tables.shape[0] == c.batch, "dst_tables: int32 [batch, entries]")
-    a = EvictArgs()
-    a.dst_tables = _ints(dst_tables, tuple(dst_tables.shape), "dst_tables", k_cache)
-    a.dst_table_stride, a.budget, a.sinks, a.recent = dst_tables.shape[1], budget, sinks, recent
+    c, device = _cache(k_cache, v_cache, scores, tables, kv_len, None, 0, 0, max_kv)
+    B, H = tables.shape[0], k_cache.shape[1]
+    _want(dst_tables.dim() == 2 and dst_tables.shape[0] == B, "dst_tables: int32 [batch, entries]")
     _want(budget >= 1, "budget: at least 1")
-    if new_len is None:
-        new_len = torch.empty(c.batch, dtype=torch.int32, device=k_cache.device)
-    if kept is None:
-        kept = torch.empty((c.batch, c.kv_heads, budget), dtype=torch.int32, device=k_cache.device)
-    a.new_len = _ints(new_len, (c.batch,), "new_len", k_cache)
-    a.kept = _ints(kept, (c.batch, c.kv_heads, budget), "kept", k_cache)
-    _check(_fns().tms_kv_evict(C.byref(c), C.byref(a), _stream(stream, k_cache)), "tms_kv_evict")
+    with _On(stream, device):
+        if new_len is None:
+            new_len = torch.empty(B, dtype=torch.int32, device=k_cache.device)
+        if kept is None:
+            kept = torch.empty((B, H, budget), dtype=torch.int32, device=k_cache.device)
+        a = EvictArgs(_ints(dst_tables, dst_tables.shape, "dst_tables", device), dst_tables.shape[1], budget, sinks, recent, 0,
+                      _ints(new_len, (B,), "new_len", device), _ints(kept, (B, H, budget), "kept", device))
+        _check(_fns().tms_kv_evict(C.byref(c), C.byref(a), _stream(stream, device)), "tms_kv_evict")
     return new_len, kept
 
 
@@ -281,48 +292,54 @@ def adjust_logits(logits, params=None, *, recent=None, n_recent=None, drafts=Non
     words ``[seqs * steps, ceil(vocab / 32)]``, masked ids become -inf."""
     import torch
 
-    code = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
-    _want(logits.dim() == 2 and logits.dtype in code and logits.is_cuda and (logits.stride(1) == 1 or logits.shape[1] == 1),
+    dtype, device = logits.dtype, logits.get_device()
+    _want(logits.dim() == 2 and dtype in (torch.float32, torch.float16, torch.bfloat16) and device >= 0 and
+          (logits.stride(1) == 1 or logits.shape[1] == 1),
           "logits: device [rows, vocab] of float32, float16 or bfloat16, last stride 1")
     R, V = logits.shape
     _want(steps >= 1 and R % steps == 0, "logits: a multiple of `steps` rows")
     S = R // steps
-    if out is None:
-        out = torch.empty((R, V), dtype=logits.dtype, device=logits.device)
-    _want(out.shape == logits.shape and out.dtype in (logits.dtype, torch.float32) and out.device == logits.device and
-          (out.stride(1) == 1 or V == 1), "out: like logits, of its type or float32")
     a = AdjustArgs()
-    a.logits, a.out, a.dtype, a.out_dtype = logits.data_ptr(), out.data_ptr(), code[logits.dtype], code[out.dtype]
+    a.dtype = a.out_dtype = DTYPE_F32 if dtype == torch.float32 else DTYPE_F16 if dtype == torch.float16 else DTYPE_BF16
     a.seqs, a.steps, a.vocab = S, steps, V
-    a.row_stride = logits.stride(0) if R > 1 else V
-    a.out_stride = out.stride(0) if R > 1 else V
+    a.row_stride = a.out_stride = V
+    if R > 1:
+        a.row_stride = logits.stride(0)
     if params is not None:
         _want(params.dtype == torch.uint8 and params.is_contiguous() and params.numel() == S * ROW_DTYPE.itemsize and
-              params.device == logits.device, "params: uint8 ROW_DTYPE records, one a sequence")
+              params.get_device() == device, "params: uint8 ROW_DTYPE records, one a sequence")
         a.params = params.data_ptr()
     if recent is not None:
-        _want(recent.dim() == 2 and recent.shape[0] == S, "recent: int32 [seqs, n]")
-        _want(recent.dtype == torch.int32 and recent.device == logits.device and (recent.stride(1) == 1 or recent.shape[1] <= 1),
-              "recent: int32 rows on the logits' device")
-        a.recent, a.recent_stride = recent.data_ptr(), recent.stride(0) if S > 1 else recent.shape[1]
+        _want(recent.dim() == 2 and recent.shape[0] == S and recent.dtype == torch.int32 and recent.get_device() == device and
+              (recent.stride(1) == 1 or recent.shape[1] <= 1) and (S <= 1 or recent.stride(0) >= recent.shape[1]),
+              "recent: int32 [seqs, n] on the logits' device, rows contiguous")
+        a.recent, a.recent_stride, a.n_history = recent.data_ptr(), recent.stride(0) if S > 1 else recent.shape[1], recent.shape[1]
         if n_recent is not None:
-            a.n_recent = _ints(n_recent, (S,), "n_recent", logits)
-        elif a.recent_stride != recent.shape[1]:
-            n_recent = torch.full((S,), recent.shape[1], dtype=torch.int32, device=logits.device)
-            a.n_recent = n_recent.data_ptr()
+            a.n_recent = _ints(n_recent, (S,), "n_recent", device)
     if drafts is not None and steps > 1:
-        a.drafts = _ints(drafts, (S, steps - 1), "drafts", logits)
+        a.drafts = _ints(drafts, (S, steps - 1), "drafts", device)
     _want((bias_ids is None) == (bias_values is None), "bias_ids and bias_values go together")
     if bias_ids is not None and bias_ids.numel():
         n = bias_ids.shape[-1]
-        a.n_bias, a.bias_ids = n, _ints(bias_ids, (S, n), "bias_ids", logits)
-        _want(bias_values.dtype == torch.float32 and tuple(bias_values.shape) == (S, n) and bias_values.is_contiguous() and
-              bias_values.device == logits.device, "bias_values: contiguous float32, like bias_ids")
+        a.n_bias, a.bias_ids = n, _ints(bias_ids, (S, n), "bias_ids", device)
+        _want(bias_values.dtype == torch.float32 and bias_values.shape == (S, n) and bias_values.is_contiguous() and
+              bias_values.get_device() == device, "bias_values: contiguous float32, like bias_ids")
         a.bias_values = bias_values.data_ptr()
     if mask is not None:
         _want(mask.dim() == 2 and mask.shape[0] == R and mask.element_size() == 4 and not mask.is_floating_point() and
-              (mask.stride(1) == 1 or mask.shape[1] == 1) and mask.device == logits.device and mask.shape[1] >= (V + 31) // 32,
+              (mask.stride(1) == 1 or mask.shape[1] == 1) and mask.get_device() == device and mask.shape[1] >= (V + 31) // 32,
               "mask: 32-bit words [rows, ceil(vocab / 32)]")
         a.mask, a.mask_stride = mask.data_ptr(), mask.stride(0) if R > 1 else mask.shape[1]
-    _check(_fns().tms_adjust_logits(C.byref(a), _stream(stream, logits)), "tms_adjust_logits")
+    with _On(stream, device):
+        if out is None:
+            out = torch.empty((R, V), dtype=dtype, device=logits.device)
+        else:
+            _want(out.shape == logits.shape and out.dtype in (dtype, torch.float32) and out.get_device() == device and
+                  (out.stride(1) == 1 or V == 1), "out: like logits, of its type or float32")
+            if out.dtype != dtype:
+                a.out_dtype = DTYPE_F32
+            if R > 1:
+                a.out_stride = out.stride(0)
+        a.logits, a.out = logits.data_ptr(), out.data_ptr()
+        _check(_fns().tms_adjust_logits(C.byref(a), _stream(stream, device)), "tms_adjust_logits")
     return out

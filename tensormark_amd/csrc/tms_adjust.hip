@@ -28,6 +28,7 @@ struct AdjustParams {
     const int32_t* recent;
     const int32_t* n_recent;
     int64_t rstride;
+    int history;
     const int32_t* drafts;
     const int32_t* bias_ids;
     const float* bias_values;
@@ -86,7 +87,7 @@ __global__ __launch_bounds__(256) void adjust_kernel(AdjustParams a) {
         pn.rep = P.repeat_penalty;
         pn.freq = P.frequency_penalty;
         pn.pres = P.presence_penalty;
-        if (a.recent) have = min(max(a.n_recent ? a.n_recent[seq] : (int)a.rstride, 0), (int)a.rstride);
+        if (a.recent) have = min(max(a.n_recent ? a.n_recent[seq] : a.history, 0), a.history);
         total = have + (a.drafts ? step : 0);
         pn.on = total > 0 && P.repeat_last_n > 0 && (pn.rep_on || pn.fp_on);
         from = total > P.repeat_last_n ? total - P.repeat_last_n : 0;
@@ -175,10 +176,10 @@ extern "C" int tms_adjust_logits(const tms_adjust_args* args, hipStream_t stream
     if (p.dtype < TMS_DTYPE_F32 || p.dtype > TMS_DTYPE_BF16 || (p.out_dtype != p.dtype && p.out_dtype != TMS_DTYPE_F32))
         return TMS_ERR_INVALID_ARG;
     if (p.seqs < 0 || p.steps < 1 || p.vocab < 1 || p.n_bias < 0 || p.row_stride < p.vocab || p.out_stride < p.vocab ||
-        p.recent_stride < 0)
+        p.n_history < 0 || p.recent_stride < p.n_history || p.reserved != 0)
         return TMS_ERR_INVALID_ARG;
     const int64_t rows = (int64_t)p.seqs * p.steps;
-    if (p.vocab > 1048576 || p.n_bias > 65535 || rows > 65535 || p.recent_stride > (1 << 28)) return TMS_ERR_CAPACITY;
+    if (p.vocab > 1048576 || p.n_bias > 65535 || rows > 65535 || p.n_history > (1 << 28)) return TMS_ERR_CAPACITY;
     if (rows == 0) return TMS_OK;
     if (!p.logits || !p.out || (p.n_bias && (!p.bias_ids || !p.bias_values)) ||
         (p.mask && p.mask_stride < (p.vocab + 31) / 32))
@@ -198,6 +199,7 @@ extern "C" int tms_adjust_logits(const tms_adjust_args* args, hipStream_t stream
     a.recent = p.recent;
     a.n_recent = p.n_recent;
     a.rstride = p.recent_stride;
+    a.history = p.n_history;
     a.drafts = p.drafts;
     a.bias_ids = p.bias_ids;
     a.bias_values = p.bias_values;

@@ -25,6 +25,10 @@
 namespace tms {
 
 constexpr int kShareRows = 32;   // of a workgroup of the rows kernel
+// What an item takes besides its tiles, in tiles (64 sequences of 40 to 2000
+// positions: 90 us with 0, 59 with 4, 56 with 8, 60 with 32), and the shortest
+// share in tiles: one for each wave.
+constexpr int kItemCost = 8, kLeastShare = 4;
 
 // ---- few rows: the keys of all sequences in equal shares ---------------------------------------
 //
@@ -39,13 +43,16 @@ constexpr int kShareRows = 32;   // of a workgroup of the rows kernel
 // loaded there while the values of the one before are used, and its values
 // while its keys are, so that 8 waves a CU keep some 100 KB on the way without
 // a register for it.  No wave waits for another before the item's end.
+// An item's tiles (one at least: rows that see nothing have an output all the
+// same) and what it takes besides, as tiles.
+__device__ __forceinline__ int item_length(const AttnParams& a, int tiles) { return max(tiles, 1) + kItemCost; }
+
 __device__ __forceinline__ int item_tiles(const AttnParams& a, int combo) {
     const int b = combo / a.row_tiles, tile = combo - b * a.row_tiles;
     const SeqView sq = seq_view(a.c, b);
     const int G = a.group, rows = sq.n * G, r0 = tile * kShareRows;
     if (r0 >= rows) return 0;
-    // (rows that see nothing have an output all the same)
-    return max(TileList<32>(a.window, a.sinks, sq.p0 + r0 / G, sq.p0 + (min(r0 + kShareRows, rows) - 1) / G, sq.len).n, 1);
+    return item_length(a, TileList<32>(a.window, a.sinks, sq.p0 + r0 / G, sq.p0 + (min(r0 + kShareRows, rows) - 1) / G, sq.len).n);
 }
 
 __device__ __forceinline__ int64_t share_of(const AttnParams& a, int64_t total, int shares) {
@@ -142,19 +149,23 @@ __global__ __launch_bounds__(64 * NW, ROWB > 256 ? 1 : 2) void attn_rows_kernel(
         const int nr = min(RM, rows - r0);
         const int pfirst = sq.p0 + r0 / G, plast = sq.p0 + (r0 + nr - 1) / G;
         const TileList<KT> tl(a.window, a.sinks, pfirst, plast, sq.len);
-        const int n = max(tl.n, 1);
-        if (a.split_tiles == 0) {
-            x = at = (int64_t)(blockIdx.x - combo * H) * n;   // (only this item, by its own axis)
-            at = 0;
-            end = x + n;
-        } else if (x >= at + (int64_t)n * H) {
-            at += (int64_t)n * H;
-            ++combo;
-            continue;
+        const int n = max(tl.n, 1), axis = item_length(a, tl.n);
+        int h = blockIdx.x - combo * H, k0 = 0, k1 = n;
+        int64_t item = 0;
+        if (a.split_tiles > 0) {
+            if (x >= at + (int64_t)axis * H) {
+                at += (int64_t)axis * H;
+                ++combo;
+                continue;
+            }
+            h = (int)((x - at) / axis);
+            item = at + (int64_t)h * axis;
+            k0 = (int)(x - item);
+            k1 = (int)min((int64_t)n, end - item);
+            x = min(item + axis, end);
+            if (k0 >= n) continue;
         }
-        const int h = (int)((x - at) / n);
-        const int64_t item = at + (int64_t)h * n;
-        const int k0 = (int)(x - item), k1 = (int)min((int64_t)n, end - item), kend = min(k1, tl.n);
+        const int kend = min(k1, tl.n);
 
         const int r = r0 + n32;
         const bool in = r < rows;
@@ -372,7 +383,6 @@ __global__ __launch_bounds__(64 * NW, ROWB > 256 ? 1 : 2) void attn_rows_kernel(
         }
         if (a.split_tiles == 0) return;
         __syncthreads();
-        x = item + k1;
     }
 }
 
@@ -472,6 +482,9 @@ static bool short_strides(const tms_cache* c, const int64_t* stride) {
     return 2 * stride[0] < (int64_t)1 << 32 && 2 * stride[2] * c->page_size < (int64_t)1 << 32;
 }
 
+// Up to this many tiles a workgroup of eight waves takes an item whole, with
+// nothing to join (64 sequences of 40 to 1000 positions: 34 us, 35 in shares;
+// one of 500: 12 and 14; one of 1000: 16 and 14).
 constexpr int kWholeTiles = 32;
 
 struct AttnPlan {
@@ -492,7 +505,8 @@ static int check_attention(const tms_cache* c, const tms_attention_args* a) {
     if (!a || a->q_heads < 1 || a->q_heads % c->kv_heads || a->sinks < 0 || !std::isfinite(a->scale)) return TMS_ERR_INVALID_ARG;
     for (int i = 0; i < 2; ++i)
         if (a->q_stride[i] < 0 || a->q_stride[i] % 8 || a->out_stride[i] < 0 || a->out_stride[i] % 8) return TMS_ERR_INVALID_ARG;
-    if ((int64_t)c->max_q * (a->q_heads / c->kv_heads) > (1 << 24)) return TMS_ERR_CAPACITY;
+    if ((int64_t)c->max_q * (a->q_heads / c->kv_heads) > TMS_ATTENTION_MAX_ROWS) return TMS_ERR_CAPACITY;
+    if (c->k_stride[2] >= TMS_ATTENTION_MAX_SLOT_STRIDE || c->v_stride[2] >= TMS_ATTENTION_MAX_SLOT_STRIDE) return TMS_ERR_CAPACITY;
     if (c->tokens > 0 && c->batch > 0 && (!a->q || !a->out || !aligned16(a->q) || !aligned16(a->out) || ((uintptr_t)a->lse & 3)))
         return TMS_ERR_INVALID_ARG;
     return TMS_OK;
@@ -522,12 +536,12 @@ static AttnPlan plan_attention(const tms_cache* c, const tms_attention_args* a) 
         parts = p.join ? items * p.splits : 0;
     } else {
         const int64_t tiles = std::max<int64_t>((keys + 31) / 32, 1);
-        p.waves = c->head_dim <= 128 && tiles <= kWholeTiles ? 8 : 4;
+        p.waves = c->head_dim <= 128 && tiles <= kWholeTiles && items <= 1 << 20 ? 8 : 4;
         p.join = p.waves == 4;
-        p.split_tiles = p.join ? 16 : 0;
-        p.shares = (int)(p.join ? std::min<int64_t>(c->head_dim > 128 ? 256 : 512, (tiles * items + p.split_tiles - 1) / p.split_tiles) : items);
+        p.split_tiles = p.join ? kLeastShare : 0;
+        p.shares = (int)(p.join ? std::min<int64_t>(c->head_dim > 128 ? 256 : 512, (tiles + kItemCost) * items / kLeastShare) : items);
         parts = p.join ? 2 * (int64_t)p.shares : 0;
-        p.most_parts = (int)std::min<int64_t>(tiles / 16 + 2, p.shares);
+        p.most_parts = (int)std::min<int64_t>(tiles / kLeastShare + 2, p.shares);
         p.item_bytes = p.join ? (size_t)(items * 8 + 15) / 16 * 16 : 0;
     }
     p.o_bytes = (size_t)parts * p.rm * c->head_dim * 4;
@@ -584,7 +598,6 @@ extern "C" int tms_paged_attention(const tms_cache* cache, const tms_attention_a
     if (rc != TMS_OK) return rc;
     if (cache->batch == 0 || cache->tokens == 0 || cache->max_q == 0) return TMS_OK;
     const AttnPlan p = plan_attention(cache, args);
-    if (p.row_tiles > 65535) return TMS_ERR_CAPACITY;
     if (args->workspace_bytes < p.o_bytes + p.ml_bytes + p.item_bytes ||
         (p.join && (!args->workspace || !aligned16(args->workspace))))
         return TMS_ERR_INVALID_ARG;
