@@ -4,10 +4,13 @@
 //
 // Bound by memory: a row is read once and written once.  Of its ids only those
 // of the history and of the bias list change otherwise than by the mask, some
-// hundreds among 100,000 and more.  A workgroup takes kChunk ids of a row, and
-// while its logits are on the way puts those ids' counts and biases into LDS,
-// one word each per id of the chunk; a bitmap says which words were set (the
-// others are never read, so nothing is cleared but the bitmap).
+// hundreds among 100,000 and more.  A workgroup takes kAdjChunk ids of a row
+// at a time: while their logits are on the way it puts those ids into a list
+// and a bitmap in LDS, their counts and biases into words of their own (read
+// for ids of the list alone, so nothing is cleared but the bitmap), and works
+// each id out in a thread; the vectors then only take the results.  (Worked out
+// where the vector lies, a wave went through its ids one after another: 288
+// rows of 128256 bf16 in 72 us.)
 #include <algorithm>
 
 #include "tms_device.h"
@@ -23,6 +26,7 @@ struct AdjustParams {
     const char* x;
     char* y;
     int steps, vocab, n_bias;
+    int subs;         // chunks a workgroup
     int64_t xs, ys;   // elements between rows
     const tms_row_params* params;
     const int32_t* recent;
@@ -52,29 +56,46 @@ template <> struct Widen<__bf16> {
 
 // Rows may begin at any element: vectors are moved without an alignment of
 // their own (the memory system takes them at any address).
+template <typename T> struct Vec16 {
+    static constexpr int N = 16 / sizeof(T);
+    typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+};
+
+// A workgroup takes `subs` chunks of a row one after another, the next one's
+// logits on the way meanwhile, and keeps the first kHist ids of the history and
+// the first kBias biases of a thread in registers.
 template <typename TI, typename TO>
 __global__ __launch_bounds__(256) void adjust_kernel(AdjustParams a) {
-    constexpr int VEC = 16 / sizeof(TI), NV = kAdjChunk / (256 * VEC);
-    struct In { TI x[VEC]; };
-    struct Out { TO x[VEC]; };
-    __shared__ uint32_t touched[kAdjChunk / 32];
-    __shared__ uint32_t cnt[kAdjChunk];
-    __shared__ uint32_t bias[kAdjChunk];   // the list's first entry for the id
+    constexpr int VEC = Vec16<TI>::N, NV = kAdjChunk / (256 * VEC), kHist = 4, kBias = 2;
+    typedef typename Vec16<TI>::type In;
+    typedef TO Out __attribute__((ext_vector_type(VEC), aligned(sizeof(TO))));
+    __shared__ uint32_t touched[2][kAdjChunk / 32];
+    __shared__ uint32_t cnt[kAdjChunk];    // an id's count, then its result
+    __shared__ uint32_t bias[kAdjChunk];   // the bias list's first entry for the id
     __shared__ float value[kBiasHeld];     // the first entries' values
+    __shared__ uint16_t list[kAdjChunk];   // the ids that the chunk has
+    __shared__ uint32_t listed[2];
     __shared__ int twice;
+    const float low = -__builtin_huge_valf();
     const int t = threadIdx.x;
     const int r = blockIdx.y, seq = r / a.steps, step = r - seq * a.steps;
-    const int c0 = blockIdx.x * kAdjChunk, n = min(kAdjChunk, a.vocab - c0);
-    const TI* x = (const TI*)a.x + (int64_t)r * a.xs + c0;
-    TO* y = (TO*)a.y + (int64_t)r * a.ys + c0;
+    const TI* row_in = (const TI*)a.x + (int64_t)r * a.xs;
+    TO* row_out = (TO*)a.y + (int64_t)r * a.ys;
+    const uint32_t* mrow = a.mask ? a.mask + (int64_t)r * a.mstride : nullptr;
     In v[NV];
+    uint32_t word[NV];
+    auto load = [&](int c0) __attribute__((always_inline)) {   // a whole chunk
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int i = (k * 256 + t) * VEC;
-        if (i + VEC <= n) __builtin_memcpy(&v[k], x + i, sizeof(In));
-        else
-            for (int e = 0; e < VEC; ++e) v[k].x[e] = i + e < n ? x[i + e] : (TI)0.f;
-    }
+        for (int k = 0; k < NV; ++k) v[k] = *(const In*)(row_in + c0 + (k * 256 + t) * VEC);
+        if (mrow) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) word[k] = mrow[(c0 + (k * 256 + t) * VEC) >> 5];
+        }
+    };
+#pragma unroll
+    for (int k = 0; k < NV; ++k) word[k] = ~0u;
+    const int first = blockIdx.x * a.subs * kAdjChunk, last = min(first + a.subs * kAdjChunk, a.vocab);
+    if (first + kAdjChunk <= a.vocab) load(first);
 
     Pen pn;
     pn.on = pn.rep_on = pn.fp_on = false;
@@ -97,73 +118,110 @@ __global__ __launch_bounds__(256) void adjust_kernel(AdjustParams a) {
     const int32_t* drafts = a.drafts + (int64_t)seq * (a.steps - 1);
     const int32_t* bid = a.bias_ids + (int64_t)seq * a.n_bias;
     const float* bval = a.bias_values + (int64_t)seq * a.n_bias;
-    auto hist = [&](int i) { return (i < have ? recent[i] : drafts[i - have]) - c0; };
-
-    if (t < kAdjChunk / 32) touched[t] = 0;
-    if (t == 0) twice = 0;
-    __syncthreads();
-    for (int i = from + t; i < total; i += 256) {
-        const int id = hist(i);
-        if ((unsigned)id < (unsigned)n) {
-            cnt[id] = 0;
-            bias[id] = ~0u;
-            atomicOr(&touched[id >> 5], 1u << (id & 31));
+    auto hist = [&](int i) { return *(i < have ? recent + i : drafts + (i - have)); };
+    int hid[kHist], bidr[kBias];   // -1: none (no id of a chunk)
+#pragma unroll
+    for (int k = 0; k < kBias; ++k) {
+        const int i = k * 256 + t;
+        bidr[k] = -1;
+        if (i < a.n_bias) {
+            bidr[k] = bid[i];
+            if (i < (int)kBiasHeld) value[i] = bval[i];
         }
     }
-    for (int i = t; i < a.n_bias; i += 256) {
-        const int id = bid[i] - c0;
-        if (i < (int)kBiasHeld) value[i] = bval[i];
-        if ((unsigned)id < (unsigned)n) {
-            cnt[id] = 0;
-            bias[id] = ~0u;
-            atomicOr(&touched[id >> 5], 1u << (id & 31));
-        }
+#pragma unroll
+    for (int k = 0; k < kHist; ++k) {
+        const int i = from + k * 256 + t;
+        hid[k] = -1;
+        if (i < total) hid[k] = hist(i);
     }
-    __syncthreads();
-    for (int i = from + t; i < total; i += 256) {
-        const int id = hist(i);
-        if ((unsigned)id < (unsigned)n) atomicAdd(&cnt[id], 1u);
-    }
-    for (int i = t; i < a.n_bias; i += 256) {
-        const int id = bid[i] - c0;
-        if ((unsigned)id < (unsigned)n) atomicMin(&bias[id], (uint32_t)i);
-    }
-    __syncthreads();
-    for (int i = t; i < a.n_bias; i += 256) {
-        const int id = bid[i] - c0;
-        if ((unsigned)id < (unsigned)n && bias[id] != (uint32_t)i) twice = 1;
-    }
-    __syncthreads();
-    const bool again = twice != 0;
+    // f(id, entry) of every id of the window (entry -1) and of the bias list.
+    auto each = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < kHist; ++k) f(hid[k], -1);
+        for (int i = from + kHist * 256 + t; i < total; i += 256) f(hist(i), -1);
+#pragma unroll
+        for (int k = 0; k < kBias; ++k) f(bidr[k], k * 256 + t);
+        for (int i = kBias * 256 + t; i < a.n_bias; i += 256) f(bid[i], i);
+    };
 
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int i = (k * 256 + t) * VEC;
-        if (i >= n) break;
-        const uint32_t hit = touched[i >> 5] >> (i & 31) & ((1u << VEC) - 1);
-        const uint32_t allow = a.mask ? a.mask[(int64_t)r * a.mstride + ((c0 + i) >> 5)] >> ((c0 + i) & 31) : ~0u;
-        Out o;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            float f = Widen<TI>::up(v[k].x[e]);
-            if (hit >> e & 1) {
-                const uint32_t c = cnt[i + e];
-                if (c) f = apply_pen<true>(f, c, pn);
-                const uint32_t first = bias[i + e];
-                if (first != ~0u) {
-                    float sum = first < kBiasHeld ? value[first] : bval[first];
-                    if (again)   // (most lists name an id once)
-                        for (int l = (int)first + 1; l < a.n_bias; ++l)
-                            if (bid[l] - c0 == i + e) sum += bval[l];
-                    f += sum;
-                }
+    for (int i = t; i < 2 * kAdjChunk / 32; i += 256) (&touched[0][0])[i] = 0;
+    if (t == 0) twice = listed[0] = listed[1] = 0;
+    int which = 0;
+    for (int c0 = first; c0 < last; c0 += kAdjChunk, which ^= 1) {
+        const int n = min(kAdjChunk, a.vocab - c0);
+        uint32_t* const set = touched[which];
+        lds_sync();
+        each([&](int id, int) {
+            const uint32_t at = (uint32_t)id - (uint32_t)c0;
+            if (at < (uint32_t)n) {
+                cnt[at] = 0;
+                bias[at] = ~0u;
+                const uint32_t bit = 1u << (at & 31);
+                if (!(atomicOr(&set[at >> 5], bit) & bit)) list[atomicAdd(&listed[which], 1u)] = (uint16_t)at;
             }
-            o.x[e] = Widen<TO>::down(allow >> e & 1 ? f : -__builtin_huge_valf());
+        });
+        lds_sync();
+        // A thread has an id to work out; its logit is on the way during the counts.
+        const int ids = (int)listed[which];
+        TI x = (TI)0.f;
+        if (t < ids) x = row_in[c0 + list[t]];
+        each([&](int id, int entry) {
+            const uint32_t at = (uint32_t)id - (uint32_t)c0;
+            if (at >= (uint32_t)n) return;
+            if (entry < 0) atomicAdd(&cnt[at], 1u);
+            else if (atomicMin(&bias[at], (uint32_t)entry) != ~0u) twice = 1;   // (most lists name an id once)
+        });
+        if (t < kAdjChunk / 32) touched[which ^ 1][t] = 0;
+        if (t == 0) listed[which ^ 1] = 0;
+        lds_sync();
+        for (int l = t; l < ids; l += 256) {
+            const int id = list[l];
+            if (l != t) x = row_in[c0 + id];
+            float f = Widen<TI>::up(x);
+            const uint32_t c = cnt[id];
+            if (c) f = apply_pen<true>(f, c, pn);
+            const uint32_t head = bias[id];
+            if (head != ~0u) {
+                float sum = head < kBiasHeld ? value[head] : bval[head];
+                if (twice)
+                    for (int i = (int)head + 1; i < a.n_bias; ++i)
+                        if (bid[i] - c0 == id) sum += bval[i];
+                f += sum;
+            }
+            cnt[id] = __float_as_uint(f);
         }
-        if (i + VEC <= n) __builtin_memcpy(y + i, &o, sizeof(Out));
-        else
-            for (int e = 0; e < VEC; ++e)
-                if (i + e < n) y[i + e] = o.x[e];
+        lds_sync();
+        if (n < kAdjChunk) {   // the row's last, element by element
+            for (int i = t; i < n; i += 256) {
+                float f = set[i >> 5] >> (i & 31) & 1 ? __uint_as_float(cnt[i]) : Widen<TI>::up(row_in[c0 + i]);
+                if (mrow && !(mrow[(c0 + i) >> 5] >> (i & 31) & 1)) f = low;
+                row_out[c0 + i] = Widen<TO>::down(f);
+            }
+            break;
+        }
+        In now[NV];
+        uint32_t allow[NV];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            now[k] = v[k];
+            allow[k] = word[k] >> ((k * 256 + t) * VEC & 31);
+        }
+        if (c0 + 2 * kAdjChunk <= a.vocab && c0 + kAdjChunk < last) load(c0 + kAdjChunk);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int i = (k * 256 + t) * VEC;
+            const uint32_t hit = set[i >> 5] >> (i & 31) & ((1u << VEC) - 1) & allow[k];
+            Out o;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) o[e] = Widen<TO>::down(allow[k] >> e & 1 ? Widen<TI>::up(now[k][e]) : low);
+            if (hit) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    if (hit >> e & 1) o[e] = Widen<TO>::down(__uint_as_float(cnt[i + e]));
+            }
+            *(Out*)(row_out + c0 + i) = o;
+        }
     }
 }
 
@@ -205,7 +263,11 @@ extern "C" int tms_adjust_logits(const tms_adjust_args* args, hipStream_t stream
     a.bias_values = p.bias_values;
     a.mask = p.mask;
     a.mstride = p.mask_stride;
-    const dim3 grid((p.vocab + kAdjChunk - 1) / kAdjChunk, (unsigned)rows);
+    // Chunks a workgroup: as many as leave two rounds of the 1024 workgroups that
+    // the card holds.
+    const int chunks = (p.vocab + kAdjChunk - 1) / kAdjChunk;
+    a.subs = (int)std::max<int64_t>(1, std::min<int64_t>(chunks, rows * chunks / 2048));
+    const dim3 grid((chunks + a.subs - 1) / a.subs, (unsigned)rows);
     const bool wide = p.out_dtype == TMS_DTYPE_F32;
     if (p.dtype == TMS_DTYPE_F32) hipLaunchKernelGGL((adjust_kernel<float, float>), grid, dim3(256), 0, stream, a);
     else if (p.dtype == TMS_DTYPE_F16 && wide) hipLaunchKernelGGL((adjust_kernel<_Float16, float>), grid, dim3(256), 0, stream, a);
