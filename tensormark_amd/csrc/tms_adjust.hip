@@ -20,7 +20,9 @@
 namespace tms {
 
 constexpr uint32_t kBiasHeld = 512;
-constexpr int kAdjChunk = 4096;   // ids a workgroup: 16 KiB each of counts and biases, four workgroups a CU
+// Ids at a time: 8 KiB each of counts and biases, seven workgroups a CU (288 rows
+// of 128256 bf16: 39 us; 45 with 4096 and three workgroups).
+constexpr int kAdjChunk = 2048;
 
 struct AdjustParams {
     const char* x;
@@ -263,10 +265,11 @@ extern "C" int tms_adjust_logits(const tms_adjust_args* args, hipStream_t stream
     a.bias_values = p.bias_values;
     a.mask = p.mask;
     a.mstride = p.mask_stride;
-    // Chunks a workgroup: as many as leave two rounds of the 1024 workgroups that
-    // the card holds.
+    // Chunks a workgroup: as many as leave some two rounds of the 1792 workgroups
+    // that the card holds (288 rows of 128256: 39 us with 4096 workgroups, 44 with
+    // 1024, 50 with one a chunk).
     const int chunks = (p.vocab + kAdjChunk - 1) / kAdjChunk;
-    a.subs = (int)std::max<int64_t>(1, std::min<int64_t>(chunks, rows * chunks / 2048));
+    a.subs = (int)std::max<int64_t>(1, std::min<int64_t>(chunks, rows * chunks / 4096));
     const dim3 grid((chunks + a.subs - 1) / a.subs, (unsigned)rows);
     const bool wide = p.out_dtype == TMS_DTYPE_F32;
     if (p.dtype == TMS_DTYPE_F32) hipLaunchKernelGGL((adjust_kernel<float, float>), grid, dim3(256), 0, stream, a);

@@ -53,24 +53,21 @@ __device__ __forceinline__ int evict_len(const EvictParams& a, int b) {
     return (int)(cap < L ? cap : L);
 }
 
-// A score's place in the order of eviction: larger is kept longer.  NaN, and
-// positions on unmapped pages, come first to go.
-__device__ __forceinline__ uint32_t evict_key(const EvictParams& a, const int32_t* row, int h, int j, int len) {
-    const int page = page_of(a.c, row, j, len);
-    if (page < 0) return 0u;
-    const float s = a.c.scores[(((int64_t)page * a.c.kv_heads + h) << a.c.shift) + (j & a.c.smask)];
-    return s == s ? okey(s) : 0u;
-}
-
 // One workgroup a sequence and head: the key of the last entry kept, by a
-// radix select over the order keys, 8 bits a pass; then each thread counts
-// the entries of its own stretch above it and tied with it, one scan gives
-// the counts before the stretch, and an entry's new position is
+// radix select over the scores' order keys, 8 bits a pass; then the entries
+// above it and the first of those tied with it, in order, at
 // sinks + above + min(tied, those that still fit).
+//
+// Entry j is thread j % 1024's.  Its keys of kBlocks blocks stay in registers,
+// so that a head of up to 16384 entries reads its scores once, all loads in
+// flight together (16 sequences of 1500 to 8192, 8 heads: 29 us with the scores read
+// in each pass); a longer one reads them again for each pass and stretch.
+constexpr int kBlocks = 16, kStretch = kBlocks * 1024;
+
 __global__ __launch_bounds__(1024) void evict_select_kernel(EvictParams a) {
     __shared__ uint32_t hist[16][256];
-    __shared__ uint32_t part[16][2];
-    __shared__ uint32_t pick[2];
+    __shared__ uint32_t part[kBlocks * 16][2];   // above and tied before a block's wave
+    __shared__ uint32_t total[256], pick[2];
     const int b = blockIdx.x / a.c.kv_heads, h = blockIdx.x - b * a.c.kv_heads;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int L = evict_len(a, b);
@@ -86,77 +83,128 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(EvictParams a) {
     for (int i = t; i < a.recent; i += 1024) kept[a.budget - a.recent + i] = hi + i;
     if (want == 0) return;
 
+    // A score's order key: larger is kept longer.  NaN, and positions on
+    // unmapped pages, come first to go.
+    uint32_t key[kBlocks];
+    auto load = [&](int base) __attribute__((always_inline)) {
+        int page[kBlocks];
+        float s[kBlocks];
+#pragma unroll
+        for (int k = 0; k < kBlocks; ++k)
+            if (base + k * 1024 < hi) page[k] = row[min(base + k * 1024 + t, hi - 1) >> a.c.shift];
+#pragma unroll
+        for (int k = 0; k < kBlocks; ++k)
+            if (base + k * 1024 < hi) {
+                const int j = min(base + k * 1024 + t, hi - 1);
+                const bool ok = (unsigned)page[k] < (unsigned)a.c.pages;
+                s[k] = a.c.scores[(((int64_t)(ok ? page[k] : 0) * a.c.kv_heads + h) << a.c.shift) + (j & a.c.smask)];
+                page[k] = ok;
+            }
+#pragma unroll
+        for (int k = 0; k < kBlocks; ++k)
+            if (base + k * 1024 < hi) key[k] = page[k] && s[k] == s[k] ? okey(s[k]) : 0u;
+    };
+    if (hi - lo <= kStretch) load(lo);
+
+    // Each wave counts into bins of its own, and each finds the digit from the
+    // sums by itself: two barriers a pass.  Where a digit's entries are all kept,
+    // the digits below need no look.
     uint32_t prefix = 0, fixed = 0;
     uint32_t left = (uint32_t)want;   // of the entries that share the prefix
+    for (int i = lane; i < 256; i += 64) hist[wave][i] = 0;
     for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = t; i < 16 * 256; i += 1024) ((uint32_t*)hist)[i] = 0;
-        __syncthreads();
-        for (int j = lo + t; j < hi; j += 1024) {
-            const uint32_t k = evict_key(a, row, h, j, L);
-            if ((k & fixed) == prefix) atomicAdd(&hist[wave][k >> shift & 255], 1u);
+        for (int base = lo; base < hi; base += kStretch) {
+            if (hi - lo > kStretch) load(base);
+#pragma unroll
+            for (int k = 0; k < kBlocks; ++k) {
+                if (base + k * 1024 >= hi) break;
+                if (base + k * 1024 + t < hi && (key[k] & fixed) == prefix) atomicAdd(&hist[wave][key[k] >> shift & 255], 1u);
+            }
         }
-        __syncthreads();
+        lds_sync();
         if (t < 256) {
             uint32_t n = 0;
+#pragma unroll
             for (int w = 0; w < 16; ++w) n += hist[w][t];
-            hist[0][t] = n;
+            total[t] = n;
         }
-        __syncthreads();
-        if (t < 64) {   // the highest digit with `left` entries at or above it
-            uint32_t n[4], mine = 0;
-            for (int i = 0; i < 4; ++i) mine += n[i] = hist[0][255 - (4 * t + i)];
-            uint32_t upto = mine;
-            for (int x = 1; x < 64; x <<= 1) {
-                const uint32_t y = __shfl_up(upto, x);
-                if (lane >= x) upto += y;
-            }
-            uint32_t above = upto - mine;
-            for (int i = 0; i < 4; ++i) {
-                if (above < left && above + n[i] >= left) {
-                    pick[0] = 255 - (4 * t + i);
-                    pick[1] = left - above;
-                }
-                above += n[i];
-            }
+        lds_sync();
+        for (int i = lane; i < 256; i += 64) hist[wave][i] = 0;
+        uint32_t n[4], mine = 0;   // the highest digit with `left` entries at or above it
+        for (int i = 0; i < 4; ++i) mine += n[i] = total[255 - (4 * lane + i)];
+        uint32_t upto = mine;
+        for (int x = 1; x < 64; x <<= 1) {
+            const uint32_t y = __shfl_up(upto, x);
+            if (lane >= x) upto += y;
         }
-        __syncthreads();
-        prefix |= pick[0] << shift;
+        uint32_t above = upto - mine, digit = 0, rest = 0, held = 0;
+        bool found = false;
+        for (int i = 0; i < 4; ++i) {
+            if (above < left && above + n[i] >= left) {
+                found = true;
+                digit = 255 - (4 * lane + i);
+                rest = left - above;
+                held = n[i];
+            }
+            above += n[i];
+        }
+        const int from = __ffsll((unsigned long long)__ballot(found)) - 1;
+        prefix |= (uint32_t)__builtin_amdgcn_readlane(digit, from) << shift;
         fixed |= 255u << shift;
-        left = pick[1];
-        __syncthreads();
+        left = __builtin_amdgcn_readlane(rest, from);
+        if ((uint32_t)__builtin_amdgcn_readlane(held, from) == left) break;
     }
 
-    const int per = (hi - lo + 1023) / 1024, from = min(lo + t * per, hi), to = min(from + per, hi);
-    uint32_t above = 0, tied = 0;
-    for (int j = from; j < to; ++j) {
-        const uint32_t k = evict_key(a, row, h, j, L);
-        above += k > prefix;
-        tied += k == prefix;
-    }
-    uint32_t sa = above, st = tied;
-    for (int x = 1; x < 64; x <<= 1) {
-        const uint32_t ya = __shfl_up(sa, x), yt = __shfl_up(st, x);
-        if (lane >= x) {
-            sa += ya;
-            st += yt;
+    uint32_t above0 = 0, tied0 = 0;   // before the stretch
+    const uint64_t before = (1ull << lane) - 1;
+    for (int base = lo; base < hi; base += kStretch) {
+        if (hi - lo > kStretch) load(base);
+#pragma unroll
+        for (int k = 0; k < kBlocks; ++k) {
+            uint64_t up = 0, eq = 0;
+            if (base + k * 1024 < hi) {
+                const bool in = base + k * 1024 + t < hi;
+                up = __ballot(in && (key[k] & fixed) > prefix);
+                eq = __ballot(in && (key[k] & fixed) == prefix);
+            }
+            if (lane == 0) {
+                part[k * 16 + wave][0] = __popcll(up);
+                part[k * 16 + wave][1] = __popcll(eq);
+            }
         }
-    }
-    if (lane == 63) {
-        part[wave][0] = sa;
-        part[wave][1] = st;
-    }
-    __syncthreads();
-    sa -= above;
-    st -= tied;
-    for (int w = 0; w < wave; ++w) {
-        sa += part[w][0];
-        st += part[w][1];
-    }
-    for (int j = from; j < to; ++j) {
-        const uint32_t k = evict_key(a, row, h, j, L);
-        if (k > prefix || (k == prefix && st < left)) kept[lo + sa + min(st, left)] = j;
-        sa += k > prefix;
-        st += k == prefix;
+        lds_sync();
+        if (t < 64) {
+            uint32_t n[4][2], sum[2] = {0, 0};
+            for (int i = 0; i < 4; ++i)
+                for (int c = 0; c < 2; ++c) sum[c] += n[i][c] = part[4 * t + i][c];
+            for (int c = 0; c < 2; ++c) {
+                uint32_t upto = sum[c];
+                for (int x = 1; x < 64; x <<= 1) {
+                    const uint32_t y = __shfl_up(upto, x);
+                    if (lane >= x) upto += y;
+                }
+                if (t == 63) pick[c] = upto;
+                upto -= sum[c];
+                for (int i = 0; i < 4; ++i) {
+                    part[4 * t + i][c] = upto;
+                    upto += n[i][c];
+                }
+            }
+        }
+        lds_sync();
+#pragma unroll
+        for (int k = 0; k < kBlocks; ++k) {
+            if (base + k * 1024 >= hi) break;
+            const int j = base + k * 1024 + t;
+            const bool in = j < hi, over = (key[k] & fixed) > prefix, tie = (key[k] & fixed) == prefix;
+            const uint64_t up = __ballot(in && over), eq = __ballot(in && tie);
+            const uint32_t sa = above0 + part[k * 16 + wave][0] + __popcll(up & before);
+            const uint32_t st = tied0 + part[k * 16 + wave][1] + __popcll(eq & before);
+            if (in && (over || (tie && st < left))) kept[lo + sa + min(st, left)] = j;
+        }
+        above0 += pick[0];
+        tied0 += pick[1];
+        lds_sync();
     }
 }
 
