@@ -41,6 +41,8 @@ extern "C" {
 #define TMS_CACHE_MAX_PAGE 65536
 #define TMS_ATTENTION_MAX_SLOT_STRIDE 67108864   /* elements; tms_paged_attention */
 #define TMS_ATTENTION_MAX_ROWS 2097152           /* max_q times query heads a key head */
+#define TMS_SCORES_MAX_Q_STRIDE 8388608          /* elements between tokens, and that a key head's
+                                                    query heads span; tms_kv_add_scores */
 
 /* The pools, page tables and lengths of one call. */
 typedef struct tms_cache {

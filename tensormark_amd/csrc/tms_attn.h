@@ -114,6 +114,20 @@ __device__ __forceinline__ u32x4 slots_rsrc(const char* p, int last, uint32_t st
     return (u32x4){(uint32_t)at, (uint32_t)(at >> 32) & 0xFFFF, last < 0 ? 0u : (uint32_t)(last * stride + bytes), 0x00020000u};
 }
 
+// Row r as token and head of its group, r below 2^21: a product with 1 / G is off
+// by one at most.
+__device__ __forceinline__ void split_row(int r, int G, float inv, int& tok, int& hd) {
+    tok = (int)((float)r * inv);
+    hd = r - tok * G;
+    if (hd < 0) {
+        --tok;
+        hd += G;
+    } else if (hd >= G) {
+        ++tok;
+        hd -= G;
+    }
+}
+
 // A row's 8 values from dimension d on as the operand of the scores, zeros
 // past head_dim and for a row that is none (`src` is some row in any case:
 // loads without a branch between them are in flight together).
