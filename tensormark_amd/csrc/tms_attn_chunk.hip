@@ -16,7 +16,10 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
     constexpr int KT = 32 * NK, RM = kChunkRows;
     constexpr int C = ROWB / 16, RPI = 64 / C, NI = KT / (4 * RPI);   // pieces a row; rows a load; loads a wave
     constexpr uint32_t ALL = (1u << KT / 8) - 1;
-    __shared__ __attribute__((aligned(128))) char sm[2][2][KT * ROWB];
+    constexpr bool FUSED = ROWB > 256;
+    constexpr int NV = FUSED ? 3 : 2;   // value buffers
+    __shared__ __attribute__((aligned(128))) char sm_k[2][KT * ROWB];
+    __shared__ __attribute__((aligned(128))) char sm_v[NV][KT * ROWB];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n32 = lane & 31, hh = lane >> 5;
     const int pair = blockIdx.x, tile = a.row_tiles - 1 - blockIdx.y, split = blockIdx.z;
@@ -49,7 +52,7 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
     const int32_t* row = a.c.tables + (int64_t)b * a.c.tstride;
     const char* kbase = a.c.k + (int64_t)h * a.c.kh;
     const char* vbase = a.c.v + (int64_t)h * a.c.vh;
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)&sm[0][0][0];
+    const uint32_t lds_k = (uint32_t)(uintptr_t)(lds_void*)&sm_k[0][0], lds_v = (uint32_t)(uintptr_t)(lds_void*)&sm_v[0][0];
     const uint32_t kslot = (uint32_t)a.c.ks, vslot = (uint32_t)a.c.vs, kpage = (uint32_t)a.c.kp, vpage = (uint32_t)a.c.vp;
     uint32_t koff[NI], voff[NI];
 #pragma unroll
@@ -64,7 +67,7 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
         const int j = tl.key(v) + 8 * (lane & 7);
         return (unsigned)j < (unsigned)sq.len ? row[j >> a.c.shift] : -1;
     };
-    auto load = [&](int v, int buf, int pg) {
+    auto load = [&](int v, int kbuf, int vbuf, int pg) __attribute__((always_inline)) {
         const int t0 = tl.key(v);
 #pragma unroll
         for (int g = 0; g < NI * RPI / 8; ++g) {
@@ -77,9 +80,9 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
             const u32x4 vres = slots_rsrc(vbase + (uint64_t)page * vpage + slot * vslot, last, vslot, 2 * D);
 #pragma unroll
             for (int i = g * 8 / RPI; i < (g + 1) * 8 / RPI; ++i) {
-                const uint32_t to = lds0 + buf * 2 * KT * ROWB + (wave * NI + i) * RPI * ROWB;
-                load_lds16(kres, koff[i], to);
-                load_lds16(vres, voff[i], to + KT * ROWB);
+                const uint32_t to = (wave * NI + i) * RPI * ROWB;
+                load_lds16(kres, koff[i], lds_k + kbuf * KT * ROWB + to);
+                load_lds16(vres, voff[i], lds_v + vbuf * KT * ROWB + to);
             }
         }
     };
@@ -91,13 +94,95 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
         for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
     float m = -__builtin_huge_valf(), l = 0.f;
 
-    // One tile.  EDGE: some row of the workgroup does not see all of it.
-    auto step = [&](auto edge, int t0, int buf, uint32_t there) __attribute__((always_inline)) {
-        constexpr bool EDGE = decltype(edge)::value;
-        const char* sk = sm[buf][0];
-        char* sv = sm[buf][1];
+    // The parts of a tile's work, by 32 keys.
+    auto scores = [&](const char* sk, int kt, f32x16& s) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) s = T::mfma32(key_operand<ROWB>(sk, lane, kt, ks), qf[ks], s);
+    };
+    // The reference point follows the maximum once some row's has grown by
+    // 2^kSlack: weights stay below that, which neither type minds.
+    auto refer = [&](float top) __attribute__((always_inline)) {
+        top *= a.scale;
+        if (__any(top > m + kSlack)) {
+            top = fmaxf(top, __shfl_xor(top, 32));
+            top = fmaxf(top, m);
+            const float f = __builtin_amdgcn_exp2f(m - (top == -__builtin_huge_valf() ? 0.f : top));
+            m = top;
+            l *= f;
+#pragma unroll
+            for (int t = 0; t < DT; ++t) o[t] *= f;
+        }
+    };
+    auto most = [&](const f32x16& s, float top) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, s[e]);
+        return top;
+    };
+    auto weigh = [&](f32x16& s, u32x4 (&pf)[2]) __attribute__((always_inline)) {
+        const float base = m == -__builtin_huge_valf() ? 0.f : m;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float x = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale, -base));
+            s[e] = x;
+            l += x;
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) pf[t][w] = T::pack(s[8 * t + 2 * w], s[8 * t + 2 * w + 1]);
+    };
+    auto outputs = [&](const char* sv, int kt, const u32x4 (&pf)[2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) o[dt] = T::mfma32(value_operand<ROWB>(sv, lane, dt, 2 * kt + t), pf[t], o[dt]);
+    };
+    const float low = -__builtin_huge_valf();
+    // Scores of 32 keys, while the weights of the 32 before (`s`) are worked out
+    // and go to the outputs; returns the maximum.  The order is written out: a
+    // matrix instruction, some weights, the operands of two steps on.
+    auto fused = [&](const char* sk, int kt, f32x16& next, f32x16& s, const char* sv, int vt) __attribute__((always_inline)) {
+        const float base = m == low ? 0.f : m;
+        u32x4 kf[3], vf[3], pf[2];
+        float sum = 0.f, top = low;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) next[i] = 0.f;
+        kf[0] = key_operand<ROWB>(sk, lane, kt, 0);
+        kf[1] = key_operand<ROWB>(sk, lane, kt, 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            if (ks + 2 < KS) kf[(ks + 2) % 3] = key_operand<ROWB>(sk, lane, kt, ks + 2);
+            else vf[ks + 2 - KS] = value_operand<ROWB>(sv, lane, (ks + 2 - KS) / 2, 2 * vt + (ks + 2 - KS) % 2);
+            next = T::mfma32(kf[ks % 3], qf[ks], next);
+#pragma unroll
+            for (int e = 16 * ks / KS; e < 16 * (ks + 1) / KS; ++e) {
+                s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale, -base));
+                sum += s[e];
+                if (e & 1) pf[e / 8][e % 8 / 2] = T::pack(s[e - 1], s[e]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * DT; ++i) {
+            if (i + 2 < 2 * DT) vf[(i + 2) % 3] = value_operand<ROWB>(sv, lane, (i + 2) / 2, 2 * vt + i % 2);
+            o[i / 2] = T::mfma32(vf[i % 3], pf[i % 2], o[i / 2]);
+            if (i >= 2 * DT - 2) {
+#pragma unroll
+                for (int e = 8 * (i - 2 * DT + 2); e < 8 * (i - 2 * DT + 3); ++e) top = fmaxf(top, next[e]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        l += sum;
+        return top;
+    };
+
+    // A tile of which some row of the workgroup does not see all.
+    auto edge_step = [&](int t0, const char* sk, char* sv, uint32_t there) __attribute__((always_inline)) {
         bool odd = false;
-        if constexpr (EDGE) {
+        {
             // Some row has a weight of zero: does the tile hold an infinity or NaN?
 #pragma unroll
             for (int i = 0; i < KT * ROWB / 1024; ++i) {
@@ -110,55 +195,23 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
             if (none && !odd) return;
         }
         f32x16 s[NK];
+        u32x4 pf[NK][2];
+        float top = low;
 #pragma unroll
         for (int kt = 0; kt < NK; ++kt) {
+            scores(sk, kt, s[kt]);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[kt][i] = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const u32x4 kf = key_operand<ROWB>(sk, lane, kt, ks);
-                s[kt] = T::mfma32(kf, qf[ks], s[kt]);
+            for (int i = 0; i < 16; ++i) {
+                const int j = t0 + 32 * kt + 8 * (i / 4) + 4 * hh + (i & 3);
+                const bool on = (there >> (4 * kt + i / 4) & 1) && j < sq.len && sees(j, pos, a.window, a.sinks);
+                s[kt][i] = on ? s[kt][i] : low;
             }
+            top = most(s[kt], top);
         }
-        if constexpr (EDGE) {
+        refer(top);
 #pragma unroll
-            for (int kt = 0; kt < NK; ++kt)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int j = t0 + 32 * kt + 8 * (i / 4) + 4 * hh + (i & 3);
-                    const bool on = (there >> (4 * kt + i / 4) & 1) && j < sq.len && sees(j, pos, a.window, a.sinks);
-                    s[kt][i] = on ? s[kt][i] : -__builtin_huge_valf();
-                }
-        }
-        float top = -__builtin_huge_valf();
-#pragma unroll
-        for (int e = 0; e < 16 * NK; ++e) top = fmaxf(top, s[e / 16][e % 16]);
-        top *= a.scale;
-        // The reference point follows the maximum once some row's has grown by
-        // 2^kSlack: weights stay below that, which neither type minds.
-        if (__any(top > m + kSlack)) {
-            top = fmaxf(top, __shfl_xor(top, 32));
-            top = fmaxf(top, m);
-            const float f = __builtin_amdgcn_exp2f(m - (top == -__builtin_huge_valf() ? 0.f : top));
-            m = top;
-            l *= f;
-#pragma unroll
-            for (int t = 0; t < DT; ++t) o[t] *= f;
-        }
-        const float base = m == -__builtin_huge_valf() ? 0.f : m;
-        u32x4 pf[2 * NK];
-#pragma unroll
-        for (int e = 0; e < 16 * NK; ++e) {
-            const float x = __builtin_amdgcn_exp2f(fmaf(s[e / 16][e % 16], a.scale, -base));
-            s[e / 16][e % 16] = x;
-            l += x;
-        }
-#pragma unroll
-        for (int t = 0; t < 2 * NK; ++t)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) pf[t][w] = T::pack(s[t / 2][8 * (t & 1) + 2 * w], s[t / 2][8 * (t & 1) + 2 * w + 1]);
-
-        if constexpr (EDGE) {
+        for (int kt = 0; kt < NK; ++kt) weigh(s[kt], pf[kt]);
+        {
             // A weight of zero times an infinity or NaN would reach rows that
             // do not see the value: such values go, key by key, to the rows whose
             // weight is not zero (which weight does not matter), and are zero in
@@ -199,17 +252,16 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
         }
 
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int t = 0; t < 2 * NK; ++t) o[dt] = T::mfma32(value_operand<ROWB>(sv, lane, dt, t), pf[t], o[dt]);
+        for (int kt = 0; kt < NK; ++kt) outputs(sv, kt, pf[kt]);
     };
 
     int pg = v0 < v1 ? entries(v0) : -1, ahead = v0 + 1 < v1 ? entries(v0 + 1) : -1;
     uint32_t there = (uint32_t)__ballot((unsigned)pg < (unsigned)a.c.pages) & ALL;
-    if (v0 < v1) load(v0, 0, pg);
-    int v = v0;
+    if (v0 < v1) load(v0, 0, 0, pg);
+    int v = v0, kb = 0, vb = 0;   // the tile, its key and value buffers
     // Takes tile v when it has come: the wave's loads are in, and after the
-    // barrier all are and the other buffer is free for the next tile's.
+    // barrier all are, and the buffers that the next tile's go to are free: no wave
+    // has left to do but the last values of the tile before.
     uint32_t now = 0;
     auto arrive = [&]() __attribute__((always_inline)) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -217,22 +269,64 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
         now = there;
         there = (uint32_t)__ballot((unsigned)pg < (unsigned)a.c.pages) & ALL;
         __syncthreads();
-        if (v + 1 < v1) load(v + 1, v + 1 - v0 & 1, pg);
+        if (v + 1 < v1) load(v + 1, kb ^ 1, vb == NV - 1 ? 0 : vb + 1, pg);
         if (v + 2 < v1) ahead = entries(v + 2);
+    };
+    auto advance = [&]() __attribute__((always_inline)) {
+        ++v;
+        kb ^= 1;
+        vb = vb == NV - 1 ? 0 : vb + 1;
     };
     auto is_edge = [&](int t0, uint32_t bits) {
         return bits != ALL || t0 + KT > sq.len || t0 + KT - 1 > gfirst || (a.window > 0 && t0 <= glast - a.window && t0 + KT > a.sinks);
     };
     while (v < v1) {
-        while (v < v1 && !is_edge(tl.key(v), there)) {
-            arrive();
-            step(std::false_type(), tl.key(v), v - v0 & 1, now);
-            ++v;
+        // Tiles that every row sees all of.
+        if constexpr (FUSED) {
+            if (!is_edge(tl.key(v), there)) {
+                f32x16 sa, sb;
+                u32x4 pf[2];
+                arrive();
+                scores(sm_k[kb], 0, sa);
+                refer(most(sa, low));
+                for (;;) {
+                    if constexpr (NK == 2) refer(fused(sm_k[kb], 1, sb, sa, sm_v[vb], 0));
+                    else sb = sa;
+                    if (v + 1 >= v1 || is_edge(tl.key(v + 1), there)) break;
+                    const char* before = sm_v[vb];
+                    advance();
+                    arrive();
+                    refer(fused(sm_k[kb], 0, sa, sb, before, NK - 1));
+                }
+                weigh(sb, pf);
+                outputs(sm_v[vb], NK - 1, pf);
+                advance();
+            }
+        } else {
+            while (v < v1 && !is_edge(tl.key(v), there)) {
+                f32x16 s[NK];
+                u32x4 pf[NK][2];
+                float top = low;
+                arrive();
+#pragma unroll
+                for (int kt = 0; kt < NK; ++kt) scores(sm_k[kb], kt, s[kt]);
+#pragma unroll
+                for (int kt = 0; kt < NK; ++kt) top = most(s[kt], top);
+                refer(top);
+#pragma unroll
+                for (int kt = 0; kt < NK; ++kt) weigh(s[kt], pf[kt]);
+                const char* sv = sm_v[vb];
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int t = 0; t < 2 * NK; ++t) o[dt] = T::mfma32(value_operand<ROWB>(sv, lane, dt, t), pf[t / 2][t % 2], o[dt]);
+                advance();
+            }
         }
         while (v < v1 && is_edge(tl.key(v), there)) {
             arrive();
-            step(std::true_type(), tl.key(v), v - v0 & 1, now);
-            ++v;
+            edge_step(tl.key(v), sm_k[kb], sm_v[vb], now);
+            advance();
         }
     }
     l += __shfl_xor(l, 32);
