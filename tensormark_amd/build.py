@@ -69,8 +69,11 @@ def _run(cmd: list, verbose: bool) -> str:
 # one read of the row into scratch traffic; the general kernel launched its
 # workgroups measurably slower with any scratch (B = 1024, V = 256000 bf16:
 # 243.5 against 232.3 us with 32 bytes a lane); the whole-vocabulary kernel
-# decides tokens like the wide one, and is kept to the same.
-NO_SCRATCH = ("tms_wide.hip", "tms_spec.hip", "tms_sample.hip", "tms_sparse.hip", "tms_rows.hip", "tms_topp.hip")
+# decides tokens like the wide one, and is kept to the same; the cache's kernels
+# hold outputs or keys in registers (attention of 128-dimensional heads took
+# 775 us with 88 bytes a lane, 526 with none).
+NO_SCRATCH = ("tms_wide.hip", "tms_spec.hip", "tms_sample.hip", "tms_sparse.hip", "tms_rows.hip", "tms_topp.hip",
+              "tms_attn.hip", "tms_attn_chunk.hip", "tms_scores.hip", "tms_kv.hip", "tms_adjust.hip")
 
 
 def _check_no_scratch(src: str, remarks: str) -> None:

@@ -1,10 +1,17 @@
 // tms_attn_chunk.hip -- attention over the paged cache for many rows a key
 // head: chunks of a prompt, long drafts (tms_paged_attention).
 //
+// Bound by the matrix and the vector pipe about alike (a tile of 64 keys: 1024
+// cycles of products, some 1030 of weights a wave), with LDS reads near.
+//
 // The same mathematics as tms_attn.hip's: S^T = K Q^T, weights 2^(s - m), O^T
 // = V^T P^T, m and the sum of weights running per row.  128 rows of one key
 // head a workgroup, 32 a wave, on 32x32x16 instructions; a tile of 64 keys and
-// values goes to LDS once for the four waves.
+// values goes to LDS once for the four waves, the next one on the way; two
+// workgroups a CU.  Head dimensions past 128 (FUSED) have one workgroup's registers
+// and a tile of 32 keys: there the scores of the next keys run among the weights of
+// the last within a wave (2048 new tokens over 8192, 256 dimensions: 790 us
+// without, 545 with; at 128 dimensions that spills: 526 and 775).
 #include <type_traits>
 
 #include "tms_attn.h"
@@ -303,23 +310,58 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
                 advance();
             }
         } else {
+            // The products' operands are read three steps ahead, the second 32 keys'
+            // weights are worked out among the first's outputs, and a wave in its
+            // products goes before one in its weights: the two workgroups of a CU
+            // fall into turns (2048 new tokens over 16384, 32 heads of 8 of 128: 499 us with
+            // the operands ahead alone, 493 with the weights between, 473 with all).
             while (v < v1 && !is_edge(tl.key(v), there)) {
                 f32x16 s[NK];
-                u32x4 pf[NK][2];
-                float top = low;
+                u32x4 pf[NK][2], kf[4], vf[4];
+                float top = low, sum = 0.f, w[16];
                 arrive();
+                const char* sk = sm_k[kb];
+                const char* sv = sm_v[vb];
 #pragma unroll
-                for (int kt = 0; kt < NK; ++kt) scores(sm_k[kb], kt, s[kt]);
+                for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[kt][i] = 0.f;
+                __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+                for (int i = 0; i < 3; ++i) kf[i] = key_operand<ROWB>(sk, lane, i % NK, i / NK);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < NK * KS; ++i) {
+                    if (i + 3 < NK * KS) kf[(i + 3) % 4] = key_operand<ROWB>(sk, lane, (i + 3) % NK, (i + 3) / NK);
+                    s[i % NK] = T::mfma32(kf[i % 4], qf[i / NK], s[i % NK]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                __builtin_amdgcn_s_setprio(0);
 #pragma unroll
                 for (int kt = 0; kt < NK; ++kt) top = most(s[kt], top);
                 refer(top);
+                weigh(s[0], pf[0]);
+                const float base = m == low ? 0.f : m;
+                __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-                for (int kt = 0; kt < NK; ++kt) weigh(s[kt], pf[kt]);
-                const char* sv = sm_v[vb];
+                for (int i = 0; i < 3; ++i) vf[i] = value_operand<ROWB>(sv, lane, i % DT, i / DT);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
+                for (int i = 0; i < 2 * NK * DT; ++i) {
+                    if (i + 3 < 2 * NK * DT) vf[(i + 3) % 4] = value_operand<ROWB>(sv, lane, (i + 3) % DT, (i + 3) / DT);
+                    o[i % DT] = T::mfma32(vf[i % 4], pf[i / DT / 2][i / DT % 2], o[i % DT]);
+                    if (NK == 2 && i < 2 * DT) {
 #pragma unroll
-                    for (int t = 0; t < 2 * NK; ++t) o[dt] = T::mfma32(value_operand<ROWB>(sv, lane, dt, t), pf[t / 2][t % 2], o[dt]);
+                        for (int e = 16 * i / (2 * DT); e < 16 * (i + 1) / (2 * DT); ++e) {
+                            w[e] = __builtin_amdgcn_exp2f(fmaf(s[NK - 1][e], a.scale, -base));
+                            sum += w[e];
+                            if (e & 1) pf[NK - 1][e / 8][e % 8 / 2] = T::pack(w[e - 1], w[e]);
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                __builtin_amdgcn_s_setprio(0);
+                l += sum;
                 advance();
             }
         }
