@@ -1,0 +1,68 @@
+"""Limits of the cache operators that their header names, refused before any device work."""
+from __future__ import annotations
+
+import ctypes as C
+
+import pytest
+
+from tensormark_amd import cache
+from test_cache_args import CAPACITY, INVALID, P, a_cache, rows_args
+
+
+def attend(c=None, a=None):
+    lib = cache._fns()
+    c, a = a_cache(**(c or {})), rows_args(cache.AttentionArgs, **(a or {}))
+    need = lib.tms_paged_attention_workspace(C.byref(c), C.byref(a))
+    got = lib.tms_paged_attention(C.byref(c), C.byref(a), None)
+    assert need == got
+    return got
+
+
+def scores(c=None, a=None):
+    c, a = a_cache(**(c or {})), rows_args(cache.ScoreArgs, **(a or {}))
+    return cache._fns().tms_kv_add_scores(C.byref(c), C.byref(a), None)
+
+
+@pytest.mark.parametrize("scale", [float("inf"), float("-inf"), float("nan")])
+def test_a_scale_that_is_no_number(scale):
+    assert attend(a=dict(scale=scale)) == INVALID
+    assert scores(a=dict(scale=scale)) == INVALID
+
+
+def test_slots_too_far_apart():
+    for s in ("k_stride", "v_stride"):
+        assert attend(c={s: (2, 1 << 26)}) == CAPACITY
+
+
+def test_too_many_rows():
+    assert attend(c=dict(tokens=1 << 21, max_q=1 << 21)) == CAPACITY
+    assert scores(c=dict(tokens=1 << 21, max_q=1 << 21)) == CAPACITY
+
+
+def test_too_many_sequences_and_heads():
+    assert attend(c=dict(batch=1 << 20)) == CAPACITY
+
+
+def test_queries_too_far_apart_for_scores():
+    assert scores(a=dict(q_stride=(0, (1 << 23) + 8))) == CAPACITY
+    assert scores(a=dict(q_stride=(1, 1 << 23))) == CAPACITY
+
+
+def test_histories_of_logits():
+    lib = cache._fns()
+    for kw, code in ((dict(n_history=9, recent_stride=8), INVALID), (dict(n_history=-1), INVALID), (dict(reserved=1), INVALID),
+                     (dict(n_history=1 << 29, recent_stride=1 << 29), CAPACITY)):
+        a = rows_args(cache.AdjustArgs, out=P + 4096, **kw)
+        assert lib.tms_adjust_logits(C.byref(a), None) == code
+
+
+def test_a_workspace_for_every_form():
+    """None for whole items, some for shares and for splits; never less for more."""
+    lib = cache._fns()
+    need = []
+    for kv in (100, 1024, 5000, 50000, 500000):
+        c, a = a_cache(max_kv=kv, table_stride=40000), rows_args(cache.AttentionArgs)
+        need.append(lib.tms_paged_attention_workspace(C.byref(c), C.byref(a)))
+    assert need[0] == need[1] == 0 and need[2] > 0 and need == sorted(need)
+    c = a_cache(max_kv=50000, table_stride=40000, tokens=90, max_q=30)
+    assert lib.tms_paged_attention_workspace(C.byref(c), C.byref(rows_args(cache.AttentionArgs))) > 0
