@@ -235,3 +235,22 @@ def test_histories_shared_or_cut_from_wider_rows():
     assert torch.equal(a, tm.adjust_logits(x, p, recent=wide[:, :10].contiguous()))
     with pytest.raises(ValueError):
         tm.adjust_logits(x, p, recent=wide[:1].expand(3, 40))
+
+
+def test_strides_of_single_ones_do_not_matter():
+    """One token, one head, one page: whatever stride their dimension has."""
+    bt = Batch([9], [1], H=1, G=1, D=64, page=16, extra=0, seed=3)
+    want, wl = bt.attend()
+    k = bt.k.as_strided(bt.k.shape, (7, 3, 64, 1))
+    v = bt.v.as_strided(bt.v.shape, (5, 1, 64, 1))
+    q = bt.qs.to(DEV)
+    q = q.as_strided(q.shape, (11, 13, 1))
+    o, l = tm.paged_attention(q, k, v, bt.tables, bt.kv_len, bt.q_start, max_q=1, max_kv=9)
+    assert torch.equal(o, want) and torch.equal(l, wl)
+
+
+def test_windows_past_32_bits():
+    bt = Batch([60], [3], seed=3)
+    want = bt.attend()
+    got = bt.attend(window=2 ** 32 + 1, sinks=2 ** 33)
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
