@@ -33,9 +33,11 @@ __device__ __forceinline__ float sum_rows(float* x, int n32) {
 
 // Four waves of 32 keys of one key head.  The rows that see any of the 128 come
 // by 64 through LDS, loaded there (as the chunk kernel loads its keys) while the 64
-// before are used.  Few rows: bound by the keys' one read.  Many: by the
-// exponential, 16 cycles of a SIMD for 64 weights beside 8 for the scaling and
-// the sum and 10 (D = 80) to 32 (D = 256) of the matrix pipe.
+// before are used, and the weights of 32 rows are summed among the products of the
+// next 32.  Bound by the vector pipe: 16 cycles of a SIMD for the exponentials of 64
+// weights and 8 for scaling and sum, beside 10 (D = 80) to 32 (D = 256) of the matrix
+// pipe (1024 and 777 tokens over 6000 and 4097, 8 heads of 2 of 80 dimensions, fp16: 51 us, of
+// which exponentials alone take 15; 153 us with rows read by each wave from memory).
 template <typename T, int ROWB, int KS>
 __global__ __launch_bounds__(256, KS > 8 ? 2 : 3) void score_kernel(AttnParams a) {
     constexpr int RQ = 64, C = ROWB / 16, RPI = 64 / C, NI = RQ / (4 * RPI);
@@ -131,6 +133,32 @@ __global__ __launch_bounds__(256, KS > 8 ? 2 : 3) void score_kernel(AttnParams a
 #pragma unroll
     for (int i = 0; i < 16; ++i) sum[i] = 0.f;
 
+    // The scores of 32 rows, while the weights of the 32 before (`s`) are summed:
+    // a matrix instruction, some weights, the operand of two steps on.
+    auto stage = [&](const char* sq_rows, int half, f32x16& next, const f32x16& s, float lse) __attribute__((always_inline)) {
+        u32x4 qf[3];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) next[i] = 0.f;
+        qf[0] = key_operand<ROWB>(sq_rows, lane, half, 0);
+        qf[1] = key_operand<ROWB>(sq_rows, lane, half, 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            if (ks + 2 < KS) qf[(ks + 2) % 3] = key_operand<ROWB>(sq_rows, lane, half, ks + 2);
+            next = T::mfma32(kr[ks], qf[ks % 3], next);
+#pragma unroll
+            for (int e = 16 * ks / KS; e < 16 * (ks + 1) / KS; ++e) {
+                sum[e] += __builtin_amdgcn_exp2f(fmaf(s[e], a.scale, -lse));
+                asm volatile("" : "+v"(sum[e]));   // (here, not past the branch that follows)
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    f32x16 s0, s1;
+    float lse0 = 0.f, lse1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s1[i] = -__builtin_huge_valf();   // nothing before the first
+
     int buf = 0;
     for (int r = rbegin; r < rend; r += step, buf ^= 1) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -153,29 +181,26 @@ __global__ __launch_bounds__(256, KS > 8 ? 2 : 3) void score_kernel(AttnParams a
         }
         if (t0 > pl || t0 >= sq.len || (a.window > 0 && t0 + 31 <= pf - a.window && t0 >= a.sinks)) continue;
         const bool edge = t0 + 31 > pf || (a.window > 0 && t0 <= pl - a.window && t0 + 32 > a.sinks);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            f32x16 s;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) s = T::mfma32(kr[ks], key_operand<ROWB>(sm[buf], lane, half, ks), s);
-            const float lse = sm_lse[buf][32 * half + n32];
-            if (edge) {
-                int pos = pf + prow[half];
-                if (!whole) {
-                    split_row(r + 32 * half + n32, G, inv, pos, hd);
-                    pos += sq.p0;
-                }
-                if (32 * half + n32 >= min(step, rend - r)) pos = -1;
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (!sees(t0 + 8 * (i / 4) + 4 * hh + (i & 3), pos, a.window, a.sinks)) s[i] = -__builtin_huge_valf();
+        auto mask = [&](f32x16& x, int half) __attribute__((always_inline)) {
+            int pos = pf + prow[half];
+            if (!whole) {
+                split_row(r + 32 * half + n32, G, inv, pos, hd);
+                pos += sq.p0;
             }
+            if (32 * half + n32 >= min(step, rend - r)) pos = -1;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sum[i] += __builtin_amdgcn_exp2f(fmaf(s[i], a.scale, -lse));
-        }
+            for (int i = 0; i < 16; ++i)
+                if (!sees(t0 + 8 * (i / 4) + 4 * hh + (i & 3), pos, a.window, a.sinks)) x[i] = -__builtin_huge_valf();
+        };
+        stage(sm[buf], 0, s0, s1, lse1);
+        if (edge) mask(s0, 0);
+        lse0 = sm_lse[buf][n32];
+        stage(sm[buf], 1, s1, s0, lse0);
+        if (edge) mask(s1, 1);
+        lse1 = sm_lse[buf][32 + n32];
     }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum[i] += __builtin_amdgcn_exp2f(fmaf(s1[i], a.scale, -lse1));
     const float add = sum_rows(sum, n32);
     const int i = row_key(n32), key = 8 * (i / 4) + 4 * hh + (i & 3), its = __shfl(page, key);
     if (n32 < 16 && its >= 0) {
