@@ -1,4 +1,5 @@
-"""Builds libtmsample_hip.so in-tree for gfx950 with hipcc.
+"""Builds libtmsample_hip.so in-tree for gfx950 with hipcc, and the cache calls'
+Python module, _cache_ops.so, beside it.
 
 Usage: python -m tensormark_amd.build   (or tensormark_amd.build.build())
 """
@@ -46,6 +47,26 @@ FILE_FLAGS = {
 
 BUILD_DIR = os.path.join(HERE, "_build")
 
+# The cache calls' Python side over torch tensors: a module of its own, since it
+# needs torch's headers and libraries, which libtmsample_hip.so does not.
+OPS_SOURCE = "tms_cache_py.cpp"
+OPS = os.path.join(HERE, "_cache_ops.so")
+
+
+def _ops_command(out: str) -> list:
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    system = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+              os.path.join(rocm, "include"), sysconfig.get_paths()["include"]]
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", os.path.join(ROOT, "include"),
+            *[x for d in system for x in ("-isystem", d)], os.path.join(CSRC, OPS_SOURCE), "-o", out, "-L", HERE, "-ltmsample_hip",
+            "-L", os.path.join(root, "lib"), "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+
 
 def hipcc() -> str:
     rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
@@ -58,7 +79,7 @@ def _run(cmd: list, verbose: bool) -> str:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         sys.stderr.write(r.stdout + r.stderr)
-        raise RuntimeError("hipcc failed building libtmsample_hip.so: " + " ".join(cmd))
+        raise RuntimeError("the compiler failed building the library: " + " ".join(cmd))
     return r.stderr
 
 
@@ -119,6 +140,8 @@ def build(verbose: bool = False) -> str:
             _check_lds(src, rem)
     _run([hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB + ".tmp", *[j[1] for j in jobs]], verbose)
     os.replace(LIB + ".tmp", LIB)
+    _run(_ops_command(OPS + ".tmp"), verbose)
+    os.replace(OPS + ".tmp", OPS)
     return LIB
 
 
