@@ -138,14 +138,16 @@ typedef struct tms_score_args {
 int tms_kv_add_scores(const tms_cache* cache, const tms_score_args* args, hipStream_t stream);
 
 /*
- * Cut each sequence to at most `budget` positions, per head: positions below
- * `sinks` and the last `recent` are kept, then those of the largest scores
- * (ties: the lowest position; a NaN score, or an unmapped page, ranks below
+ * Cut each sequence to at most `budget` positions, per head.  Positions on
+ * unmapped pages go first of all and are never kept.  Of the others, those
+ * below `sinks` and among the last `recent` of the kv_len[b] positions are kept,
+ * then those of the largest scores (ties: the lowest position; a NaN score ranks below
  * every number).  Kept entries keep their order and go, with their scores,
  * to positions 0, 1, ... of dst_tables (pages of the same pools that are none
- * of the sequence's own, or of another's of this call).  new_len[b] =
- * min(kv_len[b], budget); kept[b][h][i] is the old position of new position
- * i, -1 past new_len.  Entries to or from an unmapped page are not copied.
+ * of the sequence's own, or of another's of this call).  new_len[b] is the
+ * number kept, min(budget, positions on mapped pages); kept[b][h][i] is the old
+ * position of new position i, -1 past new_len.  Entries to an unmapped page
+ * are not copied.
  * max_kv may be up to TMS_EVICT_MAX_KV.
  */
 #define TMS_EVICT_MAX_KV 1048576

@@ -185,7 +185,8 @@ def kv_evict(k_cache, v_cache, scores, tables, kv_len, dst_tables, *, budget: in
     """Cut each sequence to ``budget`` positions a head: the first ``sinks``, the
     last ``recent`` and those of the largest scores stay (ties: the lowest position),
     in order, and go with their scores to ``dst_tables``' pages, which must be none of the
-    sequences' own.  Returns (new_len, kept): int32 ``[batch]`` and the old positions
+    sequences' own.  Positions on unmapped pages are not kept, so a sequence may have fewer
+    than ``budget`` left.  Returns (new_len, kept): int32 ``[batch]`` and the old positions
     ``[batch, kv_heads, budget]``, -1 past new_len."""
     if _OPS is None:
         _ready()

@@ -56,55 +56,95 @@ __device__ __forceinline__ int evict_len(const EvictParams& a, int b) {
 // One workgroup a sequence and head: the key of the last entry kept, by a
 // radix select over the scores' order keys, 8 bits a pass; then the entries
 // above it and the first of those tied with it, in order, at
-// sinks + above + min(tied, those that still fit).
+// sinks + above + min(tied, those that still fit).  The sinks and the last are
+// kept without a look.  Where some of a sequence's positions have no page, nothing
+// of it is known beforehand: all positions are gone through, those without a page below
+// every key and never among the kept, the sinks and the last above every one.
 //
 // Entry j is thread j % 1024's.  Its keys of kBlocks blocks stay in registers,
-// so that a head of up to 16384 entries reads its scores once, all loads in
-// flight together (16 sequences of 1500 to 8192, 8 heads: 29 us with the scores read
-// in each pass); a longer one reads them again for each pass and stretch.
+// so that a head of up to 16384 entries reads its scores once, four blocks' loads in
+// flight together (16 sequences of 1500 to 8192, 8 heads: 15 us; 29 with the scores
+// read in each pass); a longer one reads them again for each pass and stretch.
 constexpr int kBlocks = 16, kStretch = kBlocks * 1024;
 
 __global__ __launch_bounds__(1024) void evict_select_kernel(EvictParams a) {
     __shared__ uint32_t hist[16][256];
     __shared__ uint32_t part[kBlocks * 16][2];   // above and tied before a block's wave
-    __shared__ uint32_t total[256], pick[2];
+    __shared__ uint32_t total[256], pick[2], gone;
     const int b = blockIdx.x / a.c.kv_heads, h = blockIdx.x - b * a.c.kv_heads;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int L = evict_len(a, b);
     const int32_t* row = a.c.tables + (int64_t)b * a.c.tstride;
     int32_t* kept = a.kept + (int64_t)blockIdx.x * a.budget;
-    for (int i = min(L, a.budget) + t; i < a.budget; i += 1024) kept[i] = -1;
-    if (L <= a.budget) {
-        for (int i = t; i < L; i += 1024) kept[i] = i;
-        return;
-    }
-    const int lo = a.sinks, hi = L - a.recent, want = a.budget - a.sinks - a.recent;
-    for (int i = t; i < lo; i += 1024) kept[i] = i;
-    for (int i = t; i < a.recent; i += 1024) kept[a.budget - a.recent + i] = hi + i;
-    if (want == 0) return;
+    int lo = a.sinks, hi = L - a.recent, want = a.budget - a.sinks - a.recent;
 
-    // A score's order key: larger is kept longer.  NaN, and positions on
-    // unmapped pages, come first to go.
+    // A score's order key: larger is kept longer.  No number's is 0, 1 or ~0.
     uint32_t key[kBlocks];
-    auto load = [&](int base) __attribute__((always_inline)) {
-        int page[kBlocks];
-        float s[kBlocks];
+    int page[kBlocks];
+    float score[kBlocks];
+    auto fetch = [&](int base) __attribute__((always_inline)) {   // four blocks' loads without a branch between them
+        auto entry_of = [&](int k) { return min(base + k * 1024 + t, hi - 1); };
 #pragma unroll
-        for (int k = 0; k < kBlocks; ++k)
-            if (base + k * 1024 < hi) page[k] = row[min(base + k * 1024 + t, hi - 1) >> a.c.shift];
+        for (int g = 0; g < kBlocks; g += 4)
+            if (g == 0 || base + g * 1024 < hi)
+#pragma unroll
+                for (int k = g; k < g + 4; ++k) page[k] = row[entry_of(k) >> a.c.shift];
+#pragma unroll
+        for (int g = 0; g < kBlocks; g += 4)
+            if (g == 0 || base + g * 1024 < hi)
+#pragma unroll
+                for (int k = g; k < g + 4; ++k) {
+                    const int at = (unsigned)page[k] < (unsigned)a.c.pages ? page[k] : 0;
+                    score[k] = a.c.scores[(((int64_t)at * a.c.kv_heads + h) << a.c.shift) + (entry_of(k) & a.c.smask)];
+                }
+    };
+    bool holes = false;   // some positions have no page
+    auto keys = [&](int base) __attribute__((always_inline)) {
 #pragma unroll
         for (int k = 0; k < kBlocks; ++k)
             if (base + k * 1024 < hi) {
-                const int j = min(base + k * 1024 + t, hi - 1);
-                const bool ok = (unsigned)page[k] < (unsigned)a.c.pages;
-                s[k] = a.c.scores[(((int64_t)(ok ? page[k] : 0) * a.c.kv_heads + h) << a.c.shift) + (j & a.c.smask)];
-                page[k] = ok;
+                key[k] = score[k] == score[k] ? okey(score[k]) : 1u;
+                if (holes) {
+                    const int j = base + k * 1024 + t;
+                    if (j < a.sinks || j >= L - a.recent) key[k] = ~0u;
+                    if ((unsigned)page[k] >= (unsigned)a.c.pages) key[k] = 0u;
+                }
             }
-#pragma unroll
-        for (int k = 0; k < kBlocks; ++k)
-            if (base + k * 1024 < hi) key[k] = page[k] && s[k] == s[k] ? okey(s[k]) : 0u;
     };
-    if (hi - lo <= kStretch) load(lo);
+    auto load = [&](int base) __attribute__((always_inline)) {
+        fetch(base);
+        keys(base);
+    };
+    // How many positions have no page, counted while the scores are on the way.
+    const int entries = (L + a.c.smask) >> a.c.shift, entry = row[min(t, max(entries - 1, 0))];
+    const bool held = L > a.budget && hi - lo <= kStretch;
+    if (held) fetch(lo);
+    int none = t < entries && (unsigned)entry >= (unsigned)a.c.pages ? min(L - (t << a.c.shift), a.c.smask + 1) : 0;
+    for (int e = t + 1024; e < entries; e += 1024)
+        if ((unsigned)row[e] >= (unsigned)a.c.pages) none += min(L - (e << a.c.shift), a.c.smask + 1);
+    if (t == 0) gone = 0;
+    lds_sync();
+    if (none) atomicAdd(&gone, (uint32_t)none);
+    lds_sync();
+    const int there = L - (int)gone;
+    for (int i = min(there, a.budget) + t; i < a.budget; i += 1024) kept[i] = -1;
+    holes = there < L;
+    if (holes) {
+        lo = 0;
+        hi = L;
+        want = min(there, a.budget);
+        if (want == 0) return;
+        if (hi <= kStretch) load(0);
+    } else {
+        if (L <= a.budget) {
+            for (int i = t; i < L; i += 1024) kept[i] = i;
+            return;
+        }
+        for (int i = t; i < lo; i += 1024) kept[i] = i;
+        for (int i = t; i < a.recent; i += 1024) kept[a.budget - a.recent + i] = hi + i;
+        if (want == 0) return;
+        if (held) keys(lo);
+    }
 
     // Each wave counts into bins of its own, and each finds the digit from the
     // sums by itself: two barriers a pass.  Where a digit's entries are all kept,
@@ -137,14 +177,14 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(EvictParams a) {
             const uint32_t y = __shfl_up(upto, x);
             if (lane >= x) upto += y;
         }
-        uint32_t above = upto - mine, digit = 0, rest = 0, held = 0;
+        uint32_t above = upto - mine, digit = 0, rest = 0, alike = 0;
         bool found = false;
         for (int i = 0; i < 4; ++i) {
             if (above < left && above + n[i] >= left) {
                 found = true;
                 digit = 255 - (4 * lane + i);
                 rest = left - above;
-                held = n[i];
+                alike = n[i];
             }
             above += n[i];
         }
@@ -152,7 +192,7 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(EvictParams a) {
         prefix |= (uint32_t)__builtin_amdgcn_readlane(digit, from) << shift;
         fixed |= 255u << shift;
         left = __builtin_amdgcn_readlane(rest, from);
-        if ((uint32_t)__builtin_amdgcn_readlane(held, from) == left) break;
+        if ((uint32_t)__builtin_amdgcn_readlane(alike, from) == left) break;
     }
 
     uint32_t above0 = 0, tied0 = 0;   // before the stretch
@@ -210,16 +250,16 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(EvictParams a) {
 
 // 16 bytes of a kept entry's key and value a thread, from its old slot to its
 // new one; the first piece's thread moves the score too.  new_len may be the
-// array kv_len: a length read here is the old or the new one, and both give
-// the same number of entries; where those lie is in `kept`.
+// array kv_len: a length read here is the old or the new one, and neither is below
+// the number of entries; which there are, and where they lie, is in `kept`.
 __global__ __launch_bounds__(256) void evict_copy_kernel(EvictParams a, int hv) {
     const int b = blockIdx.x / a.c.kv_heads, h = blockIdx.x - b * a.c.kv_heads;
     const int n = min(evict_len(a, b), a.budget);
     const int end = (int)min(a.c.tstride << a.c.shift, (int64_t)kMaxLen);
-    if (h == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.new_len[b] = n;
     const int32_t* row = a.c.tables + (int64_t)b * a.c.tstride;
     const int32_t* dst = a.dst + (int64_t)b * a.dstride;
     const int32_t* kept = a.kept + (int64_t)blockIdx.x * a.budget;
+    const int last = n > 0 ? kept[n - 1] : 0;
     const int64_t all = (int64_t)n * hv;
     for (int64_t x = (int64_t)blockIdx.y * 256 + threadIdx.x; x < all; x += (int64_t)gridDim.y * 256) {
         const int i = (int)(x / hv), d = (int)(x - (int64_t)i * hv);
@@ -233,6 +273,21 @@ __global__ __launch_bounds__(256) void evict_copy_kernel(EvictParams a, int hv) 
         if (d == 0)
             a.c.scores[(((int64_t)to * a.c.kv_heads + h) << a.c.shift) + s1] =
                 a.c.scores[(((int64_t)from * a.c.kv_heads + h) << a.c.shift) + s0];
+    }
+    if (h == 0 && blockIdx.y == 0 && threadIdx.x < 64) {
+        const int lane = threadIdx.x;
+        int from = n, upto = n;   // the number of entries, at least and at most
+        if (last < 0) {
+            from = 0;
+            upto = n - 1;
+        }
+        while (from < upto) {
+            const int step = (upto - from + 63) / 64, i = from + lane * step;
+            const int k = __popcll(__ballot(i < upto && kept[i] >= 0));
+            upto = k == 0 ? from : min(upto, from + k * step);
+            from = k == 0 ? from : from + (k - 1) * step + 1;
+        }
+        if (lane == 0) a.new_len[b] = from;
     }
 }
 
