@@ -29,6 +29,7 @@ struct Bf16 {
     }
     static __device__ __forceinline__ float up(uint32_t bits16) { return __uint_as_float(bits16 << 16); }
     static constexpr uint32_t kExp = 0x7F80u;   // exponent bits: all set in infinities and NaN
+    static constexpr float kLift = 0.f, kMost = 8.f;   // of a weight's exponent: a row's largest, and what it may grow to
 };
 
 struct F16 {
@@ -45,6 +46,9 @@ struct F16 {
         return (float)__builtin_bit_cast(_Float16, (uint16_t)bits16);
     }
     static constexpr uint32_t kExp = 0x7C00u;
+    // Below 2^-14 the type has fewer bits and below 2^-25 none, above it nearly 2^16:
+    // a row's largest weight is taken as 2^11, so that one 2^-25 of it has all bits yet.
+    static constexpr float kLift = 11.f, kMost = 15.f;
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -174,7 +178,6 @@ inline void set_scale(AttnParams& a, float scale) {
 
 constexpr int kChunkRows = 128;   // of a workgroup of the chunk kernel
 inline int chunk_keys(int head_dim) { return head_dim > 128 ? 32 : 64; }   // of its tile
-constexpr float kSlack = 8.f;
 void launch_attn_chunk(const AttnParams& a, bool bf16, dim3 grid, hipStream_t stream);
 
 __device__ __forceinline__ bool sees(int j, int p, int window, int sinks) {

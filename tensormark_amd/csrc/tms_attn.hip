@@ -2,9 +2,13 @@
 // (tms_paged_attention): single tokens, short chunks of drafts and long chunks
 // of a prompt, with shared key heads, a sliding window and sinks.
 //
-// One pass over the keys with a running maximum m and sum l per row:
-//   m' = max(m, max_j s_j), o = o * 2^(m - m') + sum_j 2^(s_j - m') v_j,
-// with s_j = q . k_j * scale * log2(e).  Rows of one key head are taken
+// One pass over the keys with a running reference m and sum l per row:
+//   m' = max(m, max_j s_j - lift), o = o * 2^(m - m') + sum_j 2^(s_j - m') v_j,
+// with s_j = q . k_j * scale * log2(e), and the lift 0, or what puts a row's weights
+// where fp16 has its bits.  Weights are rounded to the cache's type, half a
+// step, because that is what the matrix instructions take beside it (a second product
+// for what rounding leaves would add half of the matrix work): an output is off
+// by some 0.0008 of itself in bf16 so, beside 0.0017 by its own rounding.  Rows of one key head are taken
 // together: row r of a sequence is token r / G and head r % G of the G query
 // heads that share the key head, so a key read once serves them all.
 //
@@ -261,9 +265,9 @@ __global__ __launch_bounds__(64 * NW, ROWB > 256 ? 1 : 2) void attn_rows_kernel(
 #pragma unroll
             for (int e = 0; e < 16; ++e) top = fmaxf(top, s[e]);
             top *= a.scale;
-            if (__any(top > m + kSlack)) {   // (as in the chunk kernel)
+            if (__any(top > m + T::kMost)) {   // (as in the chunk kernel)
                 top = fmaxf(top, __shfl_xor(top, 32));
-                top = fmaxf(top, m);
+                top = fmaxf(top - T::kLift, m);
                 const float f = __builtin_amdgcn_exp2f(m - (top == -__builtin_huge_valf() ? 0.f : top));
                 m = top;
                 l *= f;
@@ -271,11 +275,13 @@ __global__ __launch_bounds__(64 * NW, ROWB > 256 ? 1 : 2) void attn_rows_kernel(
                 for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
             }
             const float base = m == -__builtin_huge_valf() ? 0.f : m;
+            float sum = 0.f;   // (small weights add up before they meet a large sum)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale, -base));
-                l += s[e];
+                sum += s[e];
             }
+            l += sum;
             u32x4 pf[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u)

@@ -108,13 +108,13 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) s = T::mfma32(key_operand<ROWB>(sk, lane, kt, ks), qf[ks], s);
     };
-    // The reference point follows the maximum once some row's has grown by
-    // 2^kSlack: weights stay below that, which neither type minds.
+    // The reference point lies 2^kLift below the maximum, and follows it once some
+    // row's has grown past 2^kMost above: weights stay below that, in either type's range.
     auto refer = [&](float top) __attribute__((always_inline)) {
         top *= a.scale;
-        if (__any(top > m + kSlack)) {
+        if (__any(top > m + T::kMost)) {
             top = fmaxf(top, __shfl_xor(top, 32));
-            top = fmaxf(top, m);
+            top = fmaxf(top - T::kLift, m);
             const float f = __builtin_amdgcn_exp2f(m - (top == -__builtin_huge_valf() ? 0.f : top));
             m = top;
             l *= f;
@@ -129,12 +129,13 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
     };
     auto weigh = [&](f32x16& s, u32x4 (&pf)[2]) __attribute__((always_inline)) {
         const float base = m == -__builtin_huge_valf() ? 0.f : m;
+        float sum = 0.f;   // (small weights add up before they meet a large sum)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const float x = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale, -base));
-            s[e] = x;
-            l += x;
+            s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale, -base));
+            sum += s[e];
         }
+        l += sum;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
