@@ -2,7 +2,8 @@
  * tmcache_hip.h -- C ABI of the paged key/value cache operators (gfx950), in
  * the same library as tmsample_hip.h and by the same rules: device pointers,
  * sizes, a hipStream_t, an int status; the calls allocate nothing, are
- * stream-ordered, never synchronise and can be captured into a HIP graph.
+ * stream-ordered, never synchronise and can be captured into a HIP graph, and
+ * run on the current device (the stream's device must be current).
  * There is no context: scratch memory is the caller's (`workspace`).
  * TensorMark keeps one sequence's keys and values in one flat host buffer
  * (tensormark/llama.h, the kv_* members of Llama); nothing of it is paged or

@@ -53,7 +53,8 @@ OPS_SOURCE = "tms_cache_py.cpp"
 OPS = os.path.join(HERE, "_cache_ops.so")
 
 
-def _ops_command(out: str) -> list:
+def ops_command(out: str, source: str = os.path.join(CSRC, OPS_SOURCE), optimize: str = "-O2", library: bool = True) -> list:
+    """The command that builds the module `out` of `source`, with libtmsample_hip.so or what the source has in its place."""
     import sysconfig
 
     import torch
@@ -62,9 +63,9 @@ def _ops_command(out: str) -> list:
     rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
     system = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
               os.path.join(rocm, "include"), sysconfig.get_paths()["include"]]
-    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__",
+    return ["g++", optimize, "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__",
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", os.path.join(ROOT, "include"),
-            *[x for d in system for x in ("-isystem", d)], os.path.join(CSRC, OPS_SOURCE), "-o", out, "-L", HERE, "-ltmsample_hip",
+            *[x for d in system for x in ("-isystem", d)], source, "-o", out, *(["-L", HERE, "-ltmsample_hip"] if library else []),
             "-L", os.path.join(root, "lib"), "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
 
 
@@ -140,7 +141,7 @@ def build(verbose: bool = False) -> str:
             _check_lds(src, rem)
     _run([hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB + ".tmp", *[j[1] for j in jobs]], verbose)
     os.replace(LIB + ".tmp", LIB)
-    _run(_ops_command(OPS + ".tmp"), verbose)
+    _run(ops_command(OPS + ".tmp"), verbose)
     os.replace(OPS + ".tmp", OPS)
     return LIB
 

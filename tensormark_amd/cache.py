@@ -10,7 +10,7 @@ a sequence's positions, its new tokens among them; ``q_start`` (int32
 ``max_kv`` are the host's bounds on a sequence's new tokens and positions: the
 lengths themselves stay on the device and nothing is synchronised.
 
-The calls run on the current stream (or ``stream``), allocate only what they
+The calls run on the tensors' device, on its current stream (or ``stream``), allocate only what they
 return and, for ``paged_attention``, a workspace, with torch's allocator.  They raise
 ValueError for tensors that do not fit and RuntimeError for what the library
 refuses; there is no fallback.

@@ -4,6 +4,7 @@
 // same checks in Python with ctypes took 7 to 12 us of the host besides the launch;
 // a call is 4.5 to 9 us of the host with this (a token of each of 64 sequences into
 // the cache: 11.0 us with ctypes, 4.3 with this; one session's attention: 15.0 and 11.6).
+#include <c10/core/DeviceGuard.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -28,6 +29,15 @@ static void check(int rc, const char* call) {
 }
 
 static int gpu_of(const Tensor& t) { return t.is_cuda() ? t.get_device() : -1; }
+
+// The device of a call's tensors as the current one: a launch into the null stream, torch's default, goes
+// to the current device, wherever the tensors are.
+struct OnDeviceOf {
+    c10::OptionalDeviceGuard guard;
+    explicit OnDeviceOf(const Tensor& t) {
+        if (t.is_cuda()) guard.reset_device(t.device());
+    }
+};
 
 // A number of Python's as 32 bits, for the library to judge; none is a smaller one by wrapping.
 static int32_t i32(int64_t n) { return (int32_t)std::clamp<int64_t>(n, INT32_MIN, INT32_MAX); }
@@ -112,6 +122,7 @@ static hipStream_t stream_of(int64_t stream) { return reinterpret_cast<hipStream
 
 static void kv_append(const Tensor& k_new, const Tensor& v_new, const Tensor& k, const Tensor& v, const Tensor& tables,
                       const Tensor& kv_len, const Tensor& q_start, int64_t max_q, const MaybeTensor& scores, int64_t stream) {
+    const OnDeviceOf on(k);
     const tms_cache c = cache_of(k, &v, scores ? &*scores : nullptr, tables, kv_len, &q_start, k_new.dim() ? k_new.size(0) : 0, max_q, 0);
     tms_append_args a{};
     rows(k_new, k, a.k_new_stride, "k_new: [tokens, heads, head_dim] like k_cache, last stride 1");
@@ -126,6 +137,7 @@ static std::tuple<Tensor, Tensor> paged_attention(const Tensor& q, const Tensor&
                                                   const Tensor& kv_len, const Tensor& q_start, int64_t max_q, int64_t max_kv,
                                                   int64_t window, int64_t sinks, std::optional<double> scale,
                                                   const MaybeTensor& out_, const MaybeTensor& lse_, int64_t stream) {
+    const OnDeviceOf on(k);
     const tms_cache c = cache_of(k, &v, nullptr, tables, kv_len, &q_start, q.dim() ? q.size(0) : 0, max_q, max_kv);
     tms_attention_args a{};
     rows(q, k, a.q_stride, "q: [tokens, heads, head_dim] like k_cache, last stride 1");
@@ -155,6 +167,7 @@ static std::tuple<Tensor, Tensor> paged_attention(const Tensor& q, const Tensor&
 static Tensor kv_add_scores(const Tensor& q, const Tensor& lse, const Tensor& k, const MaybeTensor& scores, const Tensor& tables,
                             const Tensor& kv_len, const Tensor& q_start, int64_t max_q, int64_t max_kv, int64_t window, int64_t sinks,
                             std::optional<double> scale, const MaybeTensor& out_, int64_t stream) {
+    const OnDeviceOf on(k);
     want(scores.has_value(), "scores: needed");
     const tms_cache c = cache_of(k, nullptr, &*scores, tables, kv_len, &q_start, q.dim() ? q.size(0) : 0, max_q, max_kv);
     tms_score_args a{};
@@ -176,6 +189,7 @@ static Tensor kv_add_scores(const Tensor& q, const Tensor& lse, const Tensor& k,
 static std::tuple<Tensor, Tensor> kv_evict(const Tensor& k, const Tensor& v, const MaybeTensor& scores, const Tensor& tables,
                                            const Tensor& kv_len, const Tensor& dst_tables, int64_t budget, int64_t max_kv, int64_t sinks,
                                            int64_t recent, const MaybeTensor& new_len_, const MaybeTensor& kept_, int64_t stream) {
+    const OnDeviceOf on(k);
     want(scores.has_value(), "scores: needed");
     const tms_cache c = cache_of(k, &v, &*scores, tables, kv_len, nullptr, 0, 0, max_kv);
     const int device = gpu_of(k);
@@ -210,6 +224,7 @@ static bool row_contiguous(const Tensor& t) { return t.stride(1) == 1 || t.size(
 static Tensor adjust_logits(const Tensor& logits, const MaybeTensor& params, const MaybeTensor& recent, const MaybeTensor& n_recent,
                             const MaybeTensor& drafts, int64_t steps, const MaybeTensor& bias_ids, const MaybeTensor& bias_values,
                             const MaybeTensor& mask, const MaybeTensor& out_, int64_t stream) {
+    const OnDeviceOf on(logits);
     want(logits.dim() == 2 && dtype_code(logits) >= 0 && logits.is_cuda() && row_contiguous(logits),
          "logits: device [rows, vocab] of float32, float16 or bfloat16, last stride 1");
     const int device = gpu_of(logits);
