@@ -39,6 +39,23 @@ struct OnDeviceOf {
     }
 };
 
+static const Tensor* of(const MaybeTensor& t) { return t ? &*t : nullptr; }
+
+// No call has a backward: a gradient that would have to go through one is refused.
+static void want_no_gradient(std::initializer_list<const Tensor*> tensors) {
+    if (!at::GradMode::is_enabled()) return;
+    for (const Tensor* t : tensors)
+        want(!t || !t->requires_grad(), "no gradient goes through this call: detach its tensors, or call it under torch.no_grad()");
+}
+
+// Autograd finds by its version that a tensor it kept has been written (inference tensors have none).
+static void written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+static void written(const MaybeTensor& t) {
+    if (t) written(*t);
+}
+
 // A number of Python's as 32 bits, for the library to judge; none is a smaller one by wrapping.
 static int32_t i32(int64_t n) { return (int32_t)std::clamp<int64_t>(n, INT32_MIN, INT32_MAX); }
 
@@ -122,8 +139,9 @@ static hipStream_t stream_of(int64_t stream) { return reinterpret_cast<hipStream
 
 static void kv_append(const Tensor& k_new, const Tensor& v_new, const Tensor& k, const Tensor& v, const Tensor& tables,
                       const Tensor& kv_len, const Tensor& q_start, int64_t max_q, const MaybeTensor& scores, int64_t stream) {
+    want_no_gradient({&k_new, &v_new, &k, &v, of(scores)});
     const OnDeviceOf on(k);
-    const tms_cache c = cache_of(k, &v, scores ? &*scores : nullptr, tables, kv_len, &q_start, k_new.dim() ? k_new.size(0) : 0, max_q, 0);
+    const tms_cache c = cache_of(k, &v, of(scores), tables, kv_len, &q_start, k_new.dim() ? k_new.size(0) : 0, max_q, 0);
     tms_append_args a{};
     rows(k_new, k, a.k_new_stride, "k_new: [tokens, heads, head_dim] like k_cache, last stride 1");
     rows(v_new, k, a.v_new_stride, "v_new: [tokens, heads, head_dim] like k_cache, last stride 1");
@@ -131,12 +149,16 @@ static void kv_append(const Tensor& k_new, const Tensor& v_new, const Tensor& k,
     a.k_new = k_new.data_ptr();
     a.v_new = v_new.data_ptr();
     check(tms_kv_append(&c, &a, stream_of(stream)), "tms_kv_append");
+    written(k);
+    written(v);
+    written(scores);
 }
 
 static std::tuple<Tensor, Tensor> paged_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& tables,
                                                   const Tensor& kv_len, const Tensor& q_start, int64_t max_q, int64_t max_kv,
                                                   int64_t window, int64_t sinks, std::optional<double> scale,
                                                   const MaybeTensor& out_, const MaybeTensor& lse_, int64_t stream) {
+    want_no_gradient({&q, &k, &v, of(out_), of(lse_)});
     const OnDeviceOf on(k);
     const tms_cache c = cache_of(k, &v, nullptr, tables, kv_len, &q_start, q.dim() ? q.size(0) : 0, max_q, max_kv);
     tms_attention_args a{};
@@ -161,12 +183,15 @@ static std::tuple<Tensor, Tensor> paged_attention(const Tensor& q, const Tensor&
         a.workspace_bytes = (size_t)need;
     }
     check(tms_paged_attention(&c, &a, stream_of(stream)), "tms_paged_attention");
+    written(out_);
+    written(lse_);
     return {out, lse};
 }
 
 static Tensor kv_add_scores(const Tensor& q, const Tensor& lse, const Tensor& k, const MaybeTensor& scores, const Tensor& tables,
                             const Tensor& kv_len, const Tensor& q_start, int64_t max_q, int64_t max_kv, int64_t window, int64_t sinks,
                             std::optional<double> scale, const MaybeTensor& out_, int64_t stream) {
+    want_no_gradient({&q, &lse, &k, of(scores), of(out_)});
     const OnDeviceOf on(k);
     want(scores.has_value(), "scores: needed");
     const tms_cache c = cache_of(k, nullptr, &*scores, tables, kv_len, &q_start, q.dim() ? q.size(0) : 0, max_q, max_kv);
@@ -183,12 +208,14 @@ static Tensor kv_add_scores(const Tensor& q, const Tensor& lse, const Tensor& k,
     a.sinks = i32(sinks);
     a.scale = scale_of(scale, q);
     check(tms_kv_add_scores(&c, &a, stream_of(stream)), "tms_kv_add_scores");
+    written(out);
     return out;
 }
 
 static std::tuple<Tensor, Tensor> kv_evict(const Tensor& k, const Tensor& v, const MaybeTensor& scores, const Tensor& tables,
                                            const Tensor& kv_len, const Tensor& dst_tables, int64_t budget, int64_t max_kv, int64_t sinks,
                                            int64_t recent, const MaybeTensor& new_len_, const MaybeTensor& kept_, int64_t stream) {
+    want_no_gradient({&k, &v, of(scores)});
     const OnDeviceOf on(k);
     want(scores.has_value(), "scores: needed");
     const tms_cache c = cache_of(k, &v, &*scores, tables, kv_len, nullptr, 0, 0, max_kv);
@@ -207,6 +234,11 @@ static std::tuple<Tensor, Tensor> kv_evict(const Tensor& k, const Tensor& v, con
     a.new_len = const_cast<int32_t*>(ints(new_len, {B}, "new_len", device));
     a.kept = const_cast<int32_t*>(ints(kept, {B, H, budget}, "kept", device));
     check(tms_kv_evict(&c, &a, stream_of(stream)), "tms_kv_evict");
+    written(k);
+    written(v);
+    written(*scores);
+    written(new_len_);
+    written(kept_);
     return {new_len, kept};
 }
 
@@ -224,6 +256,7 @@ static bool row_contiguous(const Tensor& t) { return t.stride(1) == 1 || t.size(
 static Tensor adjust_logits(const Tensor& logits, const MaybeTensor& params, const MaybeTensor& recent, const MaybeTensor& n_recent,
                             const MaybeTensor& drafts, int64_t steps, const MaybeTensor& bias_ids, const MaybeTensor& bias_values,
                             const MaybeTensor& mask, const MaybeTensor& out_, int64_t stream) {
+    want_no_gradient({&logits, of(bias_values), of(out_)});
     const OnDeviceOf on(logits);
     want(logits.dim() == 2 && dtype_code(logits) >= 0 && logits.is_cuda() && row_contiguous(logits),
          "logits: device [rows, vocab] of float32, float16 or bfloat16, last stride 1");
@@ -279,6 +312,7 @@ static Tensor adjust_logits(const Tensor& logits, const MaybeTensor& params, con
     a.logits = logits.data_ptr();
     a.out = out.data_ptr();
     check(tms_adjust_logits(&a, stream_of(stream)), "tms_adjust_logits");
+    written(out_);
     return out;
 }
 
