@@ -127,7 +127,7 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(EvictParams a) {
     if (none) atomicAdd(&gone, (uint32_t)none);
     lds_sync();
     const int there = L - (int)gone;
-    for (int i = min(there, a.budget) + t; i < a.budget; i += 1024) kept[i] = -1;
+    for (int64_t i = min(there, a.budget) + t; i < a.budget; i += 1024) kept[i] = -1;   // (a budget may be any: 32 bits would wrap)
     holes = there < L;
     if (holes) {
         lo = 0;

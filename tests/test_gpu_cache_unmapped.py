@@ -82,3 +82,18 @@ def test_positions_without_a_page_are_not_kept(kv, gone, budget, sinks, recent, 
             got = bt.scores[p, h, s].cpu()
             assert torch.equal(got.view(torch.int32), bt.sums[b][want[b][h], h].view(torch.int32))
     check(after)
+
+
+@pytest.mark.parametrize("budget", [2 ** 31 - 1, 2 ** 31 - 1024, 2 ** 31 - 1025])
+def test_a_budget_that_is_no_limit(budget):
+    """All is kept; every place of `kept` past that says so, up to the last of 8 GiB."""
+    bt = Batch([50], [0], H=1, D=64, page=16, seed=3, extra=4)
+    used = set(bt.host[bt.host >= 0].tolist())
+    dst = torch.tensor([[p for p in range(bt.k.shape[0]) if p not in used][:4]], dtype=torch.int32, device=DEV)
+    kept = torch.full((1, 1, budget), 7, dtype=torch.int32, device=DEV)
+    new_len, _ = tm.kv_evict(bt.k, bt.v, bt.scores, bt.tables, bt.kv_len, dst, budget=budget, max_kv=50, sinks=4, recent=8, kept=kept)
+    assert new_len.tolist() == [50] and kept[0, 0, :50].tolist() == list(range(50))
+    assert all(bool((part == -1).all()) for part in kept[0, 0, 50:].split(1 << 28))
+    p, s = bt.where(0, np.arange(50))
+    to, at = dst[0][torch.arange(50, device=DEV) // 16].long(), torch.arange(50, device=DEV) % 16
+    assert torch.equal(bt.k[to, 0, at], bt.k[p, 0, s]) and torch.equal(bt.scores[to, 0, at], bt.scores[p, 0, s])
