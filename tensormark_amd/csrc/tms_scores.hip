@@ -181,7 +181,13 @@ __global__ __launch_bounds__(256, KS > 8 ? 2 : 3) void score_kernel(AttnParams a
         }
         if (t0 > pl || t0 >= sq.len || (a.window > 0 && t0 + 31 <= pf - a.window && t0 >= a.sinks)) continue;
         const bool edge = t0 + 31 > pf || (a.window > 0 && t0 <= pl - a.window && t0 + 32 > a.sinks);
-        auto mask = [&](f32x16& x, int half) __attribute__((always_inline)) {
+        auto mask = [&](f32x16& x, int half, float& lse) __attribute__((always_inline)) {
+            // A lse that is no number makes one of -inf no more: such a row's scores take its place.
+            if (__any(lse != lse)) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = lse != lse ? lse : x[i];
+                lse = lse != lse ? 0.f : lse;
+            }
             int pos = pf + prow[half];
             if (!whole) {
                 split_row(r + 32 * half + n32, G, inv, pos, hd);
@@ -193,11 +199,11 @@ __global__ __launch_bounds__(256, KS > 8 ? 2 : 3) void score_kernel(AttnParams a
                 if (!sees(t0 + 8 * (i / 4) + 4 * hh + (i & 3), pos, a.window, a.sinks)) x[i] = -__builtin_huge_valf();
         };
         stage(sm[buf], 0, s0, s1, lse1);
-        if (edge) mask(s0, 0);
         lse0 = sm_lse[buf][n32];
+        if (edge) mask(s0, 0, lse0);
         stage(sm[buf], 1, s1, s0, lse0);
-        if (edge) mask(s1, 1);
         lse1 = sm_lse[buf][32 + n32];
+        if (edge) mask(s1, 1, lse1);
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) sum[i] += __builtin_amdgcn_exp2f(fmaf(s1[i], a.scale, -lse1));

@@ -43,3 +43,35 @@ def test_many_small_weights_beside_a_large_one(q, G, D, copies, dt):
     tiny = torch.finfo(dt).smallest_normal * half if dt == HF else 0.0   # half a step of an output below the normal ones
     assert torch.all((o - want).abs() <= (2 * half + 2 * err) * want + tiny)
     assert torch.all((l - (1 + n * w).log()[..., 0]).abs() <= err + 8 * U)
+
+
+def added(bt, lse, window=0, sinks=0, odd=None):
+    """kv_add_scores onto sums of its own, checked where the definition gives a number: what rows
+    without one add is none, to the keys they see and to no others."""
+    with np.errstate(invalid="ignore"):
+        weights, wtol = bt.reference(window, sinks)[4:]
+    out = torch.full_like(bt.scores, 7.0)
+    tm.kv_add_scores(bt.qs.to(DEV), lse, bt.k, bt.scores, bt.tables, bt.kv_len, bt.q_start, max_q=bt.max_q, max_kv=bt.max_kv,
+                     window=window, sinks=sinks, out=out)
+    most = lse[torch.isfinite(lse)].abs().max().item()
+    for b, n in enumerate(bt.kv):
+        p, s = bt.where(b, np.arange(n))
+        new = out[p, :, s].double().cpu().numpy()
+        for h in range(bt.H):
+            w, had = weights[b * bt.H + h], bt.sums[b][:, h].double().numpy()
+            none = np.isnan(w)
+            # paged_attention's lse is off by what its own sums and exponentials are (as the weights) and a rounding
+            slack = 2 * wtol[b * bt.H + h] + w * U * 10 * most + 2 * U * np.abs(had + w)
+            assert np.array_equal(np.isnan(new[:, h]), none), (h, np.flatnonzero(np.isnan(new[:, h]) != none)[:9])
+            assert np.all(np.abs(new[:, h] - had - w)[~none] <= slack[~none])
+    return out
+
+
+@pytest.mark.parametrize("window, sinks", [(0, 0), (30, 4)])
+@pytest.mark.parametrize("q, G, D, dt", [(9, 2, 64, BF), (60, 2, 80, HF), (150, 1, 128, BF), (100, 3, 64, HF), (5, 70, 256, BF)])
+def test_a_query_that_is_no_number_reaches_the_keys_it_sees(q, G, D, dt, window, sinks):
+    bt = Batch([200], [q], H=1, G=G, D=D, dt=dt, seed=q)
+    bt.qs[q // 2, G - 1, 3] = float("nan")
+    lse = bt.attend(window=window, sinks=sinks)[1]
+    assert torch.isnan(lse[q // 2, G - 1]) and int(torch.isnan(lse).sum()) == 1
+    added(bt, lse, window, sinks)
