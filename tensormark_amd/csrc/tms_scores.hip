@@ -71,13 +71,15 @@ __global__ __launch_bounds__(256, KS > 8 ? 2 : 3) void score_kernel(AttnParams a
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)&sm[0][0];
     uint32_t off[NI];
     int loff, tok0 = first;   // the lane's row's lse; the token that the offsets count from
+    // A place of the tile without a row (past its last whole token, past the last row of
+    // all) has its first row, at no weight: zeros there, times an infinite key, would be no number.
     auto offsets = [&](int hd0) __attribute__((always_inline)) {   // rows from head hd0 of the token on
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int rr = (wave * NI + i) * RPI + lane / C, piece = (lane % C) ^ key_swizzle<ROWB>(rr);
             int tok, hd;
-            split_row(hd0 + rr, G, inv, tok, hd);
-            off[i] = rr < step && piece * 8 < D ? (uint32_t)(tok * (int)a.qt + hd * (int)a.qh + piece * 16) : 0x80000000u;
+            split_row(rr < step ? hd0 + rr : hd0, G, inv, tok, hd);
+            off[i] = piece * 8 < D ? (uint32_t)(tok * (int)a.qt + hd * (int)a.qh + piece * 16) : 0x80000000u;
         }
         int tok, hd;
         split_row(hd0 + lane, G, inv, tok, hd);
@@ -86,17 +88,24 @@ __global__ __launch_bounds__(256, KS > 8 ? 2 : 3) void score_kernel(AttnParams a
     offsets(0);
     // The tile from row r (token tok0) on: its last row's end bounds the resource.
     auto load = [&](int r, int buf) __attribute__((always_inline)) {
+        int hd0 = 0;
         if (!whole) {
-            int hd0;
             split_row(r, G, inv, tok0, hd0);
             offsets(hd0);
         }
         const char* base = qbase + (int64_t)__builtin_amdgcn_readfirstlane(tok0) * a.qt;
         const int left = rend - r;   // rows
+        if (left < step) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int rr = (wave * NI + i) * RPI + lane / C, piece = (lane % C) ^ key_swizzle<ROWB>(rr);
+                if (rr >= left && piece * 8 < D) off[i] = hd0 * (int)a.qh + piece * 16;
+            }
+        }
         const u32x4 res = (u32x4){(uint32_t)(uintptr_t)base, (uint32_t)((uintptr_t)base >> 32) & 0xFFFF, 0x7FFFFFFFu, 0x00020000u};
 #pragma unroll
         for (int i = 0; i < NI; ++i)
-            load_lds16(res, (wave * NI + i) * RPI + lane / C < left ? off[i] : 0x80000000u, lds0 + buf * RQ * ROWB + (wave * NI + i) * 1024);
+            load_lds16(res, off[i], lds0 + buf * RQ * ROWB + (wave * NI + i) * 1024);
     };
     auto lse_of = [&](int r) __attribute__((always_inline)) {   // the first wave's: row r + lane; a row that is none gets no weight
         const float x = lbase[(int64_t)tok0 * a.q_heads + (lane < step && r + lane < rend ? loff : 0)];

@@ -75,3 +75,22 @@ def test_a_query_that_is_no_number_reaches_the_keys_it_sees(q, G, D, dt, window,
     lse = bt.attend(window=window, sinks=sinks)[1]
     assert torch.isnan(lse[q // 2, G - 1]) and int(torch.isnan(lse).sum()) == 1
     added(bt, lse, window, sinks)
+
+
+@pytest.mark.parametrize("q, G, D, dt", [(9, 2, 64, BF), (60, 2, 80, HF), (70, 3, 64, HF), (45, 1, 128, BF), (5, 70, 256, BF)])
+def test_a_key_that_every_row_scores_minus_infinity(q, G, D, dt):
+    """Its weight is zero in attention, and so is what its score grows by; the others' are right."""
+    bt = Batch([300], [q], H=1, G=G, D=D, dt=dt, seed=q)
+    bt.qs[..., 2] = bt.qs[..., 2].abs() + 0.25
+    low = [1, 40, 130, 220]
+    bt.keys[0][low, 0, 2] = float("-inf")
+    bt.fill()
+    lse = bt.attend()[1]
+    assert torch.isfinite(lse).all()
+    out = torch.full_like(bt.scores, 7.0)
+    tm.kv_add_scores(bt.qs.to(DEV), lse, bt.k, bt.scores, bt.tables, bt.kv_len, bt.q_start, max_q=q, max_kv=300, out=out)
+    p, s = bt.where(0, np.arange(300))
+    grown = (out[p, 0, s].double() - bt.scores[p, 0, s].double()).cpu()
+    assert torch.all(grown[low] == 0)
+    # every row's weights sum to one: (kv + rows + 32) steps of fp32, and a step of each sum so far
+    assert abs(float(grown.sum()) - q * G) <= q * G * (300 + 32) * U + U * float(out[p, 0, s].double().sum())
