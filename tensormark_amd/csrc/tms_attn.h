@@ -64,6 +64,7 @@ struct AttnParams {
     int64_t ot, oh;
     int group, q_heads;
     int window, sinks;     // window 0: none
+    int max_kv;            // scores: positions past it are left out
     float scale;           // above 0, times log2(e): exponentials are taken to base 2
     uint32_t qand, qxor;   // a query's bits are taken through these: a scale below 0 flips its sign, 0 clears it
     int split_tiles;       // chunk kernel: key tiles a split has; rows kernel: the least that a share has

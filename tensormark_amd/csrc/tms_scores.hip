@@ -46,7 +46,8 @@ __global__ __launch_bounds__(256, KS > 8 ? 2 : 3) void score_kernel(AttnParams a
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n32 = lane & 31, hh = lane >> 5;
     const int pair = blockIdx.x, b = pair / a.c.kv_heads, h = pair - b * a.c.kv_heads;
-    const SeqView sq = seq_view(a.c, b);
+    SeqView sq = seq_view(a.c, b);
+    sq.len = min(sq.len, a.max_kv);
     const int g0 = blockIdx.y * 128, t0 = g0 + wave * 32;
     if (g0 >= sq.len) return;
     const int G = a.group, D = a.c.head_dim;
@@ -231,7 +232,8 @@ __global__ __launch_bounds__(256, KS > 8 ? 2 : 3) void score_rows_kernel(AttnPar
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n32 = lane & 31, hh = lane >> 5;
     const int pair = blockIdx.x, b = pair / a.c.kv_heads, h = pair - b * a.c.kv_heads;
-    const SeqView sq = seq_view(a.c, b);
+    SeqView sq = seq_view(a.c, b);
+    sq.len = min(sq.len, a.max_kv);
     const int t0 = (blockIdx.y * 4 + wave) * 32 * KT;
     if (t0 >= sq.len) return;
     const int G = a.group, rows = sq.n * G, D = a.c.head_dim;
@@ -334,6 +336,7 @@ extern "C" int tms_kv_add_scores(const tms_cache* cache, const tms_score_args* a
     a.qh = 2 * args->q_stride[1];
     a.q_heads = args->q_heads;
     a.group = args->q_heads / cache->kv_heads;
+    a.max_kv = cache->max_kv;
     a.window = args->window > 0 && args->window < kMaxLen ? args->window : 0;
     a.sinks = std::min(args->sinks, kMaxLen);
     set_scale(a, args->scale);
