@@ -41,7 +41,9 @@ extern "C" {
 #define TMS_CACHE_MIN_PAGE 8
 #define TMS_CACHE_MAX_PAGE 65536
 #define TMS_ATTENTION_MAX_SLOT_STRIDE 67108864   /* elements; tms_paged_attention */
-#define TMS_ATTENTION_MAX_ROWS 2097152           /* max_q times query heads a key head */
+#define TMS_ATTENTION_MAX_ROWS 2097152           /* max_q times query heads a key head; where a page's stride or
+                                                    slots span 2^32 bytes, batch times kv_heads times
+                                                    tiles of 32 such rows is below 2^31 too */
 #define TMS_SCORES_MAX_Q_STRIDE 8388608          /* elements between tokens, and that a key head's
                                                     query heads span; tms_kv_add_scores */
 

@@ -498,6 +498,7 @@ constexpr int kWholeTiles = 32;
 
 struct AttnPlan {
     bool chunk;        // the chunk kernel
+    bool fits;         // its items are counted in 32 bits
     int rm;            // rows a workgroup
     int row_tiles;
     int split_tiles, splits;
@@ -531,6 +532,7 @@ static AttnPlan plan_attention(const tms_cache* c, const tms_attention_args* a) 
     if (a->window > 0) keys = std::min<int64_t>(keys, (int64_t)a->window + p.rm + a->sinks + 128);
     const int64_t items = (int64_t)c->batch * c->kv_heads * p.row_tiles;
     int64_t parts;
+    p.fits = p.chunk || items <= INT32_MAX;
     p.splits = p.shares = 0;
     p.item_bytes = 0;
     if (p.chunk) {
@@ -598,6 +600,7 @@ extern "C" int64_t tms_paged_attention_workspace(const tms_cache* cache, const t
     const int rc = tms::check_attention(cache, args);
     if (rc != TMS_OK) return rc;
     const tms::AttnPlan p = tms::plan_attention(cache, args);
+    if (!p.fits) return TMS_ERR_CAPACITY;
     return (int64_t)(p.o_bytes + p.ml_bytes + p.item_bytes);
 }
 
@@ -607,6 +610,7 @@ extern "C" int tms_paged_attention(const tms_cache* cache, const tms_attention_a
     if (rc != TMS_OK) return rc;
     if (cache->batch == 0 || cache->tokens == 0 || cache->max_q == 0) return TMS_OK;
     const AttnPlan p = plan_attention(cache, args);
+    if (!p.fits) return TMS_ERR_CAPACITY;
     if (args->workspace_bytes < p.o_bytes + p.ml_bytes + p.item_bytes ||
         (p.join && (!args->workspace || !aligned16(args->workspace))))
         return TMS_ERR_INVALID_ARG;

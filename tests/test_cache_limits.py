@@ -66,3 +66,16 @@ def test_a_workspace_for_every_form():
     assert need[0] == need[1] == 0 and need[2] > 0 and need == sorted(need)
     c = a_cache(max_kv=50000, table_stride=40000, tokens=90, max_q=30)
     assert lib.tms_paged_attention_workspace(C.byref(c), C.byref(rows_args(cache.AttentionArgs))) > 0
+
+
+def test_more_items_than_32_bits_count():
+    """Strides past the chunk kernel's offsets, and so many sequences and rows that tiles of
+    32 rows are past 2^31: refused; the same with ordinary strides is not."""
+    def call(batch, heads, far):
+        c = a_cache(batch=batch, kv_heads=heads, tokens=1 << 20, max_q=1 << 20, page_size=65536)
+        for s in (c.k_stride, c.v_stride):
+            s[0], s[1], s[2] = 0, 0, 1 << 25 if far else 64
+        return cache._fns().tms_paged_attention_workspace(C.byref(c), C.byref(rows_args(cache.AttentionArgs, q_heads=2 * heads)))
+
+    assert call(1 << 15, 1, True) == CAPACITY and call(1 << 14, 2, True) == CAPACITY
+    assert call((1 << 15) - 1, 1, True) > 0 and call(1 << 15, 1, False) >= 0
