@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import os
 import re
+import shutil
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
@@ -48,7 +49,8 @@ FILE_FLAGS = {
 BUILD_DIR = os.path.join(HERE, "_build")
 
 # The cache calls' Python side over torch tensors: a module of its own, since it
-# needs torch's headers and libraries, which libtmsample_hip.so does not.
+# needs torch's headers and libraries, which libtmsample_hip.so does not.  Host
+# code alone; where there is no torch or no g++ it is left out.
 OPS_SOURCE = "tms_cache_py.cpp"
 OPS = os.path.join(HERE, "_cache_ops.so")
 
@@ -63,6 +65,8 @@ def ops_command(out: str, source: str = os.path.join(CSRC, OPS_SOURCE), optimize
     rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
     system = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
               os.path.join(rocm, "include"), sysconfig.get_paths()["include"]]
+    if shutil.which("g++") is None:   # (torch's own compiler; hipcc mangles some of its templates otherwise)
+        raise ImportError("g++ is not there")
     return ["g++", optimize, "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__",
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", os.path.join(ROOT, "include"),
             *[x for d in system for x in ("-isystem", d)], source, "-o", out, *(["-L", HERE, "-ltmsample_hip"] if library else []),
@@ -141,7 +145,14 @@ def build(verbose: bool = False) -> str:
             _check_lds(src, rem)
     _run([hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB + ".tmp", *[j[1] for j in jobs]], verbose)
     os.replace(LIB + ".tmp", LIB)
-    _run(ops_command(OPS + ".tmp"), verbose)
+    try:
+        command = ops_command(OPS + ".tmp")
+    except ImportError as e:
+        print(f"built without _cache_ops.so, the Python side of the cache calls: {e}", file=sys.stderr)
+        if os.path.exists(OPS):   # (of a library that may be another)
+            os.remove(OPS)
+        return LIB
+    _run(command, verbose)
     os.replace(OPS + ".tmp", OPS)
     return LIB
 

@@ -122,7 +122,10 @@ def _ready():
     load_library()   # (says how to build, if it is not)
     import torch
 
-    from . import _cache_ops
+    try:
+        from . import _cache_ops
+    except ImportError as e:
+        raise ImportError(f"the cache calls' module is not built, or not for this torch: run python -m tensormark_amd.build ({e})") from e
 
     _OPS, _RAW_STREAM = _cache_ops, torch._C._cuda_getCurrentRawStream
 
