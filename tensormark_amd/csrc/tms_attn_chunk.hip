@@ -24,6 +24,7 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
     constexpr int C = ROWB / 16, RPI = 64 / C, NI = KT / (4 * RPI);   // pieces a row; rows a load; loads a wave
     constexpr uint32_t ALL = (1u << KT / 8) - 1;
     constexpr bool FUSED = ROWB > 256;
+    static_assert(NK == (FUSED ? 1 : 2), "a tile's keys by 32");
     constexpr int NV = FUSED ? 3 : 2;   // value buffers
     __shared__ __attribute__((aligned(128))) char sm_k[2][KT * ROWB];
     __shared__ __attribute__((aligned(128))) char sm_v[NV][KT * ROWB];
@@ -151,19 +152,19 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
     // Scores of 32 keys, while the weights of the 32 before (`s`) are worked out
     // and go to the outputs; returns the maximum.  The order is written out: a
     // matrix instruction, some weights, the operands of two steps on.
-    auto fused = [&](const char* sk, int kt, f32x16& next, f32x16& s, const char* sv, int vt) __attribute__((always_inline)) {
+    auto fused = [&](const char* sk, f32x16& next, f32x16& s, const char* sv) __attribute__((always_inline)) {
         const float base = m == low ? 0.f : m;
         u32x4 kf[3], vf[3], pf[2];
         float sum = 0.f, top = low;
 #pragma unroll
         for (int i = 0; i < 16; ++i) next[i] = 0.f;
-        kf[0] = key_operand<ROWB>(sk, lane, kt, 0);
-        kf[1] = key_operand<ROWB>(sk, lane, kt, 1);
+        kf[0] = key_operand<ROWB>(sk, lane, 0, 0);
+        kf[1] = key_operand<ROWB>(sk, lane, 0, 1);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            if (ks + 2 < KS) kf[(ks + 2) % 3] = key_operand<ROWB>(sk, lane, kt, ks + 2);
-            else vf[ks + 2 - KS] = value_operand<ROWB>(sv, lane, (ks + 2 - KS) / 2, 2 * vt + (ks + 2 - KS) % 2);
+            if (ks + 2 < KS) kf[(ks + 2) % 3] = key_operand<ROWB>(sk, lane, 0, ks + 2);
+            else vf[ks + 2 - KS] = value_operand<ROWB>(sv, lane, (ks + 2 - KS) / 2, (ks + 2 - KS) % 2);
             next = T::mfma32(kf[ks % 3], qf[ks], next);
 #pragma unroll
             for (int e = 16 * ks / KS; e < 16 * (ks + 1) / KS; ++e) {
@@ -175,7 +176,7 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
         }
 #pragma unroll
         for (int i = 0; i < 2 * DT; ++i) {
-            if (i + 2 < 2 * DT) vf[(i + 2) % 3] = value_operand<ROWB>(sv, lane, (i + 2) / 2, 2 * vt + i % 2);
+            if (i + 2 < 2 * DT) vf[(i + 2) % 3] = value_operand<ROWB>(sv, lane, (i + 2) / 2, i % 2);
             o[i / 2] = T::mfma32(vf[i % 3], pf[i % 2], o[i / 2]);
             if (i >= 2 * DT - 2) {
 #pragma unroll
@@ -298,16 +299,15 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
                 scores(sm_k[kb], 0, sa);
                 refer(most(sa, low));
                 for (;;) {
-                    if constexpr (NK == 2) refer(fused(sm_k[kb], 1, sb, sa, sm_v[vb], 0));
-                    else sb = sa;
+                    sb = sa;
                     if (v + 1 >= v1 || is_edge(tl.key(v + 1), there)) break;
                     const char* before = sm_v[vb];
                     advance();
                     arrive();
-                    refer(fused(sm_k[kb], 0, sa, sb, before, NK - 1));
+                    refer(fused(sm_k[kb], sa, sb, before));
                 }
                 weigh(sb, pf);
-                outputs(sm_v[vb], NK - 1, pf);
+                outputs(sm_v[vb], 0, pf);
                 advance();
             }
         } else {
@@ -351,12 +351,12 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
                 for (int i = 0; i < 2 * NK * DT; ++i) {
                     if (i + 3 < 2 * NK * DT) vf[(i + 3) % 4] = value_operand<ROWB>(sv, lane, (i + 3) % DT, (i + 3) / DT);
                     o[i % DT] = T::mfma32(vf[i % 4], pf[i / DT / 2][i / DT % 2], o[i % DT]);
-                    if (NK == 2 && i < 2 * DT) {
+                    if (i < 2 * DT) {
 #pragma unroll
                         for (int e = 16 * i / (2 * DT); e < 16 * (i + 1) / (2 * DT); ++e) {
-                            w[e] = __builtin_amdgcn_exp2f(fmaf(s[NK - 1][e], a.scale, -base));
+                            w[e] = __builtin_amdgcn_exp2f(fmaf(s[1][e], a.scale, -base));
                             sum += w[e];
-                            if (e & 1) pf[NK - 1][e / 8][e % 8 / 2] = T::pack(w[e - 1], w[e]);
+                            if (e & 1) pf[1][e / 8][e % 8 / 2] = T::pack(w[e - 1], w[e]);
                         }
                     }
                     __builtin_amdgcn_sched_barrier(0);
