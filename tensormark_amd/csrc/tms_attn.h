@@ -108,7 +108,8 @@ template <int ROWB> __device__ __forceinline__ int value_swizzle(int row) { retu
 // 16 bytes a lane from `off` of the resource to LDS at `lds` (wave-uniform) +
 // 16 * lane; zeros where the resource ends before.  Counted by vmcnt only:
 // the loop waits for it, the compiler does not know of it.  (A wait state
-// lies between m0's write and the load that reads it.)
+// lies between m0's write and the load that reads it.  m0 is reserved: the compiler
+// keeps nothing in it and takes no clobber of it, and nothing else in these kernels uses it.)
 __device__ __forceinline__ void load_lds16(u32x4 rsrc, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc) : "memory");
 }
