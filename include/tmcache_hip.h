@@ -102,7 +102,8 @@ int tms_kv_append(const tms_cache* cache, const tms_append_args* args, hipStream
  */
 typedef struct tms_attention_args {
     const void* q;            /* device, [tokens][q_heads][head_dim]; 16-byte aligned */
-    void* out;                /* device, like q, of the same dtype */
+    void* out;                /* device, like q, of the same dtype; may be q itself with q's
+                                 strides, and shares no other memory with the inputs */
     float* lse;               /* device, [tokens][q_heads] contiguous, nullable */
     int64_t q_stride[2];      /* token, head: multiples of 8 */
     int64_t out_stride[2];
@@ -124,7 +125,7 @@ int tms_paged_attention(const tms_cache* cache, const tms_attention_args* args, 
  *   out[j] = scores[j] + sum over rows that see j of exp(scale * q . k_j - lse).
  * `lse` is tms_paged_attention's, for the same q, window, sinks and scale;
  * rows with lse = -inf add nothing.  `out` has the layout of cache->scores
- * and may be the same array; every mapped position below kv_len is written,
+ * and may be the same array, but not overlap it otherwise; every mapped position below kv_len is written,
  * nothing else.  Sums are in a fixed order.  A page that two sequences share
  * may get either one's sum.
  */
@@ -178,7 +179,7 @@ int tms_kv_evict(const tms_cache* cache, const tms_evict_args* args, hipStream_t
  *      tmsample_hip.h, apply_repeat_penalty, tensormark/tmsample.h:52-63);
  *   3. the sum of the sequence's biases for an id, taken in list order, is added.
  * Ids outside [0, vocab) are left out.  `out` may be `logits` (same dtype and
- * stride).  Of params only repeat_penalty, repeat_last_n, frequency_penalty
+ * stride), but not overlap it otherwise.  Of params only repeat_penalty, repeat_last_n, frequency_penalty
  * and presence_penalty are read.
  */
 typedef struct tms_adjust_args {

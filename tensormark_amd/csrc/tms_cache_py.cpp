@@ -4,6 +4,7 @@
 // same checks in Python with ctypes took 7 to 12 us of the host besides the launch;
 // a call is 4.5 to 9 us of the host with this (a token of each of 64 sequences into
 // the cache: 11.0 us with ctypes, 4.3 with this; one session's attention: 15.0 and 11.6).
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/extension.h>
 
@@ -54,6 +55,12 @@ static void written(const Tensor& t) {
 }
 static void written(const MaybeTensor& t) {
     if (t) written(*t);
+}
+
+// An output is the input's own tensor or shares no memory with it, as far as their strides tell.
+static void want_apart(const Tensor& out, const Tensor& in) {
+    want(at::has_internal_overlap(out) != at::MemOverlap::Yes && at::get_overlap_status(out, in) != at::MemOverlapStatus::Partial,
+         "out: overlaps itself or, in part, the input");
 }
 
 // A number of Python's as 32 bits, for the library to judge; none is a smaller one by wrapping.
@@ -167,6 +174,7 @@ static std::tuple<Tensor, Tensor> paged_attention(const Tensor& q, const Tensor&
     const Tensor lse = lse_ ? *lse_ : at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
     want(out.sizes() == q.sizes(), "out: like q");
     rows(out, k, a.out_stride, "out: like q");
+    if (out_) want_apart(out, q);
     a.q = q.data_ptr();
     a.out = out.data_ptr();
     a.lse = f32_rows(lse, q, "lse: contiguous float32 [tokens, q_heads]");
@@ -200,6 +208,7 @@ static Tensor kv_add_scores(const Tensor& q, const Tensor& lse, const Tensor& k,
     const Tensor out = out_ ? *out_ : *scores;
     want(out.scalar_type() == at::kFloat && out.sizes() == scores->sizes() && out.is_contiguous() && gpu_of(out) == gpu_of(k),
          "out: like scores");
+    if (out_) want_apart(out, *scores);
     a.q = q.data_ptr();
     a.lse = f32_rows(lse, q, "lse: contiguous float32 [tokens, q_heads]");
     a.out = out.data_ptr<float>();
@@ -307,6 +316,7 @@ static Tensor adjust_logits(const Tensor& logits, const MaybeTensor& params, con
     want(out.sizes() == logits.sizes() && (out.scalar_type() == logits.scalar_type() || out.scalar_type() == at::kFloat) &&
              gpu_of(out) == device && row_contiguous(out),
          "out: like logits, of its type or float32");
+    if (out_) want_apart(out, logits);
     a.out_dtype = dtype_code(out);
     a.out_stride = R > 1 ? out.stride(0) : V;
     a.logits = logits.data_ptr();
