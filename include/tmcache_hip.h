@@ -25,6 +25,8 @@
  * in tms_kv_add_scores and tms_kv_evict (attention reads them, more slowly).
  * Lengths are taken as at most 2^29.
  *
+ * Past the limits below a call answers TMS_ERR_CAPACITY.
+ *
  * Visible positions.  A row at position p sees j <= p on mapped pages; with
  * window > 0 only j > p - window or j < sinks.
  */
@@ -40,6 +42,10 @@ extern "C" {
 #define TMS_CACHE_MAX_HEAD_DIM 256
 #define TMS_CACHE_MIN_PAGE 8
 #define TMS_CACHE_MAX_PAGE 65536
+#define TMS_CACHE_MAX_PAIRS 1048576              /* batch times kv_heads */
+#define TMS_CACHE_MAX_TOKENS 268435456
+#define TMS_APPEND_MAX_BATCH 65535
+#define TMS_SCORES_MAX_KV 4194304                /* max_kv */
 #define TMS_ATTENTION_MAX_SLOT_STRIDE 67108864   /* elements; tms_paged_attention */
 #define TMS_ATTENTION_MAX_ROWS 2097152           /* max_q times query heads a key head; where a page's stride or
                                                     slots span 2^32 bytes, batch times kv_heads times

@@ -73,7 +73,7 @@ inline int check_cache(const tms_cache* c, bool need_v, bool need_q) {
     }
     if (c->batch > 0 && (!c->tables || c->table_stride < 1 || !c->kv_len || (need_q && !c->q_start)))
         return TMS_ERR_INVALID_ARG;
-    if ((int64_t)c->batch * c->kv_heads > (1 << 20) || c->tokens > (1 << 28)) return TMS_ERR_CAPACITY;
+    if ((int64_t)c->batch * c->kv_heads > TMS_CACHE_MAX_PAIRS || c->tokens > TMS_CACHE_MAX_TOKENS) return TMS_ERR_CAPACITY;
     return TMS_OK;
 }
 

@@ -301,7 +301,7 @@ extern "C" int tms_kv_append(const tms_cache* cache, const tms_append_args* args
     for (int i = 0; i < 2; ++i)
         if (args->k_new_stride[i] < 0 || args->k_new_stride[i] % 8 || args->v_new_stride[i] < 0 || args->v_new_stride[i] % 8)
             return TMS_ERR_INVALID_ARG;
-    if (cache->batch > 65535) return TMS_ERR_CAPACITY;
+    if (cache->batch > TMS_APPEND_MAX_BATCH) return TMS_ERR_CAPACITY;
     if (cache->batch == 0 || cache->tokens == 0 || cache->max_q == 0) return TMS_OK;
     if (!args->k_new || !args->v_new || !aligned16(args->k_new) || !aligned16(args->v_new)) return TMS_ERR_INVALID_ARG;
     AppendParams a;

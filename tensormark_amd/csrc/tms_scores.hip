@@ -321,7 +321,7 @@ extern "C" int tms_kv_add_scores(const tms_cache* cache, const tms_score_args* a
         !std::isfinite(args->scale) || args->q_stride[0] < 0 || args->q_stride[0] % 8 || args->q_stride[1] < 0 ||
         args->q_stride[1] % 8 || ((uintptr_t)args->out & 15) || ((uintptr_t)args->lse & 3))
         return TMS_ERR_INVALID_ARG;
-    if (cache->max_kv > 4 * 1024 * 1024 || (int64_t)cache->max_q * (args->q_heads / cache->kv_heads) > TMS_ATTENTION_MAX_ROWS ||
+    if (cache->max_kv > TMS_SCORES_MAX_KV || (int64_t)cache->max_q * (args->q_heads / cache->kv_heads) > TMS_ATTENTION_MAX_ROWS ||
         args->q_stride[0] > TMS_SCORES_MAX_Q_STRIDE || args->q_stride[1] > TMS_SCORES_MAX_Q_STRIDE ||
         args->q_stride[1] * (args->q_heads / cache->kv_heads) > TMS_SCORES_MAX_Q_STRIDE)
         return TMS_ERR_CAPACITY;

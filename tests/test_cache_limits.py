@@ -79,3 +79,22 @@ def test_more_items_than_32_bits_count():
 
     assert call(1 << 15, 1, True) == CAPACITY and call(1 << 14, 2, True) == CAPACITY
     assert call((1 << 15) - 1, 1, True) > 0 and call(1 << 15, 1, False) >= 0
+
+
+def test_the_limits_that_the_header_names():
+    import os
+    import re
+
+    from test_cache_args import ROOT
+
+    with open(os.path.join(ROOT, "include", "tmcache_hip.h")) as f:
+        most = {k: int(v) for k, v in re.findall(r"#define (TMS_\w+_MAX_\w+) (\d+)", f.read())}
+    lib, n = cache._fns(), most["TMS_APPEND_MAX_BATCH"]
+    append = C.byref(rows_args(cache.AppendArgs))
+    assert lib.tms_kv_append(C.byref(a_cache(batch=n + 1, kv_heads=1)), append, None) == CAPACITY
+    assert lib.tms_kv_append(C.byref(a_cache(batch=n, kv_heads=1, tokens=0)), append, None) == 0
+    assert scores(c=dict(max_kv=most["TMS_SCORES_MAX_KV"] + 1)) == CAPACITY
+    assert attend(c=dict(batch=most["TMS_CACHE_MAX_PAIRS"] // 2 + 1)) == CAPACITY
+    assert attend(c=dict(tokens=most["TMS_CACHE_MAX_TOKENS"] + 1)) == CAPACITY
+    evict = C.byref(rows_args(cache.EvictArgs))
+    assert lib.tms_kv_evict(C.byref(a_cache(max_kv=most["TMS_EVICT_MAX_KV"] + 1)), evict, None) == CAPACITY
