@@ -3,6 +3,9 @@
 // group of rows sees.
 #pragma once
 
+#include <algorithm>
+#include <limits>
+
 #include "tms_cache.h"
 
 namespace tms {
@@ -171,11 +174,12 @@ template <int ROWB> __device__ __forceinline__ u32x4 value_operand(const char* s
 }
 
 // The scale of a call, split into one above 0 and what becomes of the query:
-// masked scores are -inf before the scale and stay so.
+// masked scores are -inf before the scale and stay so.  (A scale near the type's
+// largest number stays finite: a score of 0 stays 0.)
 inline void set_scale(AttnParams& a, float scale) {
     a.qand = scale == 0.f ? 0u : ~0u;
     a.qxor = scale < 0.f ? 0x80008000u : 0u;
-    a.scale = scale == 0.f ? 1.f : (scale < 0.f ? -scale : scale) * kLog2e;
+    a.scale = scale == 0.f ? 1.f : std::min((scale < 0.f ? -scale : scale) * kLog2e, std::numeric_limits<float>::max());
 }
 
 constexpr int kChunkRows = 128;   // of a workgroup of the chunk kernel

@@ -94,3 +94,19 @@ def test_a_key_that_every_row_scores_minus_infinity(q, G, D, dt):
     assert torch.all(grown[low] == 0)
     # every row's weights sum to one: (kv + rows + 32) steps of fp32, and a step of each sum so far
     assert abs(float(grown.sum()) - q * G) <= q * G * (300 + 32) * U + U * float(out[p, 0, s].double().sum())
+
+
+@pytest.mark.parametrize("scale", [3e38, -3e38, 1e-45, -1e-38])
+@pytest.mark.parametrize("q, D", [(3, 64), (50, 128), (40, 256)])
+def test_a_scale_at_the_type_s_ends(q, D, scale):
+    """Rows that score every key 0 weigh all alike, whatever the scale."""
+    bt = Batch([130], [q], H=1, G=2, D=D, dt=HF, seed=q)
+    bt.qs[:] = 0
+    out, lse, tol, ltol, weights, wtol = bt.reference(scale=1.0)
+    o, l = bt.attend(scale=scale)
+    assert np.all(np.abs(o.double().cpu().numpy() - out) <= tol) and np.all(np.abs(l.double().cpu().numpy() - lse) <= ltol)
+    zero = torch.zeros_like(bt.scores)
+    tm.kv_add_scores(bt.qs.to(DEV), l, bt.k, zero, bt.tables, bt.kv_len, bt.q_start, max_q=q, max_kv=130, scale=scale)
+    p, s = bt.where(0, np.arange(130))
+    want = weights[0]
+    assert np.all(np.abs(zero[p, 0, s].double().cpu().numpy() - want) <= 2 * wtol[0] + want * U * 10 * np.abs(lse).max() + 2 * U * want)
