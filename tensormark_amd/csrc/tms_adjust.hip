@@ -21,7 +21,7 @@ namespace tms {
 
 constexpr uint32_t kBiasHeld = 512;
 // Ids at a time: 8 KiB each of counts and biases, seven workgroups a CU (288 rows
-// of 128256 bf16: 39 us; 45 with 4096 and three workgroups).
+// of 128256 bf16, other ones each time: 46 us; 63 with 4096 and three workgroups).
 constexpr int kAdjChunk = 2048;
 
 struct AdjustParams {
@@ -266,8 +266,8 @@ extern "C" int tms_adjust_logits(const tms_adjust_args* args, hipStream_t stream
     a.mask = p.mask;
     a.mstride = p.mask_stride;
     // Chunks a workgroup: as many as leave some two rounds of the 1792 workgroups
-    // that the card holds (288 rows of 128256: 39 us with 4096 workgroups, 44 with
-    // 1024, 50 with one a chunk).
+    // that the card holds (288 rows of 128256 bf16, other ones each time: 46 us with 4096
+    // workgroups, 50 with 1024, 54 with 8192, 58 with one a chunk).
     const int chunks = (p.vocab + kAdjChunk - 1) / kAdjChunk;
     a.subs = (int)std::max<int64_t>(1, std::min<int64_t>(chunks, rows * chunks / 4096));
     const dim3 grid((chunks + a.subs - 1) / a.subs, (unsigned)rows);
