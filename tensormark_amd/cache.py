@@ -11,7 +11,8 @@ a sequence's positions, its new tokens among them; ``q_start`` (int32
 lengths themselves stay on the device and nothing is synchronised.
 
 The calls run on the tensors' device, on its current stream (or ``stream``), allocate only what they
-return and, for ``paged_attention``, a workspace, with torch's allocator.  They raise
+return (theirs is the given stream's memory; a tensor that is let go before that
+stream has run needs its ``record_stream``) and, for ``paged_attention``, a workspace, with torch's allocator.  They raise
 ValueError for tensors that do not fit and RuntimeError for what the library
 refuses; there is no fallback.  None has a backward: where autograd is on, a tensor
 that requires a gradient is refused.
