@@ -10,12 +10,12 @@ a sequence's positions, its new tokens among them; ``q_start`` (int32
 ``max_kv`` are the host's bounds on a sequence's new tokens and positions: the
 lengths themselves stay on the device and nothing is synchronised.
 
-The calls run on the tensors' device, on its current stream (or ``stream``), allocate only what they
-return (theirs is the given stream's memory; a tensor that is let go before that
-stream has run needs its ``record_stream``) and, for ``paged_attention``, a workspace, with torch's allocator.  They raise
-ValueError for tensors that do not fit and RuntimeError for what the library
-refuses; there is no fallback.  None has a backward: where autograd is on, a tensor
-that requires a gradient is refused.
+The calls run on the tensors' device, on its current stream or on ``stream`` (a
+tensor let go before that one has run needs its ``record_stream``), allocate only
+what they return and, for ``paged_attention``, a workspace, with torch's allocator.
+They raise ValueError for tensors that do not fit and RuntimeError for what the
+library refuses; there is no fallback.  None has a backward: where autograd is on, a
+tensor that requires a gradient is refused.
 
 The functions here are thin: the checks and the calls are in
 csrc/tms_cache_py.cpp, built beside the library.  The ctypes structures are the C
