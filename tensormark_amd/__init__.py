@@ -22,7 +22,16 @@ from .sampler import (  # noqa: F401
     make_history,
     make_params,
 )
+from .tree import (  # noqa: F401
+    kv_append_rotary,
+    kv_compact,
+    rotary,
+    rotary_frequencies,
+    tree_attention,
+    verify_tree,
+)
 
 __all__ = ["EXPORTS", "HISTORY_DTYPE", "Opts", "RowParams", "ROW_DTYPE", "Sampler", "load_library",
            "make_history", "make_params", "adjust_logits", "kv_add_scores", "kv_append", "kv_evict",
-           "paged_attention"]
+           "paged_attention", "kv_append_rotary", "kv_compact", "rotary", "rotary_frequencies",
+           "tree_attention", "verify_tree"]

@@ -1,5 +1,5 @@
-"""Builds libtmsample_hip.so in-tree for gfx950 with hipcc, and the cache calls'
-Python module, _cache_ops.so, beside it.
+"""Builds libtmsample_hip.so in-tree for gfx950 with hipcc, and the cache and tree
+calls' Python modules, _cache_ops.so and _tree_ops.so, beside it.
 
 Usage: python -m tensormark_amd.build   (or tensormark_amd.build.build())
 """
@@ -16,7 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtmsample_hip.so")
-SOURCES = ["tms_sample.hip", "tms_topp.hip", "tms_wide.hip", "tms_sparse.hip", "tms_rows.hip", "tms_hist.hip", "tms_chain.hip", "tms_spec.hip", "tms_debug.hip", "tms_attn.hip", "tms_attn_chunk.hip", "tms_scores.hip", "tms_kv.hip", "tms_adjust.hip", "tms_history.cpp", "tms_grammar.cpp", "tms_filter.cpp"]
+SOURCES = ["tms_sample.hip", "tms_topp.hip", "tms_wide.hip", "tms_sparse.hip", "tms_rows.hip", "tms_hist.hip", "tms_chain.hip", "tms_spec.hip", "tms_debug.hip", "tms_attn.hip", "tms_attn_chunk.hip", "tms_scores.hip", "tms_kv.hip", "tms_adjust.hip", "tms_rotary.hip", "tms_verify_tree.hip", "tms_compact.hip", "tms_history.cpp", "tms_grammar.cpp", "tms_filter.cpp"]
 
 # -ffp-contract=off keeps every a*b+c as two rounded operations, so the
 # device arithmetic matches the host checker bit for bit.  Packed-FP32 ops
@@ -50,9 +50,15 @@ BUILD_DIR = os.path.join(HERE, "_build")
 
 # The cache calls' Python side over torch tensors: a module of its own, since it
 # needs torch's headers and libraries, which libtmsample_hip.so does not.  Host
-# code alone; where there is no torch or no g++ it is left out.
+# code alone; where there is no torch or no g++ it is left out.  The tree calls' is
+# another beside it.
 OPS_SOURCE = "tms_cache_py.cpp"
 OPS = os.path.join(HERE, "_cache_ops.so")
+TREE_SOURCE = "tms_tree_py.cpp"
+
+
+def tree_ops() -> str:
+    return os.path.join(os.path.dirname(OPS), "_tree_ops.so")
 
 
 def ops_command(out: str, source: str = os.path.join(CSRC, OPS_SOURCE), optimize: str = "-O2", library: bool = True) -> list:
@@ -99,7 +105,8 @@ def _run(cmd: list, verbose: bool) -> str:
 # hold outputs or keys in registers (attention of 128-dimensional heads took
 # 775 us with 88 bytes a lane, 526 with none).
 NO_SCRATCH = ("tms_wide.hip", "tms_spec.hip", "tms_sample.hip", "tms_sparse.hip", "tms_rows.hip", "tms_topp.hip",
-              "tms_attn.hip", "tms_attn_chunk.hip", "tms_scores.hip", "tms_kv.hip", "tms_adjust.hip")
+              "tms_attn.hip", "tms_attn_chunk.hip", "tms_scores.hip", "tms_kv.hip", "tms_adjust.hip", "tms_rotary.hip",
+              "tms_verify_tree.hip", "tms_compact.hip")
 
 
 def _check_no_scratch(src: str, remarks: str) -> None:
@@ -145,15 +152,19 @@ def build(verbose: bool = False) -> str:
             _check_lds(src, rem)
     _run([hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB + ".tmp", *[j[1] for j in jobs]], verbose)
     os.replace(LIB + ".tmp", LIB)
+    modules = ((OPS, OPS_SOURCE), (tree_ops(), TREE_SOURCE))
     try:
-        command = ops_command(OPS + ".tmp")
+        commands = [ops_command(out + ".tmp", os.path.join(CSRC, src)) for out, src in modules]
     except ImportError as e:
-        print(f"built without _cache_ops.so, the Python side of the cache calls: {e}", file=sys.stderr)
-        if os.path.exists(OPS):   # (of a library that may be another)
-            os.remove(OPS)
+        print(f"built without _cache_ops.so and _tree_ops.so, the Python side of the cache and tree calls: {e}", file=sys.stderr)
+        for out, _ in modules:
+            if os.path.exists(out):   # (of a library that may be another)
+                os.remove(out)
         return LIB
-    _run(command, verbose)
-    os.replace(OPS + ".tmp", OPS)
+    with ThreadPoolExecutor(max_workers=len(modules)) as ex:
+        list(ex.map(lambda c: _run(c, verbose), commands))
+    for out, _ in modules:
+        os.replace(out + ".tmp", out)
     return LIB
 
 

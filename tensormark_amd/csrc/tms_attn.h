@@ -7,6 +7,7 @@
 #include <limits>
 
 #include "tms_cache.h"
+#include "../../include/tmtree_hip.h"
 
 namespace tms {
 
@@ -76,6 +77,7 @@ struct AttnParams {
     float* part_o;         // parts of rows, [part][rows a tile][head_dim]
     float* part_ml;        // [part][rows a tile][2]: maximum, sum
     int2* item_parts;      // rows kernel, [pairs * row_tiles]: the first share and the number of shares with a part
+    const int32_t* parents;   // trees
 };
 
 // The key tiles of `KT` keys that the rows at positions [pmin, pmax] see, as
@@ -189,5 +191,53 @@ void launch_attn_chunk(const AttnParams& a, bool bf16, dim3 grid, hipStream_t st
 __device__ __forceinline__ bool sees(int j, int p, int window, int sinks) {
     return j <= p && (window <= 0 || j > p - window || j < sinks);
 }
+
+// Trees: what the tokens of a group of rows see of the new tokens, a bit each, found by
+// climbing from node to parent in LDS (some 100 cycles a step), and their depths.  With a
+// window a node's own line is cut by it here.
+constexpr int kTreeWords = TMS_TREE_MAX_NODES / 32;
+template <int TOKENS>
+struct TreeRows {
+    int16_t up[TMS_TREE_MAX_NODES];
+    uint32_t seen[TOKENS][kTreeWords + 1];
+    int depth[TOKENS];
+
+    // Of tokens [tok0, tok0 + n) of the sequence; by all threads of the workgroup.
+    __device__ __forceinline__ void find(const AttnParams& a, const SeqView& sq, int tok0, int n) {
+        const int t = threadIdx.x;
+        for (int i = t; i < min(tok0 + n, TMS_TREE_MAX_NODES); i += blockDim.x) {
+            const int p = a.parents[sq.q0 + i];
+            up[i] = (int16_t)(p >= 0 && p < i ? p : -1);
+        }
+        __syncthreads();
+        for (int i = t; i < n; i += blockDim.x) {
+            for (int w = 0; w <= kTreeWords; ++w) seen[i][w] = 0;
+            int far = 0;
+            for (int x = up[tok0 + i]; x >= 0; x = up[x]) ++far;
+            depth[i] = far;
+            int back = 0;
+            for (int x = tok0 + i; x >= 0; x = up[x], ++back)
+                if (a.window <= 0 || back < a.window || sq.p0 + far - back < a.sinks) seen[i][x >> 5] |= 1u << (x & 31);
+        }
+        __syncthreads();
+    }
+
+    // Bit e: token `i` of these sees key t0 + e.
+    __device__ __forceinline__ uint32_t sees(const AttnParams& a, int p0, int i, int t0) const {
+        const int first = t0 - p0;   // the node that the first key is
+        uint32_t m = ~0u;
+        if (first >= 0) {
+            const int w = min(first >> 5, kTreeWords), s = first & 31;
+            m = (uint32_t)(((uint64_t)(w < kTreeWords ? seen[i][w + 1] : 0u) << 32 | seen[i][w]) >> s);
+        } else if (first > -32) {
+            m = seen[i][0] << -first | ((1u << -first) - 1);
+        }
+        if (a.window > 0) {   // the prefix ends with p0, and is hidden from `sinks` to the window
+            const int lo = max(a.sinks - t0, 0), hi = min(min(p0 + depth[i] - a.window, p0 - 1) - t0, 31);
+            if (lo <= hi) m &= ~((~0u >> (31 - (hi - lo))) << lo);
+        }
+        return m;
+    }
+};
 
 }  // namespace tms

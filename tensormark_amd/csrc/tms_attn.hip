@@ -54,12 +54,13 @@ constexpr int kItemCost = 8, kLeastShare = 4;
 // same) and what it takes besides, as tiles.
 __device__ __forceinline__ int item_length(const AttnParams& a, int tiles) { return max(tiles, 1) + kItemCost; }
 
+template <bool TREE>
 __device__ __forceinline__ int item_tiles(const AttnParams& a, int combo) {
     const int b = combo / a.row_tiles, tile = combo - b * a.row_tiles;
     const SeqView sq = seq_view(a.c, b);
     const int G = a.group, rows = sq.n * G, r0 = tile * kShareRows;
     if (r0 >= rows) return 0;
-    return item_length(a, TileList<32>(a.window, a.sinks, sq.p0 + r0 / G, sq.p0 + (min(r0 + kShareRows, rows) - 1) / G, sq.len).n);
+    return item_length(a, TileList<32>(a.window, a.sinks, TREE ? sq.p0 : sq.p0 + r0 / G, sq.p0 + (min(r0 + kShareRows, rows) - 1) / G, sq.len).n);
 }
 
 __device__ __forceinline__ int64_t share_of(const AttnParams& a, int64_t total, int shares) {
@@ -76,7 +77,7 @@ __device__ __forceinline__ void write_row(const AttnParams& a, const SeqView& sq
         (u32x2){T::pack(o[0] * inv, o[1] * inv), T::pack(o[2] * inv, o[3] * inv)};
 }
 
-template <typename T, int ROWB, int KS, int DT, int NW>
+template <typename T, int ROWB, int KS, int DT, int NW, bool TREE>
 __global__ __launch_bounds__(64 * NW, ROWB > 256 ? 1 : 2) void attn_rows_kernel(AttnParams a) {
     constexpr int RM = kShareRows, KT = 32, NL = KT * ROWB / 1024, RPI = 1024 / ROWB, PAD = 33;
     // LDS: the waves' pieces, and at an item's end their outputs, maxima and sums.
@@ -84,6 +85,7 @@ __global__ __launch_bounds__(64 * NW, ROWB > 256 ? 1 : 2) void attn_rows_kernel(
     constexpr int MERGE = NW * DT * 32 * PAD * 4, ML = NW * 32 * 2 * 4;
     __shared__ __attribute__((aligned(128))) char sm[MERGE + ML > RING ? MERGE + ML : RING];
     float* const sm_ml = (float*)(sm + MERGE);   // [wave][row][maximum, sum]
+    __shared__ std::conditional_t<TREE, TreeRows<RM>, char> sm_tree;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int n32 = lane & 31, hh = lane >> 5;
     const int H = a.c.kv_heads, G = a.group, D = a.c.head_dim;
@@ -98,7 +100,7 @@ __global__ __launch_bounds__(64 * NW, ROWB > 256 ? 1 : 2) void attn_rows_kernel(
         int64_t* const wsum = (int64_t*)sm;   // [NW], then where the share starts
         const int per = (combos + 64 * NW - 1) / (64 * NW), c0 = min(t * per, combos), c1 = min(c0 + per, combos);
         int64_t mine = 0;
-        for (int c = c0; c < c1; ++c) mine += item_tiles(a, c);
+        for (int c = c0; c < c1; ++c) mine += item_tiles<TREE>(a, c);
         int64_t upto = mine;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -118,7 +120,7 @@ __global__ __launch_bounds__(64 * NW, ROWB > 256 ? 1 : 2) void attn_rows_kernel(
         if (x >= end) return;
         if (x >= before * H && x < (before + mine) * H)
             for (int c = c0;; ++c) {
-                const int n = item_tiles(a, c);
+                const int n = item_tiles<TREE>(a, c);
                 if (x < (before + n) * H) {
                     wsum[NW] = c;
                     wsum[NW + 1] = before * H;
@@ -154,7 +156,9 @@ __global__ __launch_bounds__(64 * NW, ROWB > 256 ? 1 : 2) void attn_rows_kernel(
             continue;
         }
         const int nr = min(RM, rows - r0);
-        const int pfirst = sq.p0 + r0 / G, plast = sq.p0 + (r0 + nr - 1) / G;
+        // Positions of the rows.  A tree's row sees no key past the prefix but its own line,
+        // and stands at p0 or behind.
+        const int pfirst = TREE ? sq.p0 : sq.p0 + r0 / G, plast = sq.p0 + (r0 + nr - 1) / G, pall = TREE ? sq.p0 - 1 : pfirst;
         const TileList<KT> tl(a.window, a.sinks, pfirst, plast, sq.len);
         const int n = max(tl.n, 1), axis = item_length(a, tl.n);
         int h = blockIdx.x - combo * H, k0 = 0, k1 = n;
@@ -178,6 +182,9 @@ __global__ __launch_bounds__(64 * NW, ROWB > 256 ? 1 : 2) void attn_rows_kernel(
         const bool in = r < rows;
         const int tok = in ? r / G : 0, hd = in ? r - tok * G : 0;
         const int pos = in ? sq.p0 + tok : -1;
+        if constexpr (TREE) {   // (a share of the prefix alone needs none, but for a window)
+            if (a.window > 0 || (k0 < kend && tl.key(kend - 1) + KT > sq.p0)) sm_tree.find(a, sq, r0 / G, (r0 + nr - 1) / G - r0 / G + 1);
+        }
         u32x4 qf[KS];
         {
             const char* src = a.q + (int64_t)(sq.q0 + tok) * a.qt + (int64_t)(h * G + hd) * a.qh;
@@ -251,13 +258,15 @@ __global__ __launch_bounds__(64 * NW, ROWB > 256 ? 1 : 2) void attn_rows_kernel(
                 load(v + NW, kbase, a.c.kp, kslot, koff, lds0);
                 if (v + 2 * NW < kend) entries(v + 2 * NW);
             }
-            const bool edge = now != 15 || t0 + KT > sq.len || t0 + KT - 1 > pfirst ||
+            const bool edge = now != 15 || t0 + KT > sq.len || t0 + KT - 1 > pall ||
                               (a.window > 0 && t0 <= plast - a.window && t0 + KT > a.sinks);
             if (edge) {
+                uint32_t seen = 0;
+                if constexpr (TREE) seen = in ? sm_tree.sees(a, sq.p0, tok - r0 / G, t0) : 0;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int j = t0 + 8 * (i / 4) + 4 * hh + (i & 3);
-                    const bool on = (now >> (i / 4) & 1) && j < sq.len && sees(j, pos, a.window, a.sinks);
+                    const bool on = (now >> (i / 4) & 1) && j < sq.len && (TREE ? seen >> (j - t0) & 1 : sees(j, pos, a.window, a.sinks));
                     s[i] = on ? s[i] : -__builtin_huge_valf();
                 }
             }
@@ -522,14 +531,14 @@ static int check_attention(const tms_cache* c, const tms_attention_args* a) {
     return TMS_OK;
 }
 
-static AttnPlan plan_attention(const tms_cache* c, const tms_attention_args* a) {
+static AttnPlan plan_attention(const tms_cache* c, const tms_attention_args* a, bool tree) {
     AttnPlan p;
     const int rows = p.rows = min(c->max_q, c->tokens) * (a->q_heads / c->kv_heads);
     p.chunk = rows > kShareRows && short_strides(c, c->k_stride) && short_strides(c, c->v_stride);
     p.rm = p.chunk ? kChunkRows : kShareRows;
     p.row_tiles = (rows + p.rm - 1) / p.rm;
     int64_t keys = min(c->max_kv, kMaxLen);
-    if (a->window > 0) keys = std::min<int64_t>(keys, (int64_t)a->window + p.rm + a->sinks + 128);
+    if (a->window > 0) keys = std::min<int64_t>(keys, (int64_t)a->window + (tree ? c->max_q : p.rm) + a->sinks + 128);
     const int64_t items = (int64_t)c->batch * c->kv_heads * p.row_tiles;
     int64_t parts;
     p.fits = p.chunk || items <= INT32_MAX;
@@ -560,15 +569,15 @@ static AttnPlan plan_attention(const tms_cache* c, const tms_attention_args* a) 
     return p;
 }
 
-template <typename T, int ROWB, int KS, int DT>
+template <typename T, int ROWB, int KS, int DT, bool TREE>
 static void launch_rows(const AttnPlan& p, const AttnParams& a, hipStream_t stream) {
     if constexpr (ROWB <= 256) {
         if (p.waves == 8) {
-            hipLaunchKernelGGL((attn_rows_kernel<T, ROWB, KS, DT, 8>), dim3(p.shares), dim3(512), 0, stream, a);
+            hipLaunchKernelGGL((attn_rows_kernel<T, ROWB, KS, DT, 8, TREE>), dim3(p.shares), dim3(512), 0, stream, a);
             return;
         }
     }
-    hipLaunchKernelGGL((attn_rows_kernel<T, ROWB, KS, DT, 4>), dim3(p.shares), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((attn_rows_kernel<T, ROWB, KS, DT, 4, TREE>), dim3(p.shares), dim3(256), 0, stream, a);
 }
 
 template <typename T, int LPR>
@@ -580,40 +589,37 @@ static void launch_join(const AttnPlan& p, const AttnParams& a, int pairs, hipSt
                        p.rm, sub);
 }
 
-template <typename T>
+template <typename T, bool TREE>
 static void launch_attention(const AttnPlan& p, const AttnParams& a, hipStream_t stream) {
     const int D = a.c.head_dim, pairs = a.c.batch * a.c.kv_heads;
     if (p.chunk) launch_attn_chunk(a, std::is_same<T, Bf16>::value, dim3(pairs, p.row_tiles, p.splits), stream);
-    else if (D <= 64) launch_rows<T, 128, 4, 2>(p, a, stream);
-    else if (D <= 96) launch_rows<T, 256, 6, 3>(p, a, stream);
-    else if (D <= 128) launch_rows<T, 256, 8, 4>(p, a, stream);
-    else launch_rows<T, 512, 16, 8>(p, a, stream);
+    else if (D <= 64) launch_rows<T, 128, 4, 2, TREE>(p, a, stream);
+    else if (D <= 96) launch_rows<T, 256, 6, 3, TREE>(p, a, stream);
+    else if (D <= 128) launch_rows<T, 256, 8, 4, TREE>(p, a, stream);
+    else launch_rows<T, 512, 16, 8, TREE>(p, a, stream);
     if (!p.join) return;
     if (D <= 64) launch_join<T, 16>(p, a, pairs, stream);
     else if (D <= 128) launch_join<T, 32>(p, a, pairs, stream);
     else launch_join<T, 64>(p, a, pairs, stream);
 }
 
-}  // namespace tms
-
-extern "C" int64_t tms_paged_attention_workspace(const tms_cache* cache, const tms_attention_args* args) {
-    const int rc = tms::check_attention(cache, args);
+static int64_t attention_workspace(const tms_cache* cache, const tms_attention_args* args, bool tree) {
+    const int rc = check_attention(cache, args);
     if (rc != TMS_OK) return rc;
-    const tms::AttnPlan p = tms::plan_attention(cache, args);
+    if (tree && cache->max_q > TMS_TREE_MAX_NODES) return TMS_ERR_CAPACITY;
+    const AttnPlan p = plan_attention(cache, args, tree);
     if (!p.fits) return TMS_ERR_CAPACITY;
     return (int64_t)(p.o_bytes + p.ml_bytes + p.item_bytes);
 }
 
-extern "C" int tms_paged_attention(const tms_cache* cache, const tms_attention_args* args, hipStream_t stream) {
-    using namespace tms;
-    const int rc = check_attention(cache, args);
-    if (rc != TMS_OK) return rc;
+template <bool TREE>
+static int attention(const tms_cache* cache, const tms_attention_args* args, const int32_t* parents, hipStream_t stream) {
+    const int64_t need = attention_workspace(cache, args, TREE);
+    if (need < 0) return (int)need;
     if (cache->batch == 0 || cache->tokens == 0 || cache->max_q == 0) return TMS_OK;
-    const AttnPlan p = plan_attention(cache, args);
-    if (!p.fits) return TMS_ERR_CAPACITY;
-    if (args->workspace_bytes < p.o_bytes + p.ml_bytes + p.item_bytes ||
-        (p.join && (!args->workspace || !aligned16(args->workspace))))
-        return TMS_ERR_INVALID_ARG;
+    if (TREE && (!parents || ((uintptr_t)parents & 3))) return TMS_ERR_INVALID_ARG;
+    const AttnPlan p = plan_attention(cache, args, TREE);
+    if (args->workspace_bytes < (size_t)need || (p.join && (!args->workspace || !aligned16(args->workspace)))) return TMS_ERR_INVALID_ARG;
     AttnParams a;
     a.c = view_of(cache);
     a.q = (const char*)args->q;
@@ -635,7 +641,26 @@ extern "C" int tms_paged_attention(const tms_cache* cache, const tms_attention_a
     a.part_o = (float*)args->workspace;
     a.part_ml = (float*)((char*)args->workspace + p.o_bytes);
     a.item_parts = p.chunk ? nullptr : (int2*)((char*)args->workspace + p.o_bytes + p.ml_bytes);
-    if (cache->dtype == TMS_DTYPE_BF16) launch_attention<Bf16>(p, a, stream);
-    else launch_attention<F16>(p, a, stream);
+    a.parents = parents;
+    if (cache->dtype == TMS_DTYPE_BF16) launch_attention<Bf16, TREE>(p, a, stream);
+    else launch_attention<F16, TREE>(p, a, stream);
     return hipGetLastError() == hipSuccess ? TMS_OK : TMS_ERR_HIP;
+}
+
+}  // namespace tms
+
+extern "C" int64_t tms_paged_attention_workspace(const tms_cache* cache, const tms_attention_args* args) {
+    return tms::attention_workspace(cache, args, false);
+}
+
+extern "C" int tms_paged_attention(const tms_cache* cache, const tms_attention_args* args, hipStream_t stream) {
+    return tms::attention<false>(cache, args, nullptr, stream);
+}
+
+extern "C" int64_t tms_tree_attention_workspace(const tms_cache* cache, const tms_attention_args* args) {
+    return tms::attention_workspace(cache, args, true);
+}
+
+extern "C" int tms_tree_attention(const tms_cache* cache, const tms_attention_args* args, const int32_t* parents, hipStream_t stream) {
+    return tms::attention<true>(cache, args, parents, stream);
 }

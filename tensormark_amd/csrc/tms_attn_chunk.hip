@@ -18,7 +18,7 @@
 
 namespace tms {
 
-template <typename T, int ROWB, int KS, int DT, int NK>
+template <typename T, int ROWB, int KS, int DT, int NK, bool TREE>
 __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(AttnParams a) {
     constexpr int KT = 32 * NK, RM = kChunkRows;
     constexpr int C = ROWB / 16, RPI = 64 / C, NI = KT / (4 * RPI);   // pieces a row; rows a load; loads a wave
@@ -28,6 +28,7 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
     constexpr int NV = FUSED ? 3 : 2;   // value buffers
     __shared__ __attribute__((aligned(128))) char sm_k[2][KT * ROWB];
     __shared__ __attribute__((aligned(128))) char sm_v[NV][KT * ROWB];
+    __shared__ std::conditional_t<TREE, TreeRows<RM>, char> sm_tree;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n32 = lane & 31, hh = lane >> 5;
     const int pair = blockIdx.x, tile = a.row_tiles - 1 - blockIdx.y, split = blockIdx.z;
@@ -36,16 +37,21 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
     const int G = a.group, rows = sq.n * G, r0 = tile * RM;
     if (r0 >= rows) return;
     const int D = a.c.head_dim;
-    const int gfirst = sq.p0 + r0 / G, glast = sq.p0 + (min(r0 + RM, rows) - 1) / G;   // positions of the workgroup's rows
+    // Positions of the workgroup's rows.  A tree's row sees no key past the prefix but its
+    // own line, and stands at p0 or behind.
+    const int gfirst = TREE ? sq.p0 : sq.p0 + r0 / G, glast = sq.p0 + (min(r0 + RM, rows) - 1) / G, gall = TREE ? sq.p0 - 1 : gfirst;
     const TileList<KT> tl(a.window, a.sinks, gfirst, glast, sq.len);
     const int v0 = split * a.split_tiles, v1 = a.splits == split + 1 ? tl.n : min(tl.n, v0 + a.split_tiles);
 
     // The wave's rows, and the lane's: its query and its position.
     const int w0 = r0 + wave * 32, r = w0 + n32;
     const bool in = r < rows;
-    const int pfirst = sq.p0 + w0 / G, plast = w0 < rows ? sq.p0 + (min(w0 + 32, rows) - 1) / G : -1;
+    const int pfirst = TREE ? sq.p0 : sq.p0 + w0 / G, plast = w0 < rows ? sq.p0 + (min(w0 + 32, rows) - 1) / G : -1;
     const int tok = in ? r / G : 0, hd = in ? r - tok * G : 0;
     const int pos = in ? sq.p0 + tok : -1;
+    if constexpr (TREE) {   // (a split of the prefix alone needs none, but for a window)
+        if (a.window > 0 || (v0 < v1 && tl.key(v1 - 1) + KT > sq.p0)) sm_tree.find(a, sq, r0 / G, glast - sq.p0 - r0 / G + 1);
+    }
     u32x4 qf[KS];
     {
         const char* src = a.q + (int64_t)(sq.q0 + tok) * a.qt + (int64_t)(h * G + hd) * a.qh;
@@ -209,10 +215,13 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
 #pragma unroll
         for (int kt = 0; kt < NK; ++kt) {
             scores(sk, kt, s[kt]);
+            uint32_t seen = 0;
+            if constexpr (TREE) seen = in ? sm_tree.sees(a, sq.p0, tok - r0 / G, t0 + 32 * kt) : 0;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int j = t0 + 32 * kt + 8 * (i / 4) + 4 * hh + (i & 3);
-                const bool on = (there >> (4 * kt + i / 4) & 1) && j < sq.len && sees(j, pos, a.window, a.sinks);
+                const bool on = (there >> (4 * kt + i / 4) & 1) && j < sq.len &&
+                                (TREE ? seen >> (j - t0 - 32 * kt) & 1 : sees(j, pos, a.window, a.sinks));
                 s[kt][i] = on ? s[kt][i] : low;
             }
             top = most(s[kt], top);
@@ -287,7 +296,7 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
         vb = vb == NV - 1 ? 0 : vb + 1;
     };
     auto is_edge = [&](int t0, uint32_t bits) {
-        return bits != ALL || t0 + KT > sq.len || t0 + KT - 1 > gfirst || (a.window > 0 && t0 <= glast - a.window && t0 + KT > a.sinks);
+        return bits != ALL || t0 + KT > sq.len || t0 + KT - 1 > gall || (a.window > 0 && t0 <= glast - a.window && t0 + KT > a.sinks);
     };
     while (v < v1) {
         // Tiles that every row sees all of.
@@ -406,18 +415,24 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
         }
 }
 
-template <typename T>
+template <typename T, bool TREE>
 static void launch_chunk_type(const AttnParams& a, dim3 grid, hipStream_t stream) {
     const int D = a.c.head_dim;
-    if (D <= 64) hipLaunchKernelGGL((attn_chunk_kernel<T, 128, 4, 2, 2>), grid, dim3(256), 0, stream, a);
-    else if (D <= 96) hipLaunchKernelGGL((attn_chunk_kernel<T, 256, 6, 3, 2>), grid, dim3(256), 0, stream, a);
-    else if (D <= 128) hipLaunchKernelGGL((attn_chunk_kernel<T, 256, 8, 4, 2>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((attn_chunk_kernel<T, 512, 16, 8, 1>), grid, dim3(256), 0, stream, a);
+    if (D <= 64) hipLaunchKernelGGL((attn_chunk_kernel<T, 128, 4, 2, 2, TREE>), grid, dim3(256), 0, stream, a);
+    else if (D <= 96) hipLaunchKernelGGL((attn_chunk_kernel<T, 256, 6, 3, 2, TREE>), grid, dim3(256), 0, stream, a);
+    else if (D <= 128) hipLaunchKernelGGL((attn_chunk_kernel<T, 256, 8, 4, 2, TREE>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((attn_chunk_kernel<T, 512, 16, 8, 1, TREE>), grid, dim3(256), 0, stream, a);
+}
+
+template <bool TREE>
+static void launch_chunk(const AttnParams& a, bool bf16, dim3 grid, hipStream_t stream) {
+    if (bf16) launch_chunk_type<Bf16, TREE>(a, grid, stream);
+    else launch_chunk_type<F16, TREE>(a, grid, stream);
 }
 
 void launch_attn_chunk(const AttnParams& a, bool bf16, dim3 grid, hipStream_t stream) {
-    if (bf16) launch_chunk_type<Bf16>(a, grid, stream);
-    else launch_chunk_type<F16>(a, grid, stream);
+    if (a.parents) launch_chunk<true>(a, bf16, grid, stream);
+    else launch_chunk<false>(a, bf16, grid, stream);
 }
 
 }  // namespace tms

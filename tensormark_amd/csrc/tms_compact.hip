@@ -1,0 +1,175 @@
+// tms_compact.hip -- chosen entries of each sequence of the paged cache moved to the
+// front (tms_kv_compact): the accepted path of a tree of drafts, a session cut to its first
+// and last positions, a copy on other pages.
+//
+// Bound by memory, and by latency (list, page, data, one after another) for a tree's path.
+#include <algorithm>
+
+#include "tms_cache.h"
+#include "../../include/tmtree_hip.h"
+
+namespace tms {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+struct CompactParams {
+    CacheView c;
+    const int32_t* kept;
+    int64_t kstride;
+    const int32_t* n_kept;
+    const int32_t* dst;      // null: in place
+    int64_t dstride;
+    int32_t* new_len;
+    int max_kept;
+    int hv;                  // 16-byte pieces of a head's row
+    int columns, width;      // of a key's or value's row; pieces of a column
+    bool apart;              // in place: keys and values by different workgroups
+};
+
+// The entries of a sequence from `base` on, `n` of them (32 bits hold every sum below:
+// lengths are at most 2^29, a span of q_start too).
+struct CompactSeq {
+    int base, n, len;
+};
+
+__device__ __forceinline__ CompactSeq compact_seq(const CompactParams& a, int b) {
+    CompactSeq s;
+    const int64_t cap = a.c.tstride << a.c.shift;
+    const int L = min(max(a.c.kv_len[b], 0), kMaxLen);
+    s.len = (int)(cap < L ? cap : L);
+    int64_t span = L;
+    if (a.c.q_start) span = min(max((int64_t)a.c.q_start[b + 1] - a.c.q_start[b], (int64_t)0), (int64_t)kMaxLen);
+    s.base = L - (int)span;
+    s.n = min(max(a.n_kept[b], 0), a.max_kept);
+    if (!a.dst) s.n = min(s.n, (int)span);
+    return s;
+}
+
+// Page and slot of entry i of the list, -1 where it is not moved.
+__device__ __forceinline__ void compact_from(const CompactParams& a, const CompactSeq& s, const int32_t* row, int i, int kept, int& page, int& slot) {
+    const int j = s.base + kept;
+    page = (unsigned)kept < (unsigned)kMaxLen && (a.dst || kept > i) ? page_of(a.c, row, j, s.len) : -1;   // (kept == i stays)
+    slot = j & a.c.smask;
+}
+
+__device__ __forceinline__ void compact_to(const CompactParams& a, const int32_t* row, int64_t stride, int j, int& page, int& slot) {
+    const bool in = j >= 0 && (j >> a.c.shift) < stride;
+    const int p = row[in ? j >> a.c.shift : 0];
+    page = in && (unsigned)p < (unsigned)a.c.pages ? p : -1;
+    slot = j & a.c.smask;
+}
+
+// To other pages: a thread moves 16 bytes of a key and of a value.
+__global__ __launch_bounds__(256) void compact_copy_kernel(CompactParams a) {
+    const int b = blockIdx.x / a.c.kv_heads, h = blockIdx.x - b * a.c.kv_heads;
+    const CompactSeq s = compact_seq(a, b);
+    if (a.new_len && h == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.new_len[b] = max(s.base + s.n, 0);
+    const int32_t* row = a.c.tables + (int64_t)b * a.c.tstride;
+    const int32_t* dst = a.dst + (int64_t)b * a.dstride;
+    const int32_t* kept = a.kept + (int64_t)b * a.kstride;
+    const int64_t all = (int64_t)s.n * a.hv;
+    for (int64_t x = (int64_t)blockIdx.y * 256 + threadIdx.x; x < all; x += (int64_t)gridDim.y * 256) {
+        const int i = (int)(x / a.hv), d = (int)(x - (int64_t)i * a.hv);
+        int from, to, s0, s1;
+        compact_from(a, s, row, i, kept[i], from, s0);
+        compact_to(a, dst, a.dstride, s.base + i, to, s1);
+        if (from < 0 || to < 0) continue;
+        const uint4 kx = *(const uint4*)(a.c.k + from * a.c.kp + h * a.c.kh + s0 * a.c.ks + 16 * d);
+        const uint4 vx = *(const uint4*)(a.c.v + from * a.c.vp + h * a.c.vh + s0 * a.c.vs + 16 * d);
+        *(uint4*)(a.c.k + to * a.c.kp + h * a.c.kh + s1 * a.c.ks + 16 * d) = kx;
+        *(uint4*)(a.c.v + to * a.c.vp + h * a.c.vh + s1 * a.c.vs + 16 * d) = vx;
+        if (d == 0 && a.c.scores)
+            a.c.scores[(((int64_t)to * a.c.kv_heads + h) << a.c.shift) + s1] = a.c.scores[(((int64_t)from * a.c.kv_heads + h) << a.c.shift) + s0];
+    }
+}
+
+// In place: entry i's place is some earlier entry's source or nobody's, never a later one's
+// (those have kept > i), so a list may be gone through from its start: a step's entries are
+// read, and once all of the workgroup's are in, written.  Only a step's own entries can meet;
+// rows are independent by head and by 16 bytes, so long lists are spread over
+// workgroups by those.
+template <int NT, int UN>
+__global__ __launch_bounds__(NT) void compact_place_kernel(CompactParams a) {
+    const int b = blockIdx.x / a.c.kv_heads, h = blockIdx.x - b * a.c.kv_heads;
+    const CompactSeq s = compact_seq(a, b);
+    const int t = threadIdx.x;
+    const int part = blockIdx.y, column = part % a.columns;
+    if (a.new_len && h == 0 && part == 0 && t == 0) a.new_len[b] = max(s.base + s.n, 0);
+    const int32_t* row = a.c.tables + (int64_t)b * a.c.tstride;
+    const int32_t* kept = a.kept + (int64_t)b * a.kstride;
+    // The thread's piece: of a key or a value, and which of a step's entries.
+    const int wide = min(a.width, a.hv - column * a.width), pieces = a.apart ? wide : 2 * wide;
+    const int entries = NT / pieces, e0 = t / pieces, p = t - e0 * pieces;
+    const bool value = a.apart ? part >= a.columns : p >= wide;
+    const int d = column * a.width + (p >= wide ? p - wide : p);
+    const bool score = a.c.scores && !value && d == 0;
+    char* const pool = (value ? a.c.v + h * a.c.vh : a.c.k + h * a.c.kh) + 16 * d;
+    const int64_t pstride = value ? a.c.vp : a.c.kp, sstride = value ? a.c.vs : a.c.ks;
+    for (int i0 = 0; i0 < s.n; i0 += entries * UN) {
+        u32x4 x[UN];
+        float sc[UN];
+        int from[UN], to[UN], s0[UN], s1[UN];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const int i = i0 + u * entries + e0, at = min(i, s.n - 1);
+            compact_from(a, s, row, at, kept[at], from[u], s0[u]);
+            compact_to(a, row, a.c.tstride, s.base + at, to[u], s1[u]);
+            if (e0 >= entries || i >= s.n || to[u] < 0) from[u] = -1;
+        }
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+            if (from[u] >= 0) {
+                x[u] = *(const u32x4*)(pool + from[u] * pstride + s0[u] * sstride);
+                if (score) sc[u] = a.c.scores[(((int64_t)from[u] * a.c.kv_heads + h) << a.c.shift) + s0[u]];
+            }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // read, by every wave, before any writes
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+            if (from[u] >= 0) {
+                *(u32x4*)(pool + to[u] * pstride + s1[u] * sstride) = x[u];
+                if (score) a.c.scores[(((int64_t)to[u] * a.c.kv_heads + h) << a.c.shift) + s1[u]] = sc[u];
+            }
+    }
+}
+
+}  // namespace tms
+
+extern "C" int tms_kv_compact(const tms_cache* cache, const tms_compact_args* args, hipStream_t stream) {
+    using namespace tms;
+    const int rc = check_cache(cache, true, false);
+    if (rc != TMS_OK) return rc;
+    if (!args || args->reserved != 0 || args->max_kept < 0) return TMS_ERR_INVALID_ARG;
+    if (args->max_kept > TMS_COMPACT_MAX_KEPT) return TMS_ERR_CAPACITY;
+    if (cache->batch == 0) return TMS_OK;
+    if (!args->n_kept || (args->max_kept > 0 && !args->kept) || args->kept_stride < args->max_kept) return TMS_ERR_INVALID_ARG;
+    if (args->dst_tables && args->dst_table_stride < 1) return TMS_ERR_INVALID_ARG;
+    if (args->new_len && (args->new_len == cache->kv_len || args->new_len == args->n_kept || args->new_len == args->kept))
+        return TMS_ERR_INVALID_ARG;
+    CompactParams a{};
+    a.c = view_of(cache);
+    a.kept = args->kept;
+    a.kstride = args->kept_stride;
+    a.n_kept = args->n_kept;
+    a.dst = args->dst_tables;
+    a.dstride = args->dst_table_stride;
+    a.new_len = args->new_len;
+    a.max_kept = args->max_kept;
+    a.hv = cache->head_dim / 8;
+    const int pairs = cache->batch * cache->kv_heads;
+    if (a.dst) {
+        const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>(((int64_t)a.max_kept * a.hv + 255) / 256, 65535));
+        hipLaunchKernelGGL(compact_copy_kernel, dim3(pairs, (unsigned)blocks), dim3(256), 0, stream, a);
+    } else if (a.max_kept <= 64) {
+        a.columns = 1;
+        a.width = a.hv;
+        a.apart = false;
+        hipLaunchKernelGGL((compact_place_kernel<256, 1>), dim3(pairs, 1), dim3(256), 0, stream, a);
+    } else {
+        a.width = std::min(a.hv, 8);
+        a.columns = (a.hv + a.width - 1) / a.width;
+        a.apart = true;
+        hipLaunchKernelGGL((compact_place_kernel<1024, 4>), dim3(pairs, 2 * a.columns), dim3(1024), 0, stream, a);
+    }
+    return hipGetLastError() == hipSuccess ? TMS_OK : TMS_ERR_HIP;
+}

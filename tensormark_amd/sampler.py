@@ -98,6 +98,14 @@ EXPORTS = (
     "tms_kv_add_scores",
     "tms_kv_evict",
     "tms_adjust_logits",
+    "tms_rotary",
+    "tms_kv_append_rotary",
+    "tms_tree_attention_workspace",
+    "tms_tree_attention",
+    "tms_verify_tree_workspace",
+    "tms_verify_tree",
+    "tms_debug_verify_polls",
+    "tms_kv_compact",
 )
 
 
