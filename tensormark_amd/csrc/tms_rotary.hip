@@ -29,12 +29,14 @@ struct TurnParams {
     float scale;
     int tokens, q_heads, heads;   // heads: keys too
     int head_dim, rotary_dim;
-    int groups;               // a thread takes every groups-th head
-    int units;                // of a head: turned ones first, then the copied
-    int turned;
+    int groups;               // a thread that turns takes every groups-th head
+    int turned, ends;         // units of a head that turn, and that are copied
+    int copies;               // threads of a token that copy
+    int turn_blocks;          // of a sequence
 };
 
 typedef uint16_t u16;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 struct TurnF32 {
     typedef float elem;
     static constexpr int kPiece = 4;   // values in 16 bytes
@@ -82,16 +84,17 @@ template <typename T, bool PAIRS, int E, bool APPEND>
 __global__ __launch_bounds__(256) void turn_kernel(TurnParams a) {
     typedef typename T::elem elem;
     constexpr int NP = PAIRS && E == 1 ? 2 : E;          // values in a turned unit's piece
-    constexpr int ANGLES = PAIRS ? NP / 2 : E, AHEAD = 4;   // heads whose loads are in flight
+    constexpr int ANGLES = PAIRS ? NP / 2 : E, AHEAD = PAIRS ? 4 : 2;   // heads whose loads are in flight
     typedef elem Piece __attribute__((ext_vector_type(NP), aligned(E == 1 ? sizeof(elem) : 16)));
     typedef elem Copy __attribute__((ext_vector_type(E), aligned(E == 1 ? sizeof(elem) : 16)));
-    const int hv = a.head_dim / 8, per = a.groups * a.units + (APPEND ? a.c.kv_heads * hv : 0);
+    // The last blocks of a sequence copy: values, and the heads' ends that do not turn.
+    const bool copies = blockIdx.x >= (unsigned)a.turn_blocks;
     const int b = APPEND ? blockIdx.y : 0;
     SeqView sq;
     if constexpr (APPEND) sq = seq_view(a.c, b);
     else sq = SeqView{0, a.tokens, 0, 0};
-    const int32_t* row = APPEND ? a.c.tables + (int64_t)b * a.c.tstride : nullptr;
-    const int64_t start = (int64_t)blockIdx.x * 256, tok0 = start / per;
+    const int per = copies ? a.copies : a.groups * a.turned;   // a token's threads
+    const int64_t start = (int64_t)(blockIdx.x - (copies ? a.turn_blocks : 0)) * 256, tok0 = start / per;
     const int at = (int)(start - tok0 * per) + (int)threadIdx.x, more = at / per, w = at - more * per;
     const int64_t i64 = tok0 + more;
     if (i64 >= sq.n) return;
@@ -99,18 +102,9 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnParams a) {
     const int64_t tok = sq.q0 + i;
     int page = -1, slot = 0;
     if constexpr (APPEND) {
-        page = page_of(a.c, row, sq.p0 + i, sq.len);
+        page = page_of(a.c, a.c.tables + (int64_t)b * a.c.tstride, sq.p0 + i, sq.len);
         slot = (sq.p0 + i) & a.c.smask;
-        if (w >= a.groups * a.units) {   // 16 bytes of a value
-            const int p = w - a.groups * a.units, h = p / hv, d = p - h * hv;
-            const uint4 y = *(const uint4*)(a.v + tok * a.vt + h * a.vh + 16 * d);
-            if (page < 0) return;
-            *(uint4*)(a.c.v + (int64_t)page * a.c.vp + h * a.c.vh + (int64_t)slot * a.c.vs + 16 * d) = y;
-            if (d == 0 && a.c.scores) a.c.scores[(((int64_t)page * a.c.kv_heads + h) << a.c.shift) + slot] = 0.f;
-            return;
-        }
     }
-    const int g = w / a.units, u = w - g * a.units;
     auto source = [&](int h) {
         return APPEND && h >= a.q_heads ? a.k + tok * a.kt + (h - a.q_heads) * a.kh : a.x + tok * a.xt + h * a.xh;
     };
@@ -120,19 +114,21 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnParams a) {
     };
     auto is = [&](int h) { return h < a.heads && (!APPEND || h < a.q_heads || page >= 0); };
 
-    if (u >= a.turned) {
-        const int at_e = a.rotary_dim + (u - a.turned) * E;
-        for (int h0 = g; h0 < a.heads; h0 += AHEAD * a.groups) {
-            Copy y[AHEAD];
-#pragma unroll
-            for (int n = 0; n < AHEAD; ++n)
-                if (is(h0 + n * a.groups)) y[n] = *(const Copy*)(source(h0 + n * a.groups) + at_e * sizeof(elem));
-#pragma unroll
-            for (int n = 0; n < AHEAD; ++n)
-                if (is(h0 + n * a.groups)) *(Copy*)(target(h0 + n * a.groups) + at_e * sizeof(elem)) = y[n];
+    if (copies) {
+        const int ends = a.heads * a.ends;
+        if (w < ends) {
+            const int h = w / a.ends, e = a.rotary_dim + (w - h * a.ends) * E;
+            if (is(h)) *(Copy*)(target(h) + e * sizeof(elem)) = *(const Copy*)(source(h) + e * sizeof(elem));
+        } else if constexpr (APPEND) {   // 16 bytes of a value
+            const int hv = a.head_dim / 8, p = w - ends, h = p / hv, d = p - h * hv;
+            const u32x4 y = *(const u32x4*)(a.v + tok * a.vt + h * a.vh + 16 * d);
+            if (page < 0) return;
+            *(u32x4*)(a.c.v + (int64_t)page * a.c.vp + h * a.c.vh + (int64_t)slot * a.c.vs + 16 * d) = y;
+            if (d == 0 && a.c.scores) a.c.scores[(((int64_t)page * a.c.kv_heads + h) << a.c.shift) + slot] = 0.f;
         }
         return;
     }
+    const int g = w / a.turned, u = w - g * a.turned;
     const int lo = u * NP, hi = lo + a.rotary_dim / 2;   // first values of the unit's pieces
     float co[ANGLES], si[ANGLES];
     {
@@ -168,14 +164,13 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnParams a) {
     }
 }
 
-// Units of a head and groups of heads: one head a thread while the card has room for more
-// threads, up to eight past that.
+// One head a thread while the card has room for more threads, up to eight past that.
 static void divide(TurnParams& a, int piece, bool pairs, bool wide, int64_t tokens) {
     const int e = wide ? piece : 1;
     a.turned = pairs ? a.rotary_dim / (wide ? e : 2) : a.rotary_dim / 2 / e;
-    a.units = a.turned + (a.head_dim - a.rotary_dim) / e;
+    a.ends = (a.head_dim - a.rotary_dim) / e;
     a.groups = std::max(a.heads, 1);
-    while (a.groups > (a.heads + 7) / 8 && tokens * a.units * a.groups > 1 << 18) a.groups = (a.groups + 1) / 2;
+    while (a.groups > (a.heads + 7) / 8 && tokens * a.turned * a.groups > 1 << 18) a.groups = (a.groups + 1) / 2;
 }
 
 template <typename T, bool PAIRS, bool APPEND>
@@ -189,9 +184,10 @@ static int launch_turns(TurnParams& a, int dtype, bool pairs, int64_t tokens, in
     const int piece = dtype == TMS_DTYPE_F32 ? 4 : 8;
     const bool wide = (pairs ? a.rotary_dim : a.rotary_dim / 2) % piece == 0;
     divide(a, piece, pairs, wide, tokens * batch);
-    const int64_t per = (int64_t)a.groups * a.units + (APPEND ? a.c.kv_heads * (a.head_dim / 8) : 0);
-    const int64_t blocks = (tokens * per + 255) / 256;
-    if (per > INT32_MAX - 256 || blocks > INT32_MAX) return TMS_ERR_CAPACITY;
+    a.copies = a.heads * a.ends + (APPEND ? a.c.kv_heads * (a.head_dim / 8) : 0);
+    const int64_t turn_blocks = (tokens * a.groups * a.turned + 255) / 256, blocks = turn_blocks + (tokens * a.copies + 255) / 256;
+    if (blocks > INT32_MAX) return TMS_ERR_CAPACITY;
+    a.turn_blocks = (int)turn_blocks;
     const dim3 grid((unsigned)blocks, (unsigned)batch);
     if (dtype == TMS_DTYPE_F32) {
         if constexpr (!APPEND) {

@@ -23,10 +23,16 @@
 namespace tms {
 
 constexpr int kVerThreads = 512, kVerWaves = kVerThreads / 64;
-constexpr int kVerNodes = TMS_TREE_MAX_NODES, kVerSets = kVerNodes / 64;
-constexpr int kVerSteps = 8;             // loads of 16 bytes a thread has of its part's row, at most
+constexpr int kVerNodes = TMS_TREE_MAX_NODES;
+constexpr int kVerParts = 128;           // of a sequence, two a lane
 constexpr int kVerPolls = 256;           // some 0.2 ms, where a call takes 10 to 60 us
 constexpr uint64_t kThere = 1ull << 63;
+static_assert(kVerNodes == kVerThreads, "a thread has a node");
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// A part's ids: those whose R a thread keeps in registers, 16 (32 where it keeps them in 16 bits).
+constexpr int verify_ids(bool wide, bool drawn) { return kVerThreads * (wide || drawn ? 16 : 32); }
 
 struct VerifyParams {
     const void* target;
@@ -40,8 +46,9 @@ struct VerifyParams {
     int32_t* path;
     int32_t* kept;
     int32_t* token;
-    uint64_t* slots;            // [batch][max_q + 1 passes][parts]
-    int parts, steps;
+    uint64_t* slots;            // [batch][passes][parts]
+    int64_t words;              // of them
+    int passes, parts;
     int polls;                  // of a wait for another part's sum
 };
 
@@ -55,50 +62,58 @@ __device__ __forceinline__ TreeView tree_view(const VerifyParams& a, int b) {
     return s;
 }
 
-__global__ __launch_bounds__(256) void verify_clear_kernel(VerifyParams a) {
-    const int b = blockIdx.x;
-    const int64_t all = (int64_t)(tree_view(a, b).n + 1) * a.parts;
-    uint64_t* s = a.slots + (int64_t)b * (a.max_q + 1) * a.parts;
-    for (int64_t i = threadIdx.x; i < all; i += 256) st_agent(s + i, (uint64_t)0);
+// One workgroup where it has few words to clear (on one XCD it takes 1.4 us, on all of them 4).
+__global__ __launch_bounds__(1024) void verify_clear_kernel(VerifyParams a) {
+    for (int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x; i < a.words; i += (int64_t)gridDim.x * 1024) st_agent(a.slots + i, (uint64_t)0);
 }
 
 // Entries that are no probability count as 0.
 __device__ __forceinline__ double clean(float p) { return p > 0.f && p <= 3.402823466e38f ? (double)p : 0.0; }
 
-__device__ __forceinline__ double wave_sum(double x) {   // the same in every lane
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-    return x;
+// x of the lane that `CTRL` names, 0 where that is none or the row is not in ROWS.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double lane_move(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 15, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 15, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
-__device__ __forceinline__ double wave_upto(double x, int lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const double y = __shfl_up(x, d);
-        if (lane >= d) x += y;
-    }
+// Sums up to each lane: within rows of 16 by shifts of 1, 2, 4 and 8, then the last lane of a row
+// to the next one, and of the first two rows to the others.
+__device__ __forceinline__ double wave_upto(double x) {
+    x += lane_move<0x111, 15>(x);
+    x += lane_move<0x112, 15>(x);
+    x += lane_move<0x114, 15>(x);
+    x += lane_move<0x118, 15>(x);
+    x += lane_move<0x142, 10>(x);
+    x += lane_move<0x143, 12>(x);
     return x;
 }
 
 template <typename T, bool DRAWN>
 struct Verify {
-    static constexpr int VEC = Elt<T>::kVec, STEP = kVerThreads * VEC, NB = 16 / VEC;   // NB steps' values in registers
+    // Of a part's ids a wave has CELL one after another, in steps of STEP, VEC of them a lane.
+    static constexpr int VEC = Elt<T>::kVec, STEP = 64 * VEC;
+    static constexpr int PART = verify_ids(sizeof(T) == 4, DRAWN), CELL = PART / kVerWaves, STEPS = CELL / STEP;
     struct Shared {
-        double u[kVerNodes], left[kVerNodes], q[kVerNodes];   // R(x) and q(x) of a node under its parent
-        double hist[kVerNodes];                               // S before each refusal at the current node
-        double cell[kVerSteps * kVerWaves];                   // sums of a wave's 64 VEC ids
-        double part[64];
-        int32_t id[kVerNodes];
-        int16_t up[kVerNodes], path[kVerNodes];
-        uint32_t gone[DRAWN ? 1 : kVerSteps * STEP / 32];     // given drafts refused, of a part's ids
-        uint64_t missing;
+        double u[kVerNodes], left[kVerNodes], q[DRAWN ? kVerNodes : 1];   // R(x) and q(x) of a node under its parent
+        double hist[DRAWN ? kVerNodes : 1];                               // S before each refusal at the current node
+        double cell[kVerWaves], other[kVerWaves];                         // sums of the waves' ids
+        double part[kVerParts];
+        int32_t id[DRAWN ? 1 : kVerNodes];
+        int16_t up[kVerNodes], path[kVerNodes];   // (given drafts: the parent of a node that it accepts, else -1)
+        int16_t kin[DRAWN ? 1 : kVerNodes];       // given drafts: the parent
+        uint64_t missing[2];
     };
     const VerifyParams& a;
     Shared& sm;
     const int b, own, t, lane, wave;
     const TreeView tree;
-    int up[kVerSets], id[kVerSets];   // the lane's nodes, 64 k + lane: parent and token
-    int cells_of = -1;                // the part that sm.cell is of
+    int up_t;                         // the thread's node, t: parent, R(x) and q(x)
+    double left_t, q_t;
+    u32x4 row[STEPS];                 // the part's ids: p, with drawn drafts q
+    double rest[DRAWN ? STEPS : 1][VEC];   // and R
     int pass = 0;
 
     __device__ Verify(const VerifyParams& a_, Shared& sm_, int b_, int part)
@@ -110,227 +125,337 @@ struct Verify {
 
     // The tree, and each node's two numbers.
     __device__ void load() {
-        for (int i = t; i < tree.n; i += kVerThreads) {
-            const int p = a.parents[tree.q0 + i], x = a.ids[tree.q0 + i];
-            const bool in = p >= 0 && p < i && (unsigned)x < (unsigned)a.vocab;
-            sm.u[i] = a.uniforms[tree.q0 + i];
-            sm.id[i] = x;
-            sm.up[i] = (int16_t)(p >= 0 && p < i ? p : -1);
-            sm.left[i] = in ? clean(Elt<T>::scalar(target_row(p) + x)) : 0.0;
-            sm.q[i] = !DRAWN ? 1.0 : in ? clean(Elt<T>::scalar(draft_row(p) + x)) : 0.0;
+        int p = -1, x = -1;
+        double u = 0.0;
+        if (t < tree.n) {
+            p = a.parents[tree.q0 + t];
+            x = a.ids[tree.q0 + t];
+            u = a.uniforms[tree.q0 + t];
         }
-#pragma unroll
-        for (int k = 0; k < kVerSets; ++k) {
-            const int i = 64 * k + lane;
-            up[k] = -1;
-            id[k] = 0;
-            if (i < tree.n) {
-                const int p = a.parents[tree.q0 + i];
-                up[k] = p >= 0 && p < i ? p : -1;
-                id[k] = a.ids[tree.q0 + i];
-            }
+        up_t = p < t ? p : -1;
+        const bool in = up_t >= 0 && (unsigned)x < (unsigned)a.vocab;
+        left_t = q_t = 0.0;
+        if (in) {
+            const float y = Elt<T>::scalar(target_row(up_t) + x), z = DRAWN ? Elt<T>::scalar(draft_row(up_t) + x) : 0.f;
+            left_t = clean(y);
+            q_t = clean(z);
+        }
+        up_t = max(up_t, -1);
+        sm.u[t] = u;
+        sm.left[t] = left_t;
+        if constexpr (DRAWN) {
+            sm.up[t] = (int16_t)up_t;
+            sm.q[t] = q_t;
+        } else {
+            // Whether a node would be accepted depends on its elder siblings alone: S is 1 without
+            // what they have, a token that several of them have counting once.
+            sm.kin[t] = (int16_t)up_t;
+            sm.id[t] = x;
+            lds_sync();
+            bool twice = false;
+            for (int i = up_t + 1; i < t && t < tree.n; ++i) twice |= sm.kin[i] == up_t && sm.id[i] == x;
+            lds_sync();
+            if (twice) sm.left[t] = left_t = 0.0;
+            lds_sync();
+            double S = 1.0;
+            for (int i = up_t + 1; i < t && t < tree.n; ++i) S -= sm.kin[i] == up_t ? sm.left[i] : 0.0;
+            sm.up[t] = (int16_t)(u * S < left_t ? up_t : -1);
         }
         lds_sync();
     }
 
-    // The first child of c past node j, -1 without one.
+    // The first child of c past node j (given drafts: that is accepted), -1 without one.
     __device__ int child(int c, int j) const {
-#pragma unroll
-        for (int k = 0; k < kVerSets; ++k)
-            if (64 * k < tree.n && 64 * k + 63 > j) {
-                const uint64_t m = __ballot(up[k] == c && 64 * k + lane > j);
-                if (m) return 64 * k + __builtin_ctzll(m);
-            }
+        for (int k = (j + 1) & ~63; k < tree.n; k += 64) {
+            const uint64_t m = __ballot(sm.up[k + lane] == c && k + lane > j);
+            if (m) return k + __builtin_ctzll(m);
+        }
         return -1;
     }
-    // Given drafts: an earlier child of c has the token of j.
-    __device__ bool twice(int c, int j) const {
-        const int x = sm.id[j];
-        bool same = false;
+    // A row's entries of a part's steps from `step` on: zeros past the vocabulary.
+    template <int N>
+    __device__ void fetch(const T* r, int part, int step, u32x4 (&w)[N]) const {
+        const int first = part * PART + wave * CELL + step * STEP, end = a.vocab - a.vocab % VEC;   // past it is one piece that is not whole
 #pragma unroll
-        for (int k = 0; k < kVerSets; ++k)
-            if (64 * k < j) same |= up[k] == c && 64 * k + lane < j && id[k] == x;
-        return __any(same);
-    }
-
-    __device__ uint4 fetch(const T* row, int at) const {   // VEC entries from id `at` on, zeros past the vocabulary
-        if (at + VEC <= a.vocab) return ld_any(row + at);
-        uint32_t w[4] = {0, 0, 0, 0};
-        for (int e = 0; e < VEC && at + e < a.vocab; ++e) {
-            if constexpr (sizeof(T) == 4) w[e] = __float_as_uint(Elt<T>::scalar(row + at + e));
-            else w[e / 2] |= (uint32_t)*(const uint16_t*)(row + at + e) << 16 * (e & 1);
-        }
-        return make_uint4(w[0], w[1], w[2], w[3]);
-    }
-
-    // R of NB steps from `step` on of a part, after `m` refusals at c; `whole`: the row as it is.
-    __device__ void residual(int part, int step, int n, int c, int m, bool whole, double (&r)[NB][VEC]) const {
-        const int at = part * a.steps * STEP + step * STEP + t * VEC;
-        uint4 pq[NB], dq[NB];
-#pragma unroll
-        for (int k = 0; k < NB; ++k)
-            if (k < n) {
-                pq[k] = fetch(target_row(c), at + k * STEP);
-                if (DRAWN && m > 0) dq[k] = fetch(draft_row(c), at + k * STEP);
-            }
-#pragma unroll
-        for (int k = 0; k < NB; ++k) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) r[k][e] = k < n ? clean(elt<T>(pq[k], e)) : 0.0;
-            if (!DRAWN && !whole && k < n) {
-                const int from = (step + k) * STEP + t * VEC;
-                const uint32_t bits = sm.gone[from / 32] >> (from & 31);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e)
-                    if (bits >> e & 1) r[k][e] = 0.0;
+        for (int k = 0; k < N; ++k) {
+            const int at = first + k * STEP + lane * VEC;
+            w[k] = (u32x4){0, 0, 0, 0};
+            if (at < end) {
+                const uint4 x = ld_any(r + at);
+                w[k] = (u32x4){x.x, x.y, x.z, x.w};
             }
         }
+        const int cut = end - first;
+        if (end < a.vocab && cut >= 0 && cut < N * STEP && cut % STEP / VEC == lane) {
+            u32x4 x = (u32x4){0, 0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < VEC - 1; ++e)
+                if (end + e < a.vocab) {
+                    if constexpr (sizeof(T) == 4) x[e] = *(const uint32_t*)(r + end + e);
+                    else x[e / 2] |= (uint32_t)*(const uint16_t*)(r + end + e) << 16 * (e & 1);
+                }
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (cut / STEP == k) w[k] = x;
+        }
+    }
+    // Entries that are no probability as 0: those whose bits are not below infinity's.
+    static __device__ u32x4 cleaned(u32x4 w) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                w[i] = w[i] < 0x7F800000u ? w[i] : 0;
+            } else {
+                constexpr uint32_t inf = __is_same(T, Bf16) ? 0x7F80u : 0x7C00u;
+                w[i] = (w[i] & 0xFFFFu) < inf ? w[i] : w[i] & 0xFFFF0000u;
+                w[i] = w[i] < inf << 16 ? w[i] : w[i] & 0xFFFFu;
+            }
+        }
+        return w;
+    }
+    static __device__ double entry(u32x4 w, int e) { return (double)elt<T>(make_uint4(w[0], w[1], w[2], w[3]), e); }
+
+    // Given drafts: the tokens of c's children, all refused, out of the entries of `fetch`.
+    template <int N>
+    __device__ void without(u32x4 (&w)[N], int c, int part, int step) const {
+        const int first = part * PART + wave * CELL + step * STEP;
+        for (int k = c & ~63; k < tree.n; k += 64) {
+            const int id = sm.id[k + lane];
+            for (uint64_t m = __ballot(sm.kin[k + lane] == c && id >= first && id - first < N * STEP); m; m &= m - 1) {
+                const int x = __builtin_amdgcn_readlane(id, __builtin_ctzll(m)) - first;
+                if (x % STEP / VEC != lane) continue;
+                const int word = x % VEC * (int)sizeof(T) / 4;
+                const uint32_t keep = sizeof(T) == 4 ? 0u : x & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (x / STEP == n && word == i) w[n][i] &= keep;
+            }
+        }
+    }
+
+    // R of the part's ids at node c: the target row, with given drafts (not `whole`) without c's children.
+    __device__ void begin(int c, bool whole) {
+        u32x4 p[STEPS];
+        fetch(target_row(c), own, 0, p);
         if constexpr (DRAWN) {
-            for (int i = 0; i < m; ++i) {
-                const double s = sm.hist[i];
+            if (!whole) fetch(draft_row(c), own, 0, row);
 #pragma unroll
-                for (int k = 0; k < NB; ++k)
-                    if (k < n)
+            for (int k = 0; k < STEPS; ++k) {
+                p[k] = cleaned(p[k]);
+                row[k] = cleaned(row[k]);
 #pragma unroll
-                        for (int e = 0; e < VEC; ++e) r[k][e] = fmax(r[k][e] - s * clean(elt<T>(dq[k], e)), 0.0);
+                for (int e = 0; e < VEC; ++e) rest[k][e] = entry(p[k], e);
             }
+        } else {
+            if (!whole) without(p, c, own, 0);
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) row[k] = cleaned(p[k]);
         }
     }
-
-    __device__ double lane_sum(const double (&r)[VEC]) const {
+    // R of a step's ids, and their sum.  (The entries are widened each time: kept in fp64
+    // they would not fit the registers.)
+    __device__ void values(int k, double (&r)[VEC]) const {
+        if constexpr (DRAWN) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) r[e] = rest[k][e];
+        } else {
+            u32x4 w = row[k];
+            asm volatile("" : "+v"(w));
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) r[e] = entry(w, e);
+        }
+    }
+    static __device__ double sum_of(const double (&r)[VEC]) {
         double s = r[0];
 #pragma unroll
         for (int e = 1; e < VEC; ++e) s += r[e];
         return s;
     }
-
-    // The sum of R over a part's ids, by cells of sm.cell.
-    __device__ double sum_part(int part, int c, int m, bool whole) {
-        lds_sync();   // sm.cell and sm.gone are free, sm.hist is there
-        if (!DRAWN && !whole) {
-            const int words = a.steps * STEP / 32, first = part * a.steps * STEP;
-            for (int i = t; i < words; i += kVerThreads) sm.gone[i] = 0;
-            lds_sync();
-            for (int i = t; i < tree.n; i += kVerThreads) {
-                const int64_t x = (int64_t)sm.id[i] - first;
-                if (sm.up[i] == c && x >= 0 && x < a.steps * STEP) atomicOr(&sm.gone[x / 32], 1u << (x & 31));
-            }
-            lds_sync();
-        }
-        for (int step = 0; step < a.steps; step += NB) {
-            const int n = min(NB, a.steps - step);
-            double r[NB][VEC];
-            residual(part, step, n, c, m, whole, r);
+    __device__ void refuse(double S) {
 #pragma unroll
-            for (int k = 0; k < NB; ++k)
-                if (k < n) {
-                    const double s = wave_sum(lane_sum(r[k]));
-                    if (lane == 0) sm.cell[(step + k) * kVerWaves + wave] = s;
-                }
+        for (int k = 0; k < STEPS; ++k) {
+            u32x4 w = row[k];
+            asm volatile("" : "+v"(w));
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) rest[DRAWN ? k : 0][e] = fmax(rest[DRAWN ? k : 0][e] - S * entry(w, e), 0.0);
         }
-        lds_sync();
-        cells_of = part;
-        double s = 0.0;
-        for (int i = 0; i < a.steps * kVerWaves; ++i) s += sm.cell[i];
+    }
+
+    static __device__ double cells_sum(const double (&cell)[kVerWaves]) {
+        double s = cell[0];
+#pragma unroll
+        for (int w = 1; w < kVerWaves; ++w) s += cell[w];
         return s;
+    }
+
+    // The sum of the part's R, by cells.
+    __device__ double sum_own() {
+        lds_sync();   // sm.cell has been read
+        double s = 0.0;
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k) {
+            double r[VEC];
+            values(k, r);
+            s += sum_of(r);
+        }
+        s = wave_upto(s);
+        if (lane == 63) sm.cell[wave] = s;
+        lds_sync();
+        return cells_sum(sm.cell);
+    }
+
+    // The same of another part, after `m` refusals at c: the same operations in the same order.
+    __device__ double sum_other(int part, int c, int m, bool whole) {
+        lds_sync();
+        double s = 0.0;
+#pragma unroll 1
+        for (int k = 0; k < STEPS; ++k) {
+            u32x4 p[1], q[1] = {(u32x4){0, 0, 0, 0}};
+            fetch(target_row(c), part, k, p);
+            if (DRAWN && m > 0) fetch(draft_row(c), part, k, q);
+            if (!DRAWN && !whole) without(p, c, part, k);
+            p[0] = cleaned(p[0]);
+            q[0] = cleaned(q[0]);
+            double r[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                r[e] = entry(p[0], e);
+                if constexpr (DRAWN) {
+                    const double y = entry(q[0], e);
+                    for (int i = 0; i < m; ++i) r[e] = fmax(r[e] - sm.hist[i] * y, 0.0);
+                }
+            }
+            s += sum_of(r);
+        }
+        s = wave_upto(s);
+        if (lane == 63) sm.other[wave] = s;
+        lds_sync();
+        return cells_sum(sm.other);
     }
 
     // The sum over the whole vocabulary; sm.part has the parts'.
     __device__ double sum_all(int c, int m, bool whole) {
-        const double mine = sum_part(own, c, m, whole);
+        const double mine = sum_own();
         if (a.parts == 1) return mine;
-        uint64_t* const slot = a.slots + ((int64_t)b * (a.max_q + 1) + pass) * a.parts;
+        uint64_t* const slot = a.slots + ((int64_t)b * a.passes + pass) * a.parts;
         ++pass;
         if (t == 0) st_agent(slot + own, __builtin_bit_cast(uint64_t, mine) | kThere);
         if (wave == 0) {
-            uint64_t v = lane < a.parts ? 0 : kThere, none = 0;
-            if (lane == own) v = __builtin_bit_cast(uint64_t, mine) | kThere;
-            none = __ballot(v == 0);
-            for (int it = 0; none && it < a.polls; ++it) {
-                if (v == 0) v = ld_agent(slot + lane);
-                none = __ballot(v == 0);
-                if (none) __builtin_amdgcn_s_sleep(1);
+            uint64_t v[2], none[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                v[i] = 2 * lane + i == own ? __builtin_bit_cast(uint64_t, mine) | kThere : 2 * lane + i < a.parts ? 0 : kThere;
+                none[i] = __ballot(v[i] == 0);
             }
-            sm.part[lane] = __builtin_bit_cast(double, v & ~kThere);
-            if (lane == 0) sm.missing = none;
+            for (int it = 0; (none[0] | none[1]) && it < a.polls; ++it) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (v[i] == 0) v[i] = ld_agent(slot + 2 * lane + i);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) none[i] = __ballot(v[i] == 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                sm.part[2 * lane + i] = __builtin_bit_cast(double, v[i] & ~kThere);
+                if (lane == 0) sm.missing[i] = none[i];
+            }
         }
         lds_sync();
-        for (uint64_t none = sm.missing; none; none &= none - 1) {
-            const int p = __builtin_ctzll(none);
-            const double s = sum_part(p, c, m, whole);
-            if (t == 0) sm.part[p] = s;
-        }
-        lds_sync();
-        return __shfl(wave_upto(sm.part[lane], lane), 63);
+        bool any = false;
+        for (int i = 0; i < 2; ++i)
+            for (uint64_t none = sm.missing[i]; none; none &= none - 1) {
+                const int p = 2 * __builtin_ctzll(none) + i;
+                const double s = sum_other(p, c, m, whole);
+                if (t == 0) sm.part[p] = s;
+                any = true;
+            }
+        if (any) lds_sync();
+        return readlane_f64(wave_upto(sm.part[2 * lane] + sm.part[2 * lane + 1]), 63);
     }
 
-    // The first id with more than `rest` up to it, of this workgroup's part.
-    __device__ void pick(int c, int m, bool whole, double rest) {
-        if (cells_of != own) sum_part(own, c, m, whole);
-        double run = 0.0, before = 0.0;
+    // The first id with more than `aim` up to it, of this workgroup's part, which has some.
+    __device__ void pick(double aim) {
+        double at = 0.0, run = 0.0;
         int cell = -1;
-        for (int i = 0; i < a.steps * kVerWaves; ++i) {
-            const double s = sm.cell[i];
-            if (s > 0.0) {
-                cell = i;
-                before = run;
-                if (run + s > rest) break;
-            }
-            run += s;
-        }
-        if (cell < 0 || cell % kVerWaves != wave) return;
-        const int step = cell / kVerWaves;
-        double r[NB][VEC];
-        residual(own, step, 1, c, m, whole, r);
-        const double s = lane_sum(r[0]), upto = wave_upto(s, lane);
-        const uint64_t over = __ballot(s > 0.0 && before + upto > rest), some = __ballot(s > 0.0);
-        const int who = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : -1;
-        const double below = __shfl_up(upto, 1);
-        if (lane != who) return;
-        double at = before + (lane ? below : 0.0);
-        int found = -1;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            if (r[0][e] > 0.0 && (found < 0 || !(at > rest))) found = e;
-            at += r[0][e];
+        for (int w = 0; w < kVerWaves; ++w) {
+            if (sm.cell[w] > 0.0 && (cell < 0 || !(run > aim))) {
+                cell = w;
+                at = run;
+            }
+            run += sm.cell[w];
         }
-        a.token[b] = own * a.steps * STEP + step * STEP + t * VEC + found;
+        if (cell != wave) return;
+        int found = -1;
+        for (int k = 0; k < STEPS; ++k) {
+            double r[VEC];
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i)
+                if (i == k) values(i, r);
+            const double mine = sum_of(r), here = wave_upto(mine);
+            const uint64_t some = __ballot(mine > 0.0), over = __ballot(mine > 0.0 && at + here > aim);
+            if (found >= 0 && at > aim) break;   // (a sum's last bit)
+            if (some) {   // the last step with some where none goes past
+                const int who = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
+                double x = who ? at + readlane_f64(here, who - 1) : at;
+                int e0 = -1;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    if (r[e] > 0.0 && (e0 < 0 || !(x > aim))) e0 = e;
+                    x += r[e];
+                }
+                found = own * PART + wave * CELL + k * STEP + who * VEC + __builtin_amdgcn_readlane(e0, who);
+                if (over) break;
+            }
+            at += readlane_f64(here, 63);
+        }
+        if (lane == 0) a.token[b] = found;
     }
 
     __device__ void run() {
         load();
-        int c = 0, m = 0, len = 1, j = 0;
-        double S = 1.0;
-        while ((j = child(c, j)) >= 0) {
-            const double r = !DRAWN && twice(c, j) ? 0.0 : sm.left[j];
-            if (sm.u[j] * sm.q[j] * S < r) {
+        int c = 0, m = 0, len = 1, j = 0;   // the node, refusals at it, nodes of the path, the child last tried
+        double S = 1.0, total = 0.0;
+        bool whole = false;
+        for (;;) {
+            bool refused = false;   // a drawn draft: a pass over the vocabulary
+            while (j >= 0 && (j = child(c, j)) >= 0) {
+                if (DRAWN && !(sm.u[j] * sm.q[j] * S < sm.left[j])) {
+                    refused = true;
+                    break;
+                }
                 if (t == 0) sm.path[len] = (int16_t)j;
                 ++len;
                 c = j;
                 S = 1.0;
                 m = 0;
-            } else if (DRAWN) {
-                lds_sync();   // sm.left and sm.hist have been read
-                for (int i = t; i < tree.n; i += kVerThreads)
-                    if (sm.up[i] == c) sm.left[i] = fmax(sm.left[i] - S * sm.q[i], 0.0);
-                if (t == 0) sm.hist[m] = S;
-                ++m;
-                S = sum_all(c, m, false);
-            } else {
-                S -= r;
             }
-        }
-        bool whole = false;
-        double total = DRAWN && m > 0 ? S : sum_all(c, m, false);
-        if (!(total > 0.0)) {   // nothing is left
-            whole = true;
+            if (refused || whole || m == 0) {   // (else the last refusal's sum is R's)
+                if (m == 0) begin(c, whole);
+                if (DRAWN && refused) {
+                    lds_sync();   // sm.left and sm.hist have been read
+                    if (up_t == c) sm.left[t] = left_t = fmax(left_t - S * q_t, 0.0);
+                    if (t == 0) sm.hist[m] = S;
+                    refuse(S);
+                    ++m;
+                }
+                total = sum_all(c, m, whole);
+                if (refused) {
+                    S = total;
+                    continue;
+                }
+            }
+            if (total > 0.0 || whole) break;
+            whole = true;   // nothing is left
             m = 0;
-            total = sum_all(c, m, true);
         }
         if (own == 0) {
             if (t == 0) sm.path[0] = 0;
             lds_sync();
-            for (int i = t; i < a.max_q; i += kVerThreads) a.path[(int64_t)b * a.max_q + i] = i < len ? sm.path[i] : -1;
+            if (t < a.max_q) a.path[(int64_t)b * a.max_q + t] = t < len ? sm.path[t] : -1;
             if (t == 0) {
                 a.kept[b] = len;
                 if (!(total > 0.0)) a.token[b] = -1;
@@ -340,23 +465,26 @@ struct Verify {
         const double aim = fmax(sm.u[0] * total, 0.0);   // (a NaN gives 0)
         double before = 0.0;
         if (a.parts > 1) {
-            const double s = sm.part[lane], upto = wave_upto(s, lane);
+            const double s0 = sm.part[2 * lane], s1 = sm.part[2 * lane + 1], s = s0 + s1, upto = wave_upto(s);
             const uint64_t over = __ballot(s > 0.0 && upto > aim), some = __ballot(s > 0.0);
             const int who = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
-            if (who != own) return;
-            before = own ? __shfl(upto, own - 1) : 0.0;
+            if (who) before = readlane_f64(upto, who - 1);
+            const double first = readlane_f64(s0, who), second = readlane_f64(s1, who);
+            const bool next = second > 0.0 && !(first > 0.0 && before + first > aim);
+            if (own != 2 * who + next) return;
+            if (next) before += first;
         }
-        pick(c, m, whole, aim - before);
+        pick(aim - before);
     }
 };
 
 template <typename T, bool DRAWN>
-__global__ __launch_bounds__(kVerThreads) void verify_tree_kernel(VerifyParams a) {
+__global__ __launch_bounds__(kVerThreads, DRAWN ? 4 : 8) void verify_tree_kernel(VerifyParams a) {
     __shared__ typename Verify<T, DRAWN>::Shared sm;
     const int b = blockIdx.x / a.parts, part = blockIdx.x - b * a.parts;
     if (tree_view(a, b).n == 0) {
         if (part == 0) {
-            for (int i = threadIdx.x; i < a.max_q; i += kVerThreads) a.path[(int64_t)b * a.max_q + i] = -1;
+            if ((int)threadIdx.x < a.max_q) a.path[(int64_t)b * a.max_q + threadIdx.x] = -1;
             if (threadIdx.x == 0) {
                 a.kept[b] = 0;
                 a.token[b] = -1;
@@ -369,22 +497,20 @@ __global__ __launch_bounds__(kVerThreads) void verify_tree_kernel(VerifyParams a
 }
 
 struct VerifyPlan {
-    int parts, steps;
-    size_t bytes;
+    int parts, passes;
+    size_t words, bytes;
 };
 
-// As many parts as bring the card some workgroups a CU, up to 64, with one step each at least.
 static VerifyPlan plan_verify(const tms_verify_tree_args* a) {
     VerifyPlan p;
-    const int step = kVerThreads * (a->dtype == TMS_DTYPE_F32 ? 4 : 8);
-    const int steps = (a->vocab + step - 1) / step;   // of the vocabulary
-    const int want = std::max(1, std::min(64, 1024 / std::max(a->batch, 1)));
-    p.steps = std::min(std::max(1, (steps + want - 1) / want), kVerSteps);
-    p.parts = (steps + p.steps - 1) / p.steps;
-    p.bytes = p.parts > 1 ? (size_t)a->batch * (a->max_q + 1) * p.parts * 8 : 0;
+    const int ids = verify_ids(a->dtype == TMS_DTYPE_F32, a->draft != nullptr);
+    p.parts = (a->vocab + ids - 1) / ids;
+    p.passes = a->draft ? a->max_q + 1 : 2;   // the refusals, the last draw, and that again where nothing is left
+    p.words = p.parts > 1 ? (size_t)a->batch * p.passes * p.parts : 0;
+    p.bytes = p.words * 8;
     return p;
 }
-static_assert(TMS_VERIFY_MAX_VOCAB <= 64 * kVerSteps * kVerThreads * 4, "64 parts hold a vocabulary");
+static_assert(TMS_VERIFY_MAX_VOCAB <= kVerParts * verify_ids(true, true), "the parts hold a vocabulary");
 
 static std::atomic<int> g_polls{kVerPolls};
 
@@ -443,9 +569,10 @@ extern "C" int tms_verify_tree(const tms_verify_tree_args* args, hipStream_t str
     a.token = args->token;
     a.slots = (uint64_t*)args->workspace;
     a.parts = p.parts;
-    a.steps = p.steps;
+    a.passes = p.passes;
+    a.words = (int64_t)p.words;
     a.polls = g_polls.load(std::memory_order_relaxed);
-    if (a.parts > 1) hipLaunchKernelGGL(verify_clear_kernel, dim3(args->batch), dim3(256), 0, stream, a);
+    if (a.parts > 1) hipLaunchKernelGGL(verify_clear_kernel, dim3(a.words <= 1 << 15 ? 1 : 256), dim3(1024), 0, stream, a);
     switch (args->dtype) {
         case TMS_DTYPE_F32: launch_verify<float>(a, args->batch, stream); break;
         case TMS_DTYPE_F16: launch_verify<_Float16>(a, args->batch, stream); break;
