@@ -71,12 +71,12 @@ struct AttnParams {
     int max_kv;            // scores: positions past it are left out
     float scale;           // above 0, times log2(e): exponentials are taken to base 2
     uint32_t qand, qxor;   // a query's bits are taken through these: a scale below 0 flips its sign, 0 clears it
-    int split_tiles;       // chunk kernel: key tiles a split has; rows kernel: the least that a share has
+    int split_tiles;       // chunk kernel: key tiles a split has; rows kernel and trees: the least that a share has
     int splits;            // chunk kernel
     int row_tiles;
     float* part_o;         // parts of rows, [part][rows a tile][head_dim]
     float* part_ml;        // [part][rows a tile][2]: maximum, sum
-    int2* item_parts;      // rows kernel, [pairs * row_tiles]: the first share and the number of shares with a part
+    int2* item_parts;      // rows kernel and trees, [pairs * row_tiles]: the first share and the number of shares with a part
     const int32_t* parents;   // trees
 };
 
@@ -187,10 +187,32 @@ inline void set_scale(AttnParams& a, float scale) {
 constexpr int kChunkRows = 128;   // of a workgroup of the chunk kernel
 inline int chunk_keys(int head_dim) { return head_dim > 128 ? 32 : 64; }   // of its tile
 void launch_attn_chunk(const AttnParams& a, bool bf16, dim3 grid, hipStream_t stream);
+void launch_attn_chunk_tree(const AttnParams& a, bool bf16, int rows, int workgroups, hipStream_t stream);   // `rows` of a workgroup
 
 __device__ __forceinline__ bool sees(int j, int p, int window, int sinks) {
     return j <= p && (window <= 0 || j > p - window || j < sinks);
 }
+
+// Trees in the chunk kernel: all items (sequence, row tile, key head) lie behind each other on
+// one axis of key tiles, and each workgroup takes an equal share of it, as in the rows kernel
+// (8 sequences of 9000 to 16384, trees of 64 nodes: 160 us with four splits of each sequence, 184 with
+// as many splits as its length asks for, which leaves a second round of workgroups).
+// An item takes kTreeItemCost tiles besides its own.
+constexpr int kTreeItemCost = 4, kTreeLeastShare = 4;
+template <int KT, int RM>
+struct TreeAxis {
+    static __device__ __forceinline__ int tiles(const AttnParams& a, const SeqView& sq, int tile) {
+        const int last = min((tile + 1) * RM, sq.n * a.group) - 1;
+        return TileList<KT>(a.window, a.sinks, sq.p0, sq.p0 + last / a.group, sq.len).n;
+    }
+    static __device__ __forceinline__ int length(int tiles) { return max(tiles, 1) + kTreeItemCost; }
+    // A sequence's row tile's share of the axis, for one key head.
+    static __device__ __forceinline__ int combo(const AttnParams& a, int c) {
+        const int b = c / a.row_tiles, tile = c - b * a.row_tiles;
+        const SeqView sq = seq_view(a.c, b);
+        return tile * RM < sq.n * a.group ? length(tiles(a, sq, tile)) : 0;
+    }
+};
 
 // Trees: what the tokens of a group of rows see of the new tokens, a bit each, found by
 // climbing from node to parent in LDS (some 100 cycles a step), and their depths.  With a

@@ -493,6 +493,52 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams a, int rm, in
     if (on && 4 * lane < D) write_row<T>(a, sq, h, r, 4 * lane, M, L, acc);
 }
 
+// The parts of trees' rows from the chunk kernel, which lie as the rows kernel's do: lists are
+// short, and a group of LPR lanes takes a row, four parts' loads in flight (8 sequences of 9000 to 16384, 64
+// nodes: 10 us; 20 with several groups a row).
+template <typename T, int LPR>
+__global__ __launch_bounds__(256) void attn_tree_join_kernel(AttnParams a, int rm) {
+    const int combo = blockIdx.x / a.c.kv_heads, h = blockIdx.x - combo * a.c.kv_heads;
+    const int b = combo / a.row_tiles, tile = combo - b * a.row_tiles;
+    const SeqView sq = seq_view(a.c, b);
+    const int rows = sq.n * a.group, D = a.c.head_dim;
+    if (tile * rm + (int)blockIdx.y * (256 / LPR) >= rows) return;
+    const int2 ip = a.item_parts[blockIdx.x];
+    const int parts = ip.y;
+    if (parts == 0) return;   // written by one workgroup
+    const int lane = threadIdx.x % LPR, in = blockIdx.y * (256 / LPR) + threadIdx.x / LPR, r = tile * rm + in;
+    if (in >= rm || r >= rows) return;
+    const int d = 4 * lane < D ? 4 * lane : 0;
+    float M = -__builtin_huge_valf(), L = 0.f;
+    f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < parts; s0 += 4) {
+        float2 ml[4];
+        f32x4 o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int s = min(s0 + k, parts - 1);
+            const int64_t at = (2 * (int64_t)ip.x + (s == 0 ? 1 : 2 * s)) * rm + in;
+            ml[k] = *(const float2*)(a.part_ml + 2 * at);
+            o[k] = *(const f32x4*)(a.part_o + at * D + d);
+        }
+        float top = M;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top = fmaxf(top, ml[k].x);   // (a part twice does no harm here)
+        const float ref = top == -__builtin_huge_valf() ? 0.f : top, f = __builtin_amdgcn_exp2f(M - ref);
+        M = top;
+        L *= f;
+        acc *= f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (s0 + k < parts) {
+                const float w = __builtin_amdgcn_exp2f(ml[k].x - ref);
+                L += ml[k].y * w;
+                acc += o[k] * w;
+            }
+    }
+    if (4 * lane < D) write_row<T>(a, sq, h, r, 4 * lane, M, L, acc);
+}
+
 // ---- host ---------------------------------------------------------------------------------------
 
 // A page's stride and what its slots span in 32 bits: the chunk kernel's offsets.
@@ -511,7 +557,7 @@ struct AttnPlan {
     int rm;            // rows a workgroup
     int row_tiles;
     int split_tiles, splits;
-    int shares;        // workgroups of the rows kernel
+    int shares;        // workgroups of the rows kernel, and of the chunk kernel on trees
     int waves;         // of one of them
     bool join;
     int rows, most_parts;   // bounds: of a sequence and key head, and of a row's parts
@@ -536,15 +582,26 @@ static AttnPlan plan_attention(const tms_cache* c, const tms_attention_args* a, 
     const int rows = p.rows = min(c->max_q, c->tokens) * (a->q_heads / c->kv_heads);
     p.chunk = rows > kShareRows && short_strides(c, c->k_stride) && short_strides(c, c->v_stride);
     p.rm = p.chunk ? kChunkRows : kShareRows;
+    if (p.chunk && tree && rows > kChunkRows && c->head_dim <= 128) p.rm = 2 * kChunkRows;   // (keys read once for all)
     p.row_tiles = (rows + p.rm - 1) / p.rm;
     int64_t keys = min(c->max_kv, kMaxLen);
     if (a->window > 0) keys = std::min<int64_t>(keys, (int64_t)a->window + (tree ? c->max_q : p.rm) + a->sinks + 128);
     const int64_t items = (int64_t)c->batch * c->kv_heads * p.row_tiles;
     int64_t parts;
-    p.fits = p.chunk || items <= INT32_MAX;
+    p.fits = (p.chunk && !tree) || items <= INT32_MAX;
     p.splits = p.shares = 0;
     p.item_bytes = 0;
-    if (p.chunk) {
+    if (p.chunk && tree) {
+        // As many workgroups as the card holds at once, with 4 tiles each at least.
+        const int kt = chunk_keys(c->head_dim);
+        const int64_t tiles = std::max<int64_t>((keys + kt - 1) / kt, 1);
+        p.split_tiles = kTreeLeastShare;
+        p.shares = (int)std::min<int64_t>(c->head_dim > 128 || p.rm > kChunkRows ? 256 : 512, (tiles + kTreeItemCost) * items / kTreeLeastShare + 1);
+        p.join = true;
+        parts = 2 * (int64_t)p.shares;
+        p.most_parts = (int)std::min<int64_t>(tiles / kTreeLeastShare + 2, p.shares);
+        p.item_bytes = (size_t)(items * 8 + 15) / 16 * 16;
+    } else if (p.chunk) {
         // Workgroups enough for two a CU, with 4 tiles each at least.
         const int kt = chunk_keys(c->head_dim);
         const int tiles = (int)((keys + kt - 1) / kt);
@@ -589,15 +646,29 @@ static void launch_join(const AttnPlan& p, const AttnParams& a, int pairs, hipSt
                        p.rm, sub);
 }
 
+template <typename T, int LPR>
+static void launch_tree_join(const AttnPlan& p, const AttnParams& a, hipStream_t stream) {
+    const int each = 256 / LPR, rows = std::min(p.rm, p.rows);
+    const unsigned items = (unsigned)a.c.batch * p.row_tiles * a.c.kv_heads;
+    hipLaunchKernelGGL((attn_tree_join_kernel<T, LPR>), dim3(items, (rows + each - 1) / each), dim3(256), 0, stream, a, p.rm);
+}
+
 template <typename T, bool TREE>
 static void launch_attention(const AttnPlan& p, const AttnParams& a, hipStream_t stream) {
     const int D = a.c.head_dim, pairs = a.c.batch * a.c.kv_heads;
-    if (p.chunk) launch_attn_chunk(a, std::is_same<T, Bf16>::value, dim3(pairs, p.row_tiles, p.splits), stream);
+    if (p.chunk && TREE) launch_attn_chunk_tree(a, std::is_same<T, Bf16>::value, p.rm, p.shares, stream);
+    else if (p.chunk) launch_attn_chunk(a, std::is_same<T, Bf16>::value, dim3(pairs, p.row_tiles, p.splits), stream);
     else if (D <= 64) launch_rows<T, 128, 4, 2, TREE>(p, a, stream);
     else if (D <= 96) launch_rows<T, 256, 6, 3, TREE>(p, a, stream);
     else if (D <= 128) launch_rows<T, 256, 8, 4, TREE>(p, a, stream);
     else launch_rows<T, 512, 16, 8, TREE>(p, a, stream);
     if (!p.join) return;
+    if (TREE && p.chunk) {
+        if (D <= 64) launch_tree_join<T, 16>(p, a, stream);
+        else if (D <= 128) launch_tree_join<T, 32>(p, a, stream);
+        else launch_tree_join<T, 64>(p, a, stream);
+        return;
+    }
     if (D <= 64) launch_join<T, 16>(p, a, pairs, stream);
     else if (D <= 128) launch_join<T, 32>(p, a, pairs, stream);
     else launch_join<T, 64>(p, a, pairs, stream);
@@ -619,7 +690,7 @@ static int attention(const tms_cache* cache, const tms_attention_args* args, con
     if (cache->batch == 0 || cache->tokens == 0 || cache->max_q == 0) return TMS_OK;
     if (TREE && (!parents || ((uintptr_t)parents & 3))) return TMS_ERR_INVALID_ARG;
     const AttnPlan p = plan_attention(cache, args, TREE);
-    if (args->workspace_bytes < (size_t)need || (p.join && (!args->workspace || !aligned16(args->workspace)))) return TMS_ERR_INVALID_ARG;
+    if (args->workspace_bytes < (size_t)need || (need > 0 && (!args->workspace || !aligned16(args->workspace)))) return TMS_ERR_INVALID_ARG;
     AttnParams a;
     a.c = view_of(cache);
     a.q = (const char*)args->q;
@@ -640,7 +711,7 @@ static int attention(const tms_cache* cache, const tms_attention_args* args, con
     a.row_tiles = p.row_tiles;
     a.part_o = (float*)args->workspace;
     a.part_ml = (float*)((char*)args->workspace + p.o_bytes);
-    a.item_parts = p.chunk ? nullptr : (int2*)((char*)args->workspace + p.o_bytes + p.ml_bytes);
+    a.item_parts = p.chunk && !TREE ? nullptr : (int2*)((char*)args->workspace + p.o_bytes + p.ml_bytes);
     a.parents = parents;
     if (cache->dtype == TMS_DTYPE_BF16) launch_attention<Bf16, TREE>(p, a, stream);
     else launch_attention<F16, TREE>(p, a, stream);

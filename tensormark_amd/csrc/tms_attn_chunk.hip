@@ -18,30 +18,40 @@
 
 namespace tms {
 
-template <typename T, int ROWB, int KS, int DT, int NK, bool TREE>
-__global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(AttnParams a) {
-    constexpr int KT = 32 * NK, RM = kChunkRows;
-    constexpr int C = ROWB / 16, RPI = 64 / C, NI = KT / (4 * RPI);   // pieces a row; rows a load; loads a wave
+template <int ROWB, int NK, int NW, bool TREE>
+struct ChunkShared {
+    static constexpr int KT = 32 * NK, NV = ROWB > 256 ? 3 : 2;   // keys of a tile; value buffers
+    __attribute__((aligned(128))) char k[2][KT * ROWB];
+    __attribute__((aligned(128))) char v[NV][KT * ROWB];
+};
+template <int ROWB, int NK, int NW>
+struct ChunkShared<ROWB, NK, NW, true> : ChunkShared<ROWB, NK, NW, false> {
+    TreeRows<32 * NW> tree;
+};
+
+// A row tile of one sequence and key head: its list's key tiles [v0, v1), to the output, or as part
+// `part` to the workspace (-1: all are there).
+template <typename T, int ROWB, int KS, int DT, int NK, int NW, bool TREE>
+__device__ __forceinline__ void chunk_item(const AttnParams& a, ChunkShared<ROWB, NK, NW, TREE>& sm, const SeqView& sq, int b, int h, int tile,
+                                           const TileList<32 * NK>& tl, int v0, int v1, int64_t part) {
+    constexpr int KT = 32 * NK, RM = 32 * NW;
+    constexpr int C = ROWB / 16, RPI = 64 / C, NI = KT / (NW * RPI);   // pieces a row; rows a load; loads a wave
     constexpr uint32_t ALL = (1u << KT / 8) - 1;
     constexpr bool FUSED = ROWB > 256;
     static_assert(NK == (FUSED ? 1 : 2), "a tile's keys by 32");
-    constexpr int NV = FUSED ? 3 : 2;   // value buffers
-    __shared__ __attribute__((aligned(128))) char sm_k[2][KT * ROWB];
-    __shared__ __attribute__((aligned(128))) char sm_v[NV][KT * ROWB];
-    __shared__ std::conditional_t<TREE, TreeRows<RM>, char> sm_tree;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    static_assert(NI * RPI % 8 == 0 && NI * RPI >= 8, "a wave loads whole groups of 8 keys");
+    constexpr int NV = ChunkShared<ROWB, NK, NW, TREE>::NV;
+    auto& sm_k = sm.k;
+    auto& sm_v = sm.v;
+    int thread = threadIdx.x;
+    if constexpr (TREE) asm volatile("" : "+v"(thread));   // (what follows from it is not kept from item to item)
+    const int lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6);
     const int n32 = lane & 31, hh = lane >> 5;
-    const int pair = blockIdx.x, tile = a.row_tiles - 1 - blockIdx.y, split = blockIdx.z;
-    const int b = pair / a.c.kv_heads, h = pair - b * a.c.kv_heads;
-    const SeqView sq = seq_view(a.c, b);
     const int G = a.group, rows = sq.n * G, r0 = tile * RM;
-    if (r0 >= rows) return;
     const int D = a.c.head_dim;
     // Positions of the workgroup's rows.  A tree's row sees no key past the prefix but its
     // own line, and stands at p0 or behind.
     const int gfirst = TREE ? sq.p0 : sq.p0 + r0 / G, glast = sq.p0 + (min(r0 + RM, rows) - 1) / G, gall = TREE ? sq.p0 - 1 : gfirst;
-    const TileList<KT> tl(a.window, a.sinks, gfirst, glast, sq.len);
-    const int v0 = split * a.split_tiles, v1 = a.splits == split + 1 ? tl.n : min(tl.n, v0 + a.split_tiles);
 
     // The wave's rows, and the lane's: its query and its position.
     const int w0 = r0 + wave * 32, r = w0 + n32;
@@ -49,8 +59,8 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
     const int pfirst = TREE ? sq.p0 : sq.p0 + w0 / G, plast = w0 < rows ? sq.p0 + (min(w0 + 32, rows) - 1) / G : -1;
     const int tok = in ? r / G : 0, hd = in ? r - tok * G : 0;
     const int pos = in ? sq.p0 + tok : -1;
-    if constexpr (TREE) {   // (a split of the prefix alone needs none, but for a window)
-        if (a.window > 0 || (v0 < v1 && tl.key(v1 - 1) + KT > sq.p0)) sm_tree.find(a, sq, r0 / G, glast - sq.p0 - r0 / G + 1);
+    if constexpr (TREE) {   // (a share of the prefix alone needs none, but for a window)
+        if (a.window > 0 || (v0 < v1 && tl.key(v1 - 1) + KT > sq.p0)) sm.tree.find(a, sq, r0 / G, glast - sq.p0 - r0 / G + 1);
     }
     u32x4 qf[KS];
     {
@@ -216,7 +226,7 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
         for (int kt = 0; kt < NK; ++kt) {
             scores(sk, kt, s[kt]);
             uint32_t seen = 0;
-            if constexpr (TREE) seen = in ? sm_tree.sees(a, sq.p0, tok - r0 / G, t0 + 32 * kt) : 0;
+            if constexpr (TREE) seen = in ? sm.tree.sees(a, sq.p0, tok - r0 / G, t0 + 32 * kt) : 0;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int j = t0 + 32 * kt + 8 * (i / 4) + 4 * hh + (i & 3);
@@ -256,7 +266,7 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
                         }
                 }
                 __syncthreads();
-                for (int i = threadIdx.x; i < KT * ROWB / 16; i += 256) {
+                for (int i = thread; i < KT * ROWB / 16; i += 64 * NW) {
                     u32x4 x = *(const u32x4*)(sv + 16 * i);
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
@@ -384,8 +394,8 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
     l += __shfl_xor(l, 32);
     if (!in) return;
 
-    if (a.splits > 1) {
-        const int64_t at = (((int64_t)pair * a.row_tiles + tile) * a.splits + split) * RM + (r - r0);
+    if (part >= 0) {
+        const int64_t at = part * RM + (r - r0);
         if (hh == 0) {
             a.part_ml[2 * at] = m;
             a.part_ml[2 * at + 1] = l;
@@ -415,24 +425,130 @@ __global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(Att
         }
 }
 
-template <typename T, bool TREE>
-static void launch_chunk_type(const AttnParams& a, dim3 grid, hipStream_t stream) {
-    const int D = a.c.head_dim;
-    if (D <= 64) hipLaunchKernelGGL((attn_chunk_kernel<T, 128, 4, 2, 2, TREE>), grid, dim3(256), 0, stream, a);
-    else if (D <= 96) hipLaunchKernelGGL((attn_chunk_kernel<T, 256, 6, 3, 2, TREE>), grid, dim3(256), 0, stream, a);
-    else if (D <= 128) hipLaunchKernelGGL((attn_chunk_kernel<T, 256, 8, 4, 2, TREE>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((attn_chunk_kernel<T, 512, 16, 8, 1, TREE>), grid, dim3(256), 0, stream, a);
+template <typename T, int ROWB, int KS, int DT, int NK>
+__global__ __launch_bounds__(256, ROWB > 256 ? 1 : 2) void attn_chunk_kernel(AttnParams a) {
+    constexpr int KT = 32 * NK, RM = kChunkRows;
+    __shared__ ChunkShared<ROWB, NK, 4, false> sm;
+    const int pair = blockIdx.x, tile = a.row_tiles - 1 - blockIdx.y, split = blockIdx.z;
+    const int b = pair / a.c.kv_heads, h = pair - b * a.c.kv_heads;
+    const SeqView sq = seq_view(a.c, b);
+    const int rows = sq.n * a.group, r0 = tile * RM;
+    if (r0 >= rows) return;
+    const TileList<KT> tl(a.window, a.sinks, sq.p0 + r0 / a.group, sq.p0 + (min(r0 + RM, rows) - 1) / a.group, sq.len);
+    const int v0 = split * a.split_tiles, v1 = a.splits == split + 1 ? tl.n : min(tl.n, v0 + a.split_tiles);
+    chunk_item<T, ROWB, KS, DT, NK, 4, false>(a, sm, sq, b, h, tile, tl, v0, v1,
+                                              a.splits > 1 ? ((int64_t)pair * a.row_tiles + tile) * a.splits + split : -1);
 }
 
-template <bool TREE>
-static void launch_chunk(const AttnParams& a, bool bf16, dim3 grid, hipStream_t stream) {
-    if (bf16) launch_chunk_type<Bf16, TREE>(a, grid, stream);
-    else launch_chunk_type<F16, TREE>(a, grid, stream);
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+    return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)x) | (int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
+}
+
+// Trees: a share of the axis (TreeAxis).
+template <typename T, int ROWB, int KS, int DT, int NK, int NW>
+__global__ __launch_bounds__(64 * NW, 2 * (ROWB > 256 ? 1 : 2) / (NW / 2)) void attn_tree_kernel(AttnParams a) {
+    constexpr int KT = 32 * NK, RM = 32 * NW;
+    typedef TreeAxis<KT, RM> Axis;
+    __shared__ ChunkShared<ROWB, NK, NW, true> sm;
+    __shared__ int64_t wsum[NW + 2];   // then where the share starts
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int H = a.c.kv_heads, combos = a.c.batch * a.row_tiles;
+    const int per = (combos + 64 * NW - 1) / (64 * NW), c0 = min(t * per, combos), c1 = min(c0 + per, combos);
+    int64_t mine = 0;
+    for (int c = c0; c < c1; ++c) mine += Axis::combo(a, c);
+    int64_t upto = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int64_t y = __shfl_up(upto, d);
+        if (lane >= d) upto += y;
+    }
+    if (lane == 63) wsum[wave] = upto;
+    __syncthreads();
+    int64_t total = 0, before = upto - mine;
+    for (int w = 0; w < NW; ++w) {
+        before += w < wave ? wsum[w] : 0;
+        total += wsum[w];
+    }
+    total = uniform(total) * H;
+    const int64_t share = max((total + gridDim.x - 1) / gridDim.x, (int64_t)a.split_tiles);
+    int64_t x = blockIdx.x * share;
+    const int64_t end = min(x + share, total);
+    if (x >= end) return;
+    if (x >= before * H && x < (before + mine) * H)
+        for (int c = c0;; ++c) {
+            const int n = Axis::combo(a, c);
+            if (x < (before + n) * H) {
+                wsum[NW] = c;
+                wsum[NW + 1] = before * H;
+                break;
+            }
+            before += n;
+        }
+    __syncthreads();
+    int combo = __builtin_amdgcn_readfirstlane((int)wsum[NW]);
+    int64_t at = uniform(wsum[NW + 1]);
+    while (x < end) {
+        const int b = combo / a.row_tiles, tile = combo - b * a.row_tiles;
+        const SeqView sq = seq_view(a.c, b);
+        const int rows = sq.n * a.group, r0 = tile * RM;
+        if (r0 >= rows) {
+            ++combo;
+            continue;
+        }
+        const TileList<KT> tl(a.window, a.sinks, sq.p0, sq.p0 + (min(r0 + RM, rows) - 1) / a.group, sq.len);
+        const int n = max(tl.n, 1), axis = Axis::length(tl.n);
+        if (x >= at + (int64_t)axis * H) {
+            at += (int64_t)axis * H;
+            ++combo;
+            continue;
+        }
+        const int h = (int)((x - at) / axis);
+        const int64_t item = at + (int64_t)h * axis;
+        const int k0 = (int)(x - item), k1 = (int)min((int64_t)n, end - item);
+        x = min(item + axis, end);
+        if (k0 >= n) continue;
+        const bool whole = k0 == 0 && k1 == n;
+        if (k0 == 0 && t == 0)
+            a.item_parts[combo * H + h] = make_int2(blockIdx.x, whole ? 0 : (int)((item + n - 1) / share) - (int)blockIdx.x + 1);
+        chunk_item<T, ROWB, KS, DT, NK, NW, true>(a, sm, sq, b, h, tile, tl, k0, min(k1, tl.n),
+                                                  whole ? -1 : 2 * (int64_t)blockIdx.x + (k0 == 0 ? 1 : 0));
+        __syncthreads();   // its tiles are read
+    }
+}
+
+template <typename T>
+static void launch_chunk_type(const AttnParams& a, dim3 grid, hipStream_t stream) {
+    const int D = a.c.head_dim;
+    if (D <= 64) hipLaunchKernelGGL((attn_chunk_kernel<T, 128, 4, 2, 2>), grid, dim3(256), 0, stream, a);
+    else if (D <= 96) hipLaunchKernelGGL((attn_chunk_kernel<T, 256, 6, 3, 2>), grid, dim3(256), 0, stream, a);
+    else if (D <= 128) hipLaunchKernelGGL((attn_chunk_kernel<T, 256, 8, 4, 2>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((attn_chunk_kernel<T, 512, 16, 8, 1>), grid, dim3(256), 0, stream, a);
 }
 
 void launch_attn_chunk(const AttnParams& a, bool bf16, dim3 grid, hipStream_t stream) {
-    if (a.parents) launch_chunk<true>(a, bf16, grid, stream);
-    else launch_chunk<false>(a, bf16, grid, stream);
+    if (bf16) launch_chunk_type<Bf16>(a, grid, stream);
+    else launch_chunk_type<F16>(a, grid, stream);
+}
+
+template <typename T>
+static void launch_tree_type(const AttnParams& a, int rows, int workgroups, hipStream_t stream) {
+    const int D = a.c.head_dim;
+    const dim3 grid(workgroups);
+    if (D > 128) hipLaunchKernelGGL((attn_tree_kernel<T, 512, 16, 8, 1, 4>), grid, dim3(256), 0, stream, a);
+    else if (rows == 128) {
+        if (D <= 64) hipLaunchKernelGGL((attn_tree_kernel<T, 128, 4, 2, 2, 4>), grid, dim3(256), 0, stream, a);
+        else if (D <= 96) hipLaunchKernelGGL((attn_tree_kernel<T, 256, 6, 3, 2, 4>), grid, dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL((attn_tree_kernel<T, 256, 8, 4, 2, 4>), grid, dim3(256), 0, stream, a);
+    } else {
+        if (D <= 64) hipLaunchKernelGGL((attn_tree_kernel<T, 128, 4, 2, 2, 8>), grid, dim3(512), 0, stream, a);
+        else if (D <= 96) hipLaunchKernelGGL((attn_tree_kernel<T, 256, 6, 3, 2, 8>), grid, dim3(512), 0, stream, a);
+        else hipLaunchKernelGGL((attn_tree_kernel<T, 256, 8, 4, 2, 8>), grid, dim3(512), 0, stream, a);
+    }
+}
+
+void launch_attn_chunk_tree(const AttnParams& a, bool bf16, int rows, int workgroups, hipStream_t stream) {
+    if (bf16) launch_tree_type<Bf16>(a, rows, workgroups, stream);
+    else launch_tree_type<F16>(a, rows, workgroups, stream);
 }
 
 }  // namespace tms

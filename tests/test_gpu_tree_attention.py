@@ -76,10 +76,8 @@ def test_trees(dt, kv, q, H, G, D):
 def test_kinds(kind, q):
     bt = TreeBatch([150, 131], q, H=1, G=2, D=64, kind=kind, seed=3)
     check(bt)
-    if kind == "chain":   # as paged_attention
-        out, lse = bt.attend()
-        o, l = Batch.attend(bt)
-        assert torch.equal(out, o) and torch.equal(lse, l)
+    if kind == "chain":   # what paged_attention sees too, within the same bounds
+        check(bt, got=Batch.attend(bt))
 
 
 @pytest.mark.parametrize("window, sinks", [(1, 0), (2, 0), (3, 5), (16, 0), (40, 4), (64, 130), (1000, 3)])
@@ -192,3 +190,13 @@ def test_many_sequences_of_any_lengths():
     check(TreeBatch(kv, q, H=2, G=2, D=64, seed=12))
     q[7], kv[7], q[9] = 0, 5, 0
     check(TreeBatch(kv, q, H=1, G=1, D=64, seed=13))
+
+
+@pytest.mark.parametrize("q", [[6, 2, 1], [40, 60, 33]])
+def test_positions_past_max_kv(q):
+    """max_kv sizes workspaces and grids; positions past it are attended all the same."""
+    for told in (1, 100, 2000):
+        bt = TreeBatch([3000, 90, 700], q, H=1, G=2, D=64, seed=14)
+        bt.max_kv = told
+        check(bt)
+        check(bt, window=1500, sinks=4)
