@@ -16,7 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtmsample_hip.so")
-SOURCES = ["tms_sample.hip", "tms_topp.hip", "tms_wide.hip", "tms_sparse.hip", "tms_rows.hip", "tms_hist.hip", "tms_chain.hip", "tms_spec.hip", "tms_debug.hip", "tms_attn.hip", "tms_attn_chunk.hip", "tms_scores.hip", "tms_kv.hip", "tms_adjust.hip", "tms_rotary.hip", "tms_verify_tree.hip", "tms_compact.hip", "tms_history.cpp", "tms_grammar.cpp", "tms_filter.cpp"]
+SOURCES = ["tms_sample.hip", "tms_topp.hip", "tms_wide.hip", "tms_sparse.hip", "tms_rows.hip", "tms_hist.hip", "tms_chain.hip", "tms_spec.hip", "tms_debug.hip", "tms_attn.hip", "tms_attn_chunk.hip", "tms_attn_tree.hip", "tms_scores.hip", "tms_kv.hip", "tms_adjust.hip", "tms_rotary.hip", "tms_verify_tree.hip", "tms_compact.hip", "tms_history.cpp", "tms_grammar.cpp", "tms_filter.cpp"]
 
 # -ffp-contract=off keeps every a*b+c as two rounded operations, so the
 # device arithmetic matches the host checker bit for bit.  Packed-FP32 ops
@@ -40,9 +40,11 @@ HIPCC_FLAGS = [
 # result is broadcast at once, waiting out the round trip there.  The
 # whole-vocabulary kernel is many phases in one loop: constants hoisted out of
 # it would live through every phase, in scratch (44 bytes a lane; none without).
-# Its first four argument words come in registers.
+# Its first four argument words come in registers.  The tree kernel is a loop over
+# items around a tile's registers, and the same constants do not fit there (8 to 32 bytes a lane).
 FILE_FLAGS = {
     "tms_wide.hip": ["-mllvm", "-amdgpu-atomic-optimizer-strategy=None"],
+    "tms_attn_tree.hip": ["-mllvm", "-disable-machine-licm"],
     "tms_topp.hip": ["-mllvm", "-disable-machine-licm", "-mllvm", "-amdgpu-kernarg-preload-count=4"],
 }
 
@@ -105,7 +107,7 @@ def _run(cmd: list, verbose: bool) -> str:
 # hold outputs or keys in registers (attention of 128-dimensional heads took
 # 775 us with 88 bytes a lane, 526 with none).
 NO_SCRATCH = ("tms_wide.hip", "tms_spec.hip", "tms_sample.hip", "tms_sparse.hip", "tms_rows.hip", "tms_topp.hip",
-              "tms_attn.hip", "tms_attn_chunk.hip", "tms_scores.hip", "tms_kv.hip", "tms_adjust.hip", "tms_rotary.hip",
+              "tms_attn.hip", "tms_attn_chunk.hip", "tms_attn_tree.hip", "tms_scores.hip", "tms_kv.hip", "tms_adjust.hip", "tms_rotary.hip",
               "tms_verify_tree.hip", "tms_compact.hip")
 
 

@@ -214,6 +214,13 @@ struct TreeAxis {
     }
 };
 
+// A barrier for what goes through LDS alone: loads in flight stay so.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // Trees: what the tokens of a group of rows see of the new tokens, a bit each, found by
 // climbing from node to parent in LDS (some 100 cycles a step), and their depths.  With a
 // window a node's own line is cut by it here.
@@ -224,24 +231,41 @@ struct TreeRows {
     uint32_t seen[TOKENS][kTreeWords + 1];
     int depth[TOKENS];
 
-    // Of tokens [tok0, tok0 + n) of the sequence; by all threads of the workgroup.
-    __device__ __forceinline__ void find(const AttnParams& a, const SeqView& sq, int tok0, int n) {
-        const int t = threadIdx.x;
-        for (int i = t; i < min(tok0 + n, TMS_TREE_MAX_NODES); i += blockDim.x) {
-            const int p = a.parents[sq.q0 + i];
-            up[i] = (int16_t)(p >= 0 && p < i ? p : -1);
+    // The parents of nodes below `end`, a thread's in registers: on the way with the queries, and in LDS
+    // while the first keys are (8 sequences' nodes over 508 positions: 15 us with all of it before the keys).
+    template <int NT>
+    struct Parents {
+        int up[TMS_TREE_MAX_NODES / NT];
+        __device__ __forceinline__ void fetch(const AttnParams& a, const SeqView& sq, int end) {
+#pragma unroll
+            for (int k = 0; k < TMS_TREE_MAX_NODES / NT; ++k) {
+                const int i = k * NT + (int)threadIdx.x;
+                up[k] = i < end ? a.parents[sq.q0 + i] : -1;
+            }
         }
-        __syncthreads();
-        for (int i = t; i < n; i += blockDim.x) {
+    };
+
+    // What tokens [tok0, tok0 + n) of the sequence see; by all threads of the workgroup.
+    template <int NT>
+    __device__ __forceinline__ void find(const AttnParams& a, const SeqView& sq, int tok0, int n, const Parents<NT>& p) {
+        const int t = threadIdx.x;
+#pragma unroll
+        for (int k = 0; k < TMS_TREE_MAX_NODES / NT; ++k) {
+            const int i = k * NT + t;
+            up[i] = (int16_t)(p.up[k] >= 0 && p.up[k] < i ? p.up[k] : -1);
+        }
+        lds_barrier();
+        for (int i = t; i < n; i += NT) {
             for (int w = 0; w <= kTreeWords; ++w) seen[i][w] = 0;
             int far = 0;
-            for (int x = up[tok0 + i]; x >= 0; x = up[x]) ++far;
+            if (a.window > 0)
+                for (int x = up[tok0 + i]; x >= 0; x = up[x]) ++far;
             depth[i] = far;
             int back = 0;
             for (int x = tok0 + i; x >= 0; x = up[x], ++back)
                 if (a.window <= 0 || back < a.window || sq.p0 + far - back < a.sinks) seen[i][x >> 5] |= 1u << (x & 31);
         }
-        __syncthreads();
+        lds_barrier();
     }
 
     // Bit e: token `i` of these sees key t0 + e.

@@ -182,8 +182,12 @@ __global__ __launch_bounds__(64 * NW, ROWB > 256 ? 1 : 2) void attn_rows_kernel(
         const bool in = r < rows;
         const int tok = in ? r / G : 0, hd = in ? r - tok * G : 0;
         const int pos = in ? sq.p0 + tok : -1;
-        if constexpr (TREE) {   // (a share of the prefix alone needs none, but for a window)
-            if (a.window > 0 || (k0 < kend && tl.key(kend - 1) + KT > sq.p0)) sm_tree.find(a, sq, r0 / G, (r0 + nr - 1) / G - r0 / G + 1);
+        // (a share of the prefix alone needs none of the tree, but for a window)
+        const int last = (r0 + nr - 1) / G;
+        const bool lines = TREE && (a.window > 0 || (k0 < kend && tl.key(kend - 1) + KT > sq.p0));
+        [[maybe_unused]] typename TreeRows<RM>::template Parents<64 * NW> parents;
+        if constexpr (TREE) {
+            if (lines) parents.fetch(a, sq, last + 1);
         }
         u32x4 qf[KS];
         {
@@ -220,7 +224,11 @@ __global__ __launch_bounds__(64 * NW, ROWB > 256 ? 1 : 2) void attn_rows_kernel(
             for (int g = 0; g < 4; ++g) {
                 const int j = t0 + 8 * g;
                 const uint32_t p = max(page[g], 0), sl = page[g] < 0 ? 0 : j & a.c.smask;
-                const u32x4 res = slots_rsrc(base + p * pstride + (uint64_t)sl * slot, page[g] < 0 ? -1 : min(8, sq.len - j) - 1, slot, 2 * D);
+                u32x4 res = slots_rsrc(base + p * pstride + (uint64_t)sl * slot, page[g] < 0 ? -1 : min(8, sq.len - j) - 1, slot, 2 * D);
+                if constexpr (TREE) {   // (the compiler had it in vector registers, where the load does not take it)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) res[w] = __builtin_amdgcn_readfirstlane(res[w]);
+                }
 #pragma unroll
                 for (int i = g * 8 / RPI; i < (g + 1) * 8 / RPI; ++i) load_lds16(res, off[i], to + i * 1024);
             }
@@ -240,8 +248,11 @@ __global__ __launch_bounds__(64 * NW, ROWB > 256 ? 1 : 2) void attn_rows_kernel(
             __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): what went before is not counted below
             load(v, kbase, a.c.kp, kslot, koff, lds0);
             load(v, vbase, a.c.vp, vslot, voff, lds0 + KT * ROWB);
-            if (v + NW < kend) entries(v + NW);
         }
+        if constexpr (TREE) {
+            if (lines) sm_tree.find(a, sq, r0 / G, last - r0 / G + 1, parents);
+        }
+        if (v + NW < kend) entries(v + NW);
         for (; v < kend; v += NW) {
             const bool more = v + NW < kend;
             const int t0 = tl.key(v);

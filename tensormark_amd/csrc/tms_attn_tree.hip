@@ -1,0 +1,104 @@
+// tms_attn_tree.hip -- attention of drafted trees over the paged cache for many rows a key head
+// (tms_tree_attention); up to 32 rows take the rows kernel of tms_attn.hip.
+#include "tms_attn_chunk.h"
+
+namespace tms {
+
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+    return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)x) | (int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
+}
+
+// Trees: a share of the axis (TreeAxis).
+template <typename T, int ROWB, int KS, int DT, int NK, int NW>
+__global__ __launch_bounds__(64 * NW, 2 * (ROWB > 256 ? 1 : 2) / (NW / 2)) void attn_tree_kernel(AttnParams a) {
+    constexpr int KT = 32 * NK, RM = 32 * NW;
+    typedef TreeAxis<KT, RM> Axis;
+    __shared__ ChunkShared<ROWB, NK, NW, true> sm;
+    __shared__ int64_t wsum[NW + 2];   // then where the share starts
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int H = a.c.kv_heads, combos = a.c.batch * a.row_tiles;
+    const int per = (combos + 64 * NW - 1) / (64 * NW), c0 = min(t * per, combos), c1 = min(c0 + per, combos);
+    int64_t mine = 0;
+    for (int c = c0; c < c1; ++c) mine += Axis::combo(a, c);
+    int64_t upto = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int64_t y = __shfl_up(upto, d);
+        if (lane >= d) upto += y;
+    }
+    if (lane == 63) wsum[wave] = upto;
+    __syncthreads();
+    int64_t total = 0, before = upto - mine;
+    for (int w = 0; w < NW; ++w) {
+        before += w < wave ? wsum[w] : 0;
+        total += wsum[w];
+    }
+    total = uniform(total) * H;
+    const int64_t share = max((total + gridDim.x - 1) / gridDim.x, (int64_t)a.split_tiles);
+    int64_t x = blockIdx.x * share;
+    const int64_t end = min(x + share, total);
+    if (x >= end) return;
+    if (x >= before * H && x < (before + mine) * H)
+        for (int c = c0;; ++c) {
+            const int n = Axis::combo(a, c);
+            if (x < (before + n) * H) {
+                wsum[NW] = c;
+                wsum[NW + 1] = before * H;
+                break;
+            }
+            before += n;
+        }
+    __syncthreads();
+    int combo = __builtin_amdgcn_readfirstlane((int)wsum[NW]);
+    int64_t at = uniform(wsum[NW + 1]);
+    while (x < end) {
+        const int b = combo / a.row_tiles, tile = combo - b * a.row_tiles;
+        const SeqView sq = seq_view(a.c, b);
+        const int rows = sq.n * a.group, r0 = tile * RM;
+        if (r0 >= rows) {
+            ++combo;
+            continue;
+        }
+        const TileList<KT> tl(a.window, a.sinks, sq.p0, sq.p0 + (min(r0 + RM, rows) - 1) / a.group, sq.len);
+        const int n = max(tl.n, 1), axis = Axis::length(tl.n);
+        if (x >= at + (int64_t)axis * H) {
+            at += (int64_t)axis * H;
+            ++combo;
+            continue;
+        }
+        const int h = (int)((x - at) / axis);
+        const int64_t item = at + (int64_t)h * axis;
+        const int k0 = (int)(x - item), k1 = (int)min((int64_t)n, end - item);
+        x = min(item + axis, end);
+        if (k0 >= n) continue;
+        const bool whole = k0 == 0 && k1 == n;
+        if (k0 == 0 && t == 0)
+            a.item_parts[combo * H + h] = make_int2(blockIdx.x, whole ? 0 : (int)((item + n - 1) / share) - (int)blockIdx.x + 1);
+        chunk_item<T, ROWB, KS, DT, NK, NW, true>(a, sm, sq, b, h, tile, tl, k0, min(k1, tl.n),
+                                                  whole ? -1 : 2 * (int64_t)blockIdx.x + (k0 == 0 ? 1 : 0));
+        __syncthreads();   // its tiles are read
+    }
+}
+
+template <typename T>
+static void launch_tree_type(const AttnParams& a, int rows, int workgroups, hipStream_t stream) {
+    const int D = a.c.head_dim;
+    const dim3 grid(workgroups);
+    if (D > 128) hipLaunchKernelGGL((attn_tree_kernel<T, 512, 16, 8, 1, 4>), grid, dim3(256), 0, stream, a);
+    else if (rows == 128) {
+        if (D <= 64) hipLaunchKernelGGL((attn_tree_kernel<T, 128, 4, 2, 2, 4>), grid, dim3(256), 0, stream, a);
+        else if (D <= 96) hipLaunchKernelGGL((attn_tree_kernel<T, 256, 6, 3, 2, 4>), grid, dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL((attn_tree_kernel<T, 256, 8, 4, 2, 4>), grid, dim3(256), 0, stream, a);
+    } else {
+        if (D <= 64) hipLaunchKernelGGL((attn_tree_kernel<T, 128, 4, 2, 2, 8>), grid, dim3(512), 0, stream, a);
+        else if (D <= 96) hipLaunchKernelGGL((attn_tree_kernel<T, 256, 6, 3, 2, 8>), grid, dim3(512), 0, stream, a);
+        else hipLaunchKernelGGL((attn_tree_kernel<T, 256, 8, 4, 2, 8>), grid, dim3(512), 0, stream, a);
+    }
+}
+
+void launch_attn_chunk_tree(const AttnParams& a, bool bf16, int rows, int workgroups, hipStream_t stream) {
+    if (bf16) launch_tree_type<Bf16>(a, rows, workgroups, stream);
+    else launch_tree_type<F16>(a, rows, workgroups, stream);
+}
+
+}  // namespace tms
