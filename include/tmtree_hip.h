@@ -132,7 +132,8 @@ typedef struct tms_verify_tree_args {
     const int32_t* q_start;   /* device, [batch + 1] */
     const double* uniforms;   /* device, [tokens], in [0, 1) */
     int32_t* path;            /* device, [batch][max_q]: the nodes of the walk from 0 on, -1 past
-                                 them */
+                                 them; like kept and token it shares no memory with what the call
+                                 reads */
     int32_t* kept;            /* device, [batch]: how many they are (the accepted drafts and node 0; 0
                                  without a tree) */
     int32_t* token;           /* device, [batch] */
@@ -151,12 +152,12 @@ int tms_debug_verify_polls(int polls);
 /*
  * Keep chosen entries of each sequence: entry base + kept[b][i] (key, value and
  * score, of all heads) goes to position base + i, i < n_kept[b], and new_len[b] is
- * base + n_kept[b].  base is p0 with cache->q_start (`kept` then names nodes: the
+ * base + n_kept[b], 0 at least.  base is p0 with cache->q_start (`kept` then names nodes: the
  * path of a tms_verify_tree), and 0 without.  In place, where kept[i] >= i for every i, the
  * result is as if all entries were read before any is written.  With dst_tables the entries go to the pages of
  * that table instead (of the same pools, and of none that the call reads), from any list.
  * Not copied are entries to or from unmapped pages, with kept[i] outside the sequence, and in
- * place those with kept[i] < i.
+ * place those with kept[i] < i.  A page that two sequences share is written by both, in no order.
  * n_kept is taken as at most max_kept, and in place as at most the sequence's entries from base on.
  * Of the cache's fields `tokens`, `max_q` and `max_kv` are not used.
  */
@@ -164,7 +165,8 @@ typedef struct tms_compact_args {
     const int32_t* kept;      /* device, [batch][kept_stride] */
     int64_t kept_stride;      /* >= max_kept */
     const int32_t* n_kept;    /* device, [batch] */
-    const int32_t* dst_tables; /* device, [batch][dst_table_stride], nullable: in place */
+    const int32_t* dst_tables; /* device, [batch][dst_table_stride], nullable: in place; not
+                                 the cache's tables */
     int64_t dst_table_stride;
     int32_t* new_len;         /* device, [batch], nullable; none of the call's inputs */
     int32_t max_kept;         /* 0..TMS_COMPACT_MAX_KEPT */

@@ -194,7 +194,7 @@ extern "C" int tms_kv_compact(const tms_cache* cache, const tms_compact_args* ar
     if (args->max_kept > TMS_COMPACT_MAX_KEPT) return TMS_ERR_CAPACITY;
     if (cache->batch == 0) return TMS_OK;
     if (!args->n_kept || (args->max_kept > 0 && !args->kept) || args->kept_stride < args->max_kept) return TMS_ERR_INVALID_ARG;
-    if (args->dst_tables && args->dst_table_stride < 1) return TMS_ERR_INVALID_ARG;
+    if (args->dst_tables && (args->dst_table_stride < 1 || args->dst_tables == cache->tables)) return TMS_ERR_INVALID_ARG;
     if (args->new_len && (args->new_len == cache->kv_len || args->new_len == args->n_kept || args->new_len == args->kept))
         return TMS_ERR_INVALID_ARG;
     CompactParams a{};

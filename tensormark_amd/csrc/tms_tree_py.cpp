@@ -16,6 +16,15 @@ static void head_strides(const Tensor& t, int64_t* stride) {
     for (int i = 0; i < 2; ++i) stride[i] = t.size(i) > 1 ? t.stride(i) : 0;
 }
 
+// What a call writes shares no memory with what it reads, as far as their strides tell.
+static void want_separate(const Tensor& out, std::initializer_list<const Tensor*> others, const char* what) {
+    for (const Tensor* t : others)
+        if (t && t->numel() && out.numel()) {
+            const at::MemOverlapStatus s = at::get_overlap_status(out, *t);
+            want(s != at::MemOverlapStatus::Partial && s != at::MemOverlapStatus::Full, what);
+        }
+}
+
 static Tensor rotary(const Tensor& x, const Tensor& positions, const Tensor& freqs, bool interleaved, double scale, const MaybeTensor& out_,
                      int64_t stream) {
     want_no_gradient({&x, &freqs, of(out_)});
@@ -71,10 +80,7 @@ static MaybeTensor kv_append_rotary(const MaybeTensor& q, const Tensor& k_new, c
         rows(*out, k, a.out_stride, "out: like q");
         if (out_) {
             want_apart(*out, *q);
-            for (const Tensor* t : {&k_new, &v_new}) {
-                const at::MemOverlapStatus s = at::get_overlap_status(*out, *t);
-                want(s != at::MemOverlapStatus::Partial && s != at::MemOverlapStatus::Full, "out: overlaps k_new or v_new");
-            }
+            want_separate(*out, {&k_new, &v_new}, "out: shares memory with k_new or v_new");
         }
         a.q = q->const_data_ptr();
         a.out = out->data_ptr();
@@ -172,6 +178,11 @@ static std::tuple<Tensor, Tensor, Tensor> verify_tree(const Tensor& target, cons
     a.path = const_cast<int32_t*>(ints(path, {B, max_q}, "path", device));
     a.kept = const_cast<int32_t*>(ints(kept, {B}, "kept", device));
     a.token = const_cast<int32_t*>(ints(token, {B}, "token", device));
+    for (const MaybeTensor* t : {&path_, &kept_, &token_})
+        if (*t) want_separate(**t, {&target, &tokens, &parents, &q_start, &uniforms, of(draft)}, "path, kept, token: share memory with what the call reads");
+    const char* apart = "path, kept, token: share memory";
+    if (path_) want_separate(path, {&kept, &token}, apart);
+    if (kept_) want_separate(kept, {&token}, apart);
     const int64_t need = tms_verify_tree_workspace(&a);
     if (need < 0) check((int)need, "tms_verify_tree");
     Tensor workspace;
@@ -211,11 +222,7 @@ static Tensor kv_compact(const Tensor& k, const Tensor& v, const Tensor& tables,
     const Tensor new_len = new_len_ ? *new_len_ : at::empty({B}, tables.options());
     a.new_len = const_cast<int32_t*>(ints(new_len, {B}, "new_len", device));
     if (new_len_)
-        for (const Tensor* t : {&kv_len, &n_kept, &kept, &tables, of(q_start), of(dst_tables)})
-            if (t) {
-                const at::MemOverlapStatus s = at::get_overlap_status(new_len, *t);
-                want(s != at::MemOverlapStatus::Partial && s != at::MemOverlapStatus::Full, "new_len: shares memory with what the call reads");
-            }
+        want_separate(new_len, {&kv_len, &n_kept, &kept, &tables, of(q_start), of(dst_tables)}, "new_len: shares memory with what the call reads");
     check(tms_kv_compact(&c, &a, stream_of(stream)), "tms_kv_compact");
     written(k);
     written(v);

@@ -200,3 +200,20 @@ def test_positions_past_max_kv(q):
         bt.max_kv = told
         check(bt)
         check(bt, window=1500, sinks=4)
+
+
+@pytest.mark.parametrize("q", [[6, 5], [40, 33]])
+def test_lengths_past_the_table(q):
+    """Positions past the table do not exist: a tree that lies there partly or wholly."""
+    bt = TreeBatch([70, 80], q, H=1, G=2, D=64, seed=15)
+    cap = bt.host.shape[1] * bt.page
+    for b, past in ((0, 3), (1, 200)):
+        bt.kv[b] = cap + past
+        bt.kv_len[b] = bt.kv[b]
+        grow = bt.kv[b] - bt.keys[b].shape[0]
+        for t in (bt.keys, bt.values):
+            t[b] = torch.cat([t[b], torch.zeros(grow, 1, 64, dtype=BF)])
+    bt.k.nan_to_num_(0.0)   # (slots of the last pages that hold positions now)
+    bt.v.nan_to_num_(0.0)
+    bt.host = np.concatenate([bt.host, np.full((2, 40), -1, np.int32)], 1)   # (the reference's view of what is not there)
+    check(bt)

@@ -93,7 +93,7 @@ APP = [dict(k_new=None), dict(v_new=P + 4), dict(q=None), dict(out=None), dict(q
 VER = [dict(target=None), dict(target=P + 2), dict(draft=P + 1), dict(target_stride=999), dict(draft_stride=10), dict(dtype=9), dict(vocab=0),
        dict(batch=-1), dict(tokens=-1), dict(max_q=-1), dict(reserved=1), dict(draft_tokens=None), dict(parents=None), dict(q_start=None),
        dict(uniforms=None), dict(uniforms=P + 4), dict(path=None), dict(kept=None), dict(token=None)]
-COM = [dict(kept=None), dict(n_kept=None), dict(kept_stride=7), dict(max_kept=-1), dict(reserved=1), dict(dst_tables=P, dst_table_stride=0),
+COM = [dict(kept=None), dict(n_kept=None), dict(kept_stride=7), dict(max_kept=-1), dict(reserved=1), dict(dst_tables=P + 64, dst_table_stride=0), dict(dst_tables=P, dst_table_stride=4),
        dict(new_len=P), dict(new_len=P, n_kept=P + 64)]   # (kv_len and kept are at P)
 
 
@@ -251,6 +251,19 @@ def test_python_calls_refuse_what_does_not_fit():
     x["new_len"] = x["kv_len"]
     with pytest.raises(ValueError):
         calls(x)["compact"]()
+    for name in ("n_path", "token"):
+        x = some("cuda:0")
+        x[name] = x["ids"][:1]
+        with pytest.raises(ValueError):
+            calls(x)["verify"]()
+    x = some("cuda:0")
+    x["token"] = x["path"][0, 1:]
+    with pytest.raises(ValueError):
+        calls(x)["verify"]()
+    x = some("cuda:0")
+    x["out"] = x["q"] = x["kn"]
+    with pytest.raises(ValueError):
+        calls(x)["append"]()
     x = some("cuda:0")
     x["freqs"] = torch.zeros(33, device="cuda:0")   # more than the head has
     with pytest.raises(RuntimeError):
