@@ -94,7 +94,8 @@ int tms_kv_append_rotary(const tms_cache* cache, const tms_append_rotary_args* a
  * ancestors and itself (on mapped pages).  With window > 0 it sees those of them whose
  * position in the text is above its own - window or below `sinks`.  parents: device,
  * [tokens].  Everything else, the workspace too, is as there, with its own call for the
- * workspace's size.
+ * workspace's size; batch times kv_heads times tiles of 128 rows (32, where a page's stride or slots
+ * span 2^32 bytes) may be up to 2^30.
  */
 int64_t tms_tree_attention_workspace(const tms_cache* cache, const tms_attention_args* args);
 int tms_tree_attention(const tms_cache* cache, const tms_attention_args* args, const int32_t* parents, hipStream_t stream);

@@ -593,25 +593,36 @@ static AttnPlan plan_attention(const tms_cache* c, const tms_attention_args* a, 
     const int rows = p.rows = min(c->max_q, c->tokens) * (a->q_heads / c->kv_heads);
     p.chunk = rows > kShareRows && short_strides(c, c->k_stride) && short_strides(c, c->v_stride);
     p.rm = p.chunk ? kChunkRows : kShareRows;
-    if (p.chunk && tree && rows > kChunkRows && c->head_dim <= 128) p.rm = 2 * kChunkRows;   // (keys read once for all)
+    const bool wide = p.chunk && tree && rows > kChunkRows && c->head_dim <= 128;   // keys read once for 256 rows
+    if (wide) p.rm = 2 * kChunkRows;
     p.row_tiles = (rows + p.rm - 1) / p.rm;
     int64_t keys = min(c->max_kv, kMaxLen);
     if (a->window > 0) keys = std::min<int64_t>(keys, (int64_t)a->window + (tree ? c->max_q : p.rm) + a->sinks + 128);
     const int64_t items = (int64_t)c->batch * c->kv_heads * p.row_tiles;
     int64_t parts;
-    p.fits = (p.chunk && !tree) || items <= INT32_MAX;
+    p.fits = (p.chunk && !tree) || items <= (tree ? INT32_MAX / 2 : INT32_MAX);
+    const int part_rows = p.rm;
     p.splits = p.shares = 0;
     p.item_bytes = 0;
     if (p.chunk && tree) {
-        // As many workgroups as the card holds at once, with 4 tiles each at least.
+        // Shares for as many workgroups as the card holds at once, with 4 tiles each at least; short
+        // sequences whole, and the longer ones of many items, which fill the card without shares (25 nodes, 4 heads
+        // a key head: 1 sequence of 760 20 us in shares and 24 whole, 16 of 760 28 and 25, 64 of 2000 115 and 108).
+        // The workspace is that of shares in either case past 8 tiles: it does not shrink with more items.
         const int kt = chunk_keys(c->head_dim);
         const int64_t tiles = std::max<int64_t>((keys + kt - 1) / kt, 1);
         p.split_tiles = kTreeLeastShare;
-        p.shares = (int)std::min<int64_t>(c->head_dim > 128 || p.rm > kChunkRows ? 256 : 512, (tiles + kTreeItemCost) * items / kTreeLeastShare + 1);
-        p.join = true;
-        parts = 2 * (int64_t)p.shares;
+        p.shares = (int)std::min<int64_t>(c->head_dim > 128 || wide ? 256 : 512, (tiles + kTreeItemCost) * items / kTreeLeastShare + 1);
+        parts = tiles > 8 ? 2 * (int64_t)p.shares : 0;
         p.most_parts = (int)std::min<int64_t>(tiles / kTreeLeastShare + 2, p.shares);
-        p.item_bytes = (size_t)(items * 8 + 15) / 16 * 16;
+        p.item_bytes = tiles > 8 ? (size_t)(items * 8 + 15) / 16 * 16 : 0;
+        p.join = tiles > std::min<int64_t>(8 + items / 16, 40);
+        if (!p.join) {
+            p.split_tiles = 0;
+            p.rm = kChunkRows;   // (less latency: 64 nodes over 130 to 1000 of 16 sequences 17 to 36 us, 20 to 42 with 256)
+            p.row_tiles = (rows + p.rm - 1) / p.rm;
+            p.shares = (int)((int64_t)c->batch * c->kv_heads * p.row_tiles);
+        }
     } else if (p.chunk) {
         // Workgroups enough for two a CU, with 4 tiles each at least.
         const int kt = chunk_keys(c->head_dim);
@@ -632,8 +643,8 @@ static AttnPlan plan_attention(const tms_cache* c, const tms_attention_args* a, 
         p.most_parts = (int)std::min<int64_t>(tiles / kLeastShare + 2, p.shares);
         p.item_bytes = p.join ? (size_t)(items * 8 + 15) / 16 * 16 : 0;
     }
-    p.o_bytes = (size_t)parts * p.rm * c->head_dim * 4;
-    p.ml_bytes = (size_t)parts * p.rm * 8;
+    p.o_bytes = (size_t)parts * part_rows * c->head_dim * 4;
+    p.ml_bytes = (size_t)parts * part_rows * 8;
     return p;
 }
 

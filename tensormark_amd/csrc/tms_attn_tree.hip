@@ -17,65 +17,77 @@ __global__ __launch_bounds__(64 * NW, 2 * (ROWB > 256 ? 1 : 2) / (NW / 2)) void 
     __shared__ int64_t wsum[NW + 2];   // then where the share starts
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int H = a.c.kv_heads, combos = a.c.batch * a.row_tiles;
-    const int per = (combos + 64 * NW - 1) / (64 * NW), c0 = min(t * per, combos), c1 = min(c0 + per, combos);
-    int64_t mine = 0;
-    for (int c = c0; c < c1; ++c) mine += Axis::combo(a, c);
-    int64_t upto = mine;
+    // The share: [x, end) of the axis, which starts in `combo` at `at`.  Without shares, an item a workgroup.
+    int64_t share = 0, x = 0, end = 1, at = 0;
+    int combo = blockIdx.x / H;
+    if (a.split_tiles > 0) {
+        const int per = (combos + 64 * NW - 1) / (64 * NW), c0 = min(t * per, combos), c1 = min(c0 + per, combos);
+        int64_t mine = 0;
+        for (int c = c0; c < c1; ++c) mine += Axis::combo(a, c);
+        int64_t upto = mine;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int64_t y = __shfl_up(upto, d);
-        if (lane >= d) upto += y;
-    }
-    if (lane == 63) wsum[wave] = upto;
-    __syncthreads();
-    int64_t total = 0, before = upto - mine;
-    for (int w = 0; w < NW; ++w) {
-        before += w < wave ? wsum[w] : 0;
-        total += wsum[w];
-    }
-    total = uniform(total) * H;
-    const int64_t share = max((total + gridDim.x - 1) / gridDim.x, (int64_t)a.split_tiles);
-    int64_t x = blockIdx.x * share;
-    const int64_t end = min(x + share, total);
-    if (x >= end) return;
-    if (x >= before * H && x < (before + mine) * H)
-        for (int c = c0;; ++c) {
-            const int n = Axis::combo(a, c);
-            if (x < (before + n) * H) {
-                wsum[NW] = c;
-                wsum[NW + 1] = before * H;
-                break;
-            }
-            before += n;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int64_t y = __shfl_up(upto, d);
+            if (lane >= d) upto += y;
         }
-    __syncthreads();
-    int combo = __builtin_amdgcn_readfirstlane((int)wsum[NW]);
-    int64_t at = uniform(wsum[NW + 1]);
+        if (lane == 63) wsum[wave] = upto;
+        __syncthreads();
+        int64_t total = 0, before = upto - mine;
+        for (int w = 0; w < NW; ++w) {
+            before += w < wave ? wsum[w] : 0;
+            total += wsum[w];
+        }
+        total = uniform(total) * H;
+        share = max((total + gridDim.x - 1) / gridDim.x, (int64_t)a.split_tiles);
+        x = blockIdx.x * share;
+        end = min(x + share, total);
+        if (x >= end) return;
+        if (x >= before * H && x < (before + mine) * H)
+            for (int c = c0;; ++c) {
+                const int n = Axis::combo(a, c);
+                if (x < (before + n) * H) {
+                    wsum[NW] = c;
+                    wsum[NW + 1] = before * H;
+                    break;
+                }
+                before += n;
+            }
+        __syncthreads();
+        combo = __builtin_amdgcn_readfirstlane((int)wsum[NW]);
+        at = uniform(wsum[NW + 1]);
+    }
     while (x < end) {
         const int b = combo / a.row_tiles, tile = combo - b * a.row_tiles;
         const SeqView sq = seq_view(a.c, b);
         const int rows = sq.n * a.group, r0 = tile * RM;
         if (r0 >= rows) {
+            if (a.split_tiles == 0) return;
             ++combo;
             continue;
         }
         const TileList<KT> tl(a.window, a.sinks, sq.p0, sq.p0 + (min(r0 + RM, rows) - 1) / a.group, sq.len);
         const int n = max(tl.n, 1), axis = Axis::length(tl.n);
-        if (x >= at + (int64_t)axis * H) {
-            at += (int64_t)axis * H;
-            ++combo;
-            continue;
+        int h = blockIdx.x - combo * H, k0 = 0, k1 = n;
+        bool whole = true;
+        if (a.split_tiles > 0) {
+            if (x >= at + (int64_t)axis * H) {
+                at += (int64_t)axis * H;
+                ++combo;
+                continue;
+            }
+            h = (int)((x - at) / axis);
+            const int64_t item = at + (int64_t)h * axis;
+            k0 = (int)(x - item);
+            k1 = (int)min((int64_t)n, end - item);
+            x = min(item + axis, end);
+            if (k0 >= n) continue;
+            whole = k0 == 0 && k1 == n;
+            if (k0 == 0 && t == 0)
+                a.item_parts[combo * H + h] = make_int2(blockIdx.x, whole ? 0 : (int)((item + n - 1) / share) - (int)blockIdx.x + 1);
         }
-        const int h = (int)((x - at) / axis);
-        const int64_t item = at + (int64_t)h * axis;
-        const int k0 = (int)(x - item), k1 = (int)min((int64_t)n, end - item);
-        x = min(item + axis, end);
-        if (k0 >= n) continue;
-        const bool whole = k0 == 0 && k1 == n;
-        if (k0 == 0 && t == 0)
-            a.item_parts[combo * H + h] = make_int2(blockIdx.x, whole ? 0 : (int)((item + n - 1) / share) - (int)blockIdx.x + 1);
         chunk_item<T, ROWB, KS, DT, NK, NW, true>(a, sm, sq, b, h, tile, tl, k0, min(k1, tl.n),
                                                   whole ? -1 : 2 * (int64_t)blockIdx.x + (k0 == 0 ? 1 : 0));
+        if (a.split_tiles == 0) return;
         __syncthreads();   // its tiles are read
     }
 }

@@ -30,7 +30,7 @@ struct TurnParams {
     int tokens, q_heads, heads;   // heads: keys too
     int head_dim, rotary_dim;
     int groups;               // a thread that turns takes every groups-th head
-    int turned, ends;         // units of a head that turn, and that are copied
+    int turned, ends, odd;    // units of a head that turn, and that are copied: `odd` of these single values
     int copies;               // threads of a token that copy
     int turn_blocks;          // of a sequence
 };
@@ -86,7 +86,6 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnParams a) {
     constexpr int NP = PAIRS && E == 1 ? 2 : E;          // values in a turned unit's piece
     constexpr int ANGLES = PAIRS ? NP / 2 : E, AHEAD = PAIRS ? 4 : 2;   // heads whose loads are in flight
     typedef elem Piece __attribute__((ext_vector_type(NP), aligned(E == 1 ? sizeof(elem) : 16)));
-    typedef elem Copy __attribute__((ext_vector_type(E), aligned(E == 1 ? sizeof(elem) : 16)));
     // The last blocks of a sequence copy: values, and the heads' ends that do not turn.
     const bool copies = blockIdx.x >= (unsigned)a.turn_blocks;
     const int b = APPEND ? blockIdx.y : 0;
@@ -116,9 +115,14 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnParams a) {
 
     if (copies) {
         const int ends = a.heads * a.ends;
-        if (w < ends) {
-            const int h = w / a.ends, e = a.rotary_dim + (w - h * a.ends) * E;
-            if (is(h)) *(Copy*)(target(h) + e * sizeof(elem)) = *(const Copy*)(source(h) + e * sizeof(elem));
+        if (w < ends) {   // the values up to whole pieces one by one, then those
+            const int h = w / a.ends, u = w - h * a.ends;
+            if (!is(h)) return;
+            if (u < a.odd) *((elem*)target(h) + a.rotary_dim + u) = *((const elem*)source(h) + a.rotary_dim + u);
+            else {
+                const int e = a.rotary_dim + a.odd + (u - a.odd) * T::kPiece;
+                *(u32x4*)(target(h) + e * sizeof(elem)) = *(const u32x4*)(source(h) + e * sizeof(elem));
+            }
         } else if constexpr (APPEND) {   // 16 bytes of a value
             const int hv = a.head_dim / 8, p = w - ends, h = p / hv, d = p - h * hv;
             const u32x4 y = *(const u32x4*)(a.v + tok * a.vt + h * a.vh + 16 * d);
@@ -168,7 +172,8 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnParams a) {
 static void divide(TurnParams& a, int piece, bool pairs, bool wide, int64_t tokens) {
     const int e = wide ? piece : 1;
     a.turned = pairs ? a.rotary_dim / (wide ? e : 2) : a.rotary_dim / 2 / e;
-    a.ends = (a.head_dim - a.rotary_dim) / e;
+    a.odd = (piece - a.rotary_dim % piece) % piece;
+    a.ends = a.odd + (a.head_dim - a.rotary_dim - a.odd) / piece;
     a.groups = std::max(a.heads, 1);
     while (a.groups > (a.heads + 7) / 8 && tokens * a.turned * a.groups > 1 << 18) a.groups = (a.groups + 1) / 2;
 }

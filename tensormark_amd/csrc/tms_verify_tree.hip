@@ -64,7 +64,8 @@ __device__ __forceinline__ TreeView tree_view(const VerifyParams& a, int b) {
 
 // One workgroup where it has few words to clear (on one XCD it takes 1.4 us, on all of them 4).
 __global__ __launch_bounds__(1024) void verify_clear_kernel(VerifyParams a) {
-    for (int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x; i < a.words; i += (int64_t)gridDim.x * 1024) st_agent(a.slots + i, (uint64_t)0);
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < a.words; i += (int64_t)gridDim.x * blockDim.x)
+        st_agent(a.slots + i, (uint64_t)0);
 }
 
 // Entries that are no probability count as 0.
@@ -291,9 +292,8 @@ struct Verify {
         return s;
     }
 
-    // The sum of the part's R, by cells.
+    // The sum of the part's R, by cells.  (A barrier has passed since sm.cell was read.)
     __device__ double sum_own() {
-        lds_sync();   // sm.cell has been read
         double s = 0.0;
 #pragma unroll
         for (int k = 0; k < STEPS; ++k) {
@@ -435,8 +435,8 @@ struct Verify {
             }
             if (refused || whole || m == 0) {   // (else the last refusal's sum is R's)
                 if (m == 0) begin(c, whole);
+                lds_sync();   // sm.left, sm.hist and sm.cell have been read
                 if (DRAWN && refused) {
-                    lds_sync();   // sm.left and sm.hist have been read
                     if (up_t == c) sm.left[t] = left_t = fmax(left_t - S * q_t, 0.0);
                     if (t == 0) sm.hist[m] = S;
                     refuse(S);
@@ -572,7 +572,7 @@ extern "C" int tms_verify_tree(const tms_verify_tree_args* args, hipStream_t str
     a.passes = p.passes;
     a.words = (int64_t)p.words;
     a.polls = g_polls.load(std::memory_order_relaxed);
-    if (a.parts > 1) hipLaunchKernelGGL(verify_clear_kernel, dim3(a.words <= 1 << 15 ? 1 : 256), dim3(1024), 0, stream, a);
+    if (a.parts > 1) hipLaunchKernelGGL(verify_clear_kernel, dim3(a.words <= 1 << 15 ? 1 : 256), dim3(a.words <= 1 << 11 ? 256 : 1024), 0, stream, a);
     switch (args->dtype) {
         case TMS_DTYPE_F32: launch_verify<float>(a, args->batch, stream); break;
         case TMS_DTYPE_F16: launch_verify<_Float16>(a, args->batch, stream); break;

@@ -152,6 +152,32 @@ def test_a_workspace_that_is_too_small_is_refused():
     assert lib.tms_tree_attention(C.byref(c), C.byref(a), P, None) == INVALID
 
 
+def test_workspaces_do_not_shrink():
+    """With more positions, sequences or nodes a call needs as much workspace or more."""
+    lib = tree._fns()
+
+    def need(kv, batch, q):
+        c = a_cache(max_kv=kv, table_stride=40000, batch=batch, tokens=q * batch, max_q=q)
+        return lib.tms_tree_attention_workspace(C.byref(c), C.byref(rows_args(cache.AttentionArgs)))
+
+    for q in (3, 40, 64, 200):
+        for batch in (1, 2, 16, 200, 2000):
+            sizes = [need(kv, batch, q) for kv in (1, 100, 512, 1000, 1024, 2000, 3000, 10000, 200000)]
+            assert sizes == sorted(sizes) and sizes[0] == 0 and sizes[-1] > 0, (q, batch, sizes)
+    for q in (3, 40, 64, 200):
+        for kv in (100, 800, 1500, 3000, 50000):
+            sizes = [need(kv, batch, q) for batch in (1, 2, 16, 100, 200, 2000)]
+            assert sizes == sorted(sizes), (q, kv, sizes)
+
+
+def test_more_items_than_32_bits_count():
+    def call_(batch):
+        c = a_cache(batch=batch, kv_heads=1, tokens=512 * 2, max_q=512)
+        return tree._fns().tms_tree_attention_workspace(C.byref(c), C.byref(rows_args(cache.AttentionArgs, q_heads=4096)))
+
+    assert call_(1 << 17) == CAPACITY and call_(1 << 15) >= 0
+
+
 def test_ctypes_layouts_match_the_c_header(tmp_path):
     cc = shutil.which("gcc")
     if cc is None:
