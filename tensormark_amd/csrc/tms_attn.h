@@ -195,7 +195,7 @@ __device__ __forceinline__ bool sees(int j, int p, int window, int sinks) {
 
 // Trees in the chunk kernel: all items (sequence, row tile, key head) lie behind each other on
 // one axis of key tiles, and each workgroup takes an equal share of it, as in the rows kernel
-// (8 sequences of 9000 to 16384, trees of 64 nodes: 160 us with four splits of each sequence, 184 with
+// (8 sequences of 9000 to 16384, trees of 64 nodes: 142 us; 160 with four splits of each sequence, 184 with
 // as many splits as its length asks for, which leaves a second round of workgroups).
 // An item takes kTreeItemCost tiles besides its own.
 constexpr int kTreeItemCost = 4, kTreeLeastShare = 4;
@@ -232,7 +232,7 @@ struct TreeRows {
     int depth[TOKENS];
 
     // The parents of nodes below `end`, a thread's in registers: on the way with the queries, and in LDS
-    // while the first keys are (8 sequences' nodes over 508 positions: 15 us with all of it before the keys).
+    // while the first keys come.
     template <int NT>
     struct Parents {
         int up[TMS_TREE_MAX_NODES / NT];

@@ -506,7 +506,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams a, int rm, in
 
 // The parts of trees' rows from the chunk kernel, which lie as the rows kernel's do: lists are
 // short, and a group of LPR lanes takes a row, four parts' loads in flight (8 sequences of 9000 to 16384, 64
-// nodes: 10 us; 20 with several groups a row).
+// nodes: 11 us; 20 with several groups a row).
 template <typename T, int LPR>
 __global__ __launch_bounds__(256) void attn_tree_join_kernel(AttnParams a, int rm) {
     const int combo = blockIdx.x / a.c.kv_heads, h = blockIdx.x - combo * a.c.kv_heads;

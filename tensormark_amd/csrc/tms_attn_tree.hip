@@ -1,5 +1,16 @@
 // tms_attn_tree.hip -- attention of drafted trees over the paged cache for many rows a key head
 // (tms_tree_attention); up to 32 rows take the rows kernel of tms_attn.hip.
+//
+// The mathematics of tms_attn_chunk.hip's: S^T = K Q^T, weights 2^(s - m), O^T = V^T P^T, m and
+// the sum of weights running per row.  A row sees the prefix and the nodes of its own line, a
+// bit each in LDS (TreeRows); the mask is read only in tiles that hold new tokens, or a window's edge.
+//
+// Few rows over long prefixes (8 nodes and 4 heads a key head are 32 rows): bound by memory, so a
+// key is read once for all rows of its head, 256 of them in 8 waves where there are more than 128.  32 sequences of 257
+// to 8192, 9 to 25 nodes, 8 key heads of 128, 4 heads each, bf16: 129 us, 562 MB, 4.4 TB/s (the card copies
+// at 5.0).  8 of 9000 to 16384 with 64 nodes: 142 us, 106 GFLOP, 740 TFLOP/s (a large product: 1230), where the
+// products take 46 % of a SIMD's cycles and the weights 45 % (153 us with 128 rows a workgroup; 164 with one half of
+// the waves half a tile behind the other; 160 with four tiles on their way).
 #include "tms_attn_chunk.h"
 
 namespace tms {
@@ -8,7 +19,7 @@ __device__ __forceinline__ int64_t uniform(int64_t x) {
     return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)x) | (int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
 }
 
-// Trees: a share of the axis (TreeAxis).
+// A share of the axis (TreeAxis), or an item a workgroup.
 template <typename T, int ROWB, int KS, int DT, int NK, int NW>
 __global__ __launch_bounds__(64 * NW, 2 * (ROWB > 256 ? 1 : 2) / (NW / 2)) void attn_tree_kernel(AttnParams a) {
     constexpr int KT = 32 * NK, RM = 32 * NW;

@@ -8,6 +8,10 @@
 //
 // Bound by memory for a prompt, by latency for a decode step.  An angle serves all of a
 // token's heads: a thread takes one unit (16 bytes, with two halves 2 x 16) of several heads.
+// 16385 tokens, 32 + 8 heads of 128, bf16, pairs, 336 MB: 63 us, 5.3 TB/s.  Into the cache, half
+// layout, 7 prompts of 333 to 2381 tokens, fp16, 234 MB: 58 us, 4.0 TB/s, with two heads' loads ahead (63 with one, 65 with
+// four; 135 with turning and copying by the same threads, whose registers then hold both).  The 64 tokens of a
+// decode step: 7 us, of which the kernel has 4.
 #include <algorithm>
 #include <cmath>
 

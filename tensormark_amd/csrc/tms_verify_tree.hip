@@ -13,6 +13,11 @@
 // the same numbers in the same order; a pass's sums by part go through a word each in
 // global memory, written once, its top bit saying that it is there.  No answer depends on a
 // wait: one that runs out works the missing part's sum out itself, to the same bits.
+//
+// R stays in registers from refusal to refusal, so a row is read once a node.  32 sequences of 9
+// to 25 drawn nodes over 128256 ids, fp32: 32 to 36 us, some 2.9 a pass (1.4 of them the exchange
+// between XCDs, 1.0 the sum; 90 us with R worked out from the rows at each refusal).  64 of 16 given nodes over 151936
+// ids, bf16: 15 us (3.4 the tree, 4.3 the row, 2.2 the exchange).
 #include <algorithm>
 #include <atomic>
 
@@ -32,6 +37,10 @@ static_assert(kVerNodes == kVerThreads, "a thread has a node");
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // A part's ids: those whose R a thread keeps in registers, 16 (32 where it keeps them in 16 bits).
+// A vocabulary of given drafts in 16 bits that fits 64 is one part: nothing to clear or to exchange
+// (5 sequences of 8 nodes over 32000 ids 9.1 us, 10.7 in two parts; 64 of them 9.9 and 11.0.  In fp32, whose rows are
+// twice as long, it takes longer from a few sequences on: 5 11.3 and 9.8, 64 13.1 and 10.4).
+constexpr int kVerMost = kVerThreads * 64;
 constexpr int verify_ids(bool wide, bool drawn) { return kVerThreads * (wide || drawn ? 16 : 32); }
 
 struct VerifyParams {
@@ -92,11 +101,11 @@ __device__ __forceinline__ double wave_upto(double x) {
     return x;
 }
 
-template <typename T, bool DRAWN>
+template <typename T, bool DRAWN, bool ONE>
 struct Verify {
     // Of a part's ids a wave has CELL one after another, in steps of STEP, VEC of them a lane.
     static constexpr int VEC = Elt<T>::kVec, STEP = 64 * VEC;
-    static constexpr int PART = verify_ids(sizeof(T) == 4, DRAWN), CELL = PART / kVerWaves, STEPS = CELL / STEP;
+    static constexpr int PART = ONE ? kVerMost : verify_ids(sizeof(T) == 4, DRAWN), CELL = PART / kVerWaves, STEPS = CELL / STEP;
     struct Shared {
         double u[kVerNodes], left[kVerNodes], q[DRAWN ? kVerNodes : 1];   // R(x) and q(x) of a node under its parent
         double hist[DRAWN ? kVerNodes : 1];                               // S before each refusal at the current node
@@ -339,7 +348,7 @@ struct Verify {
     // The sum over the whole vocabulary; sm.part has the parts'.
     __device__ double sum_all(int c, int m, bool whole) {
         const double mine = sum_own();
-        if (a.parts == 1) return mine;
+        if (ONE || a.parts == 1) return mine;
         uint64_t* const slot = a.slots + ((int64_t)b * a.passes + pass) * a.parts;
         ++pass;
         if (t == 0) st_agent(slot + own, __builtin_bit_cast(uint64_t, mine) | kThere);
@@ -464,7 +473,7 @@ struct Verify {
         if (!(total > 0.0)) return;
         const double aim = fmax(sm.u[0] * total, 0.0);   // (a NaN gives 0)
         double before = 0.0;
-        if (a.parts > 1) {
+        if (!ONE && a.parts > 1) {
             const double s0 = sm.part[2 * lane], s1 = sm.part[2 * lane + 1], s = s0 + s1, upto = wave_upto(s);
             const uint64_t over = __ballot(s > 0.0 && upto > aim), some = __ballot(s > 0.0);
             const int who = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
@@ -478,9 +487,9 @@ struct Verify {
     }
 };
 
-template <typename T, bool DRAWN>
-__global__ __launch_bounds__(kVerThreads, DRAWN ? 4 : 8) void verify_tree_kernel(VerifyParams a) {
-    __shared__ typename Verify<T, DRAWN>::Shared sm;
+template <typename T, bool DRAWN, bool ONE>
+__global__ __launch_bounds__(kVerThreads, DRAWN || ONE ? 4 : 8) void verify_tree_kernel(VerifyParams a) {
+    __shared__ typename Verify<T, DRAWN, ONE>::Shared sm;
     const int b = blockIdx.x / a.parts, part = blockIdx.x - b * a.parts;
     if (tree_view(a, b).n == 0) {
         if (part == 0) {
@@ -492,7 +501,7 @@ __global__ __launch_bounds__(kVerThreads, DRAWN ? 4 : 8) void verify_tree_kernel
         }
         return;
     }
-    Verify<T, DRAWN> v(a, sm, b, part);
+    Verify<T, DRAWN, ONE> v(a, sm, b, part);
     v.run();
 }
 
@@ -504,7 +513,7 @@ struct VerifyPlan {
 static VerifyPlan plan_verify(const tms_verify_tree_args* a) {
     VerifyPlan p;
     const int ids = verify_ids(a->dtype == TMS_DTYPE_F32, a->draft != nullptr);
-    p.parts = (a->vocab + ids - 1) / ids;
+    p.parts = !a->draft && a->dtype != TMS_DTYPE_F32 && a->vocab <= kVerMost ? 1 : (a->vocab + ids - 1) / ids;
     p.passes = a->draft ? a->max_q + 1 : 2;   // the refusals, the last draw, and that again where nothing is left
     p.words = p.parts > 1 ? (size_t)a->batch * p.passes * p.parts : 0;
     p.bytes = p.words * 8;
@@ -534,8 +543,10 @@ static int check_verify(const tms_verify_tree_args* a) {
 template <typename T>
 static void launch_verify(const VerifyParams& a, int batch, hipStream_t stream) {
     const dim3 grid((unsigned)(batch * a.parts));
-    if (a.draft) hipLaunchKernelGGL((verify_tree_kernel<T, true>), grid, dim3(kVerThreads), 0, stream, a);
-    else hipLaunchKernelGGL((verify_tree_kernel<T, false>), grid, dim3(kVerThreads), 0, stream, a);
+    if (a.draft) hipLaunchKernelGGL((verify_tree_kernel<T, true, false>), grid, dim3(kVerThreads), 0, stream, a);
+    else if (sizeof(T) == 2 && a.parts == 1 && a.vocab > verify_ids(false, false))
+        hipLaunchKernelGGL((verify_tree_kernel<T, false, sizeof(T) == 2>), grid, dim3(kVerThreads), 0, stream, a);
+    else hipLaunchKernelGGL((verify_tree_kernel<T, false, false>), grid, dim3(kVerThreads), 0, stream, a);
 }
 
 }  // namespace tms

@@ -143,6 +143,15 @@ def test_rows_of_any_stride_and_alignment(drawn, dt, V):
         t.check(pad=pad, offset=offset)
 
 
+@pytest.mark.parametrize("dt", [F32, HF, BF])
+@pytest.mark.parametrize("V", [8193, 16385, 32767, 32768, 32769, 70003])
+def test_given_drafts_around_whole_parts(dt, V):
+    """A workgroup a sequence (in 16 bits up to 32768 ids), and several."""
+    t = Trees([6, 1, 9], V, drawn=False, dt=dt, seed=V, sharp=3.0)
+    for pad, offset in ((0, 0), (3, 1), (8, 5)):
+        t.check(pad=pad, offset=offset)
+
+
 @pytest.mark.parametrize("drawn", [False, True])
 def test_large_vocabularies(drawn):
     for V, q in ((128256, [9, 4]), (256000, [5]), (1048576, [3])):
