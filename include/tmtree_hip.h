@@ -61,13 +61,16 @@ typedef struct tms_rotary_args {
     float scale;              /* finite */
     int32_t reserved;         /* must be 0 */
 } tms_rotary_args;
+/* Tokens times threads of a token (a thread turns 16 bytes, or twice 16, of up to eight heads, or copies 16;
+ * a value or two, where rotary_dim is not whole pieces) are below 2^32, here and in the next call with
+ * max_q for the tokens. */
 int tms_rotary(const tms_rotary_args* args, hipStream_t stream);
 
 /*
  * tms_kv_append with the keys turned on their way into the cache, and the
  * queries of the same tokens turned into `out`.  Rows of q that belong to no new token
  * (past the last sequence's, or past max_q of one's) are left out; a token without a mapped
- * slot has its queries turned all the same.
+ * slot has its queries turned all the same.  cache->k and cache->v are pools of their own.
  */
 typedef struct tms_append_rotary_args {
     const void* k_new;        /* as in tms_append_args */
@@ -95,7 +98,7 @@ int tms_kv_append_rotary(const tms_cache* cache, const tms_append_rotary_args* a
  * position in the text is above its own - window or below `sinks`.  parents: device,
  * [tokens].  Everything else, the workspace too, is as there, with its own call for the
  * workspace's size; batch times kv_heads times tiles of 128 rows (32, where a page's stride or slots
- * span 2^32 bytes) may be up to 2^30.
+ * span 2^32 bytes) is below 2^23.
  */
 int64_t tms_tree_attention_workspace(const tms_cache* cache, const tms_attention_args* args);
 int tms_tree_attention(const tms_cache* cache, const tms_attention_args* args, const int32_t* parents, hipStream_t stream);
@@ -160,7 +163,7 @@ int tms_debug_verify_polls(int polls);
  * Not copied are entries to or from unmapped pages, with kept[i] outside the sequence, and in
  * place those with kept[i] < i.  A page that two sequences share is written by both, in no order.
  * n_kept is taken as at most max_kept, and in place as at most the sequence's entries from base on.
- * Of the cache's fields `tokens`, `max_q` and `max_kv` are not used.
+ * Of the cache's fields `tokens`, `max_q` and `max_kv` are not used; `k` and `v` are pools of their own.
  */
 typedef struct tms_compact_args {
     const int32_t* kept;      /* device, [batch][kept_stride] */

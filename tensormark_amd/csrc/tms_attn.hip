@@ -600,7 +600,11 @@ static AttnPlan plan_attention(const tms_cache* c, const tms_attention_args* a, 
     if (a->window > 0) keys = std::min<int64_t>(keys, (int64_t)a->window + (tree ? c->max_q : p.rm) + a->sinks + 128);
     const int64_t items = (int64_t)c->batch * c->kv_heads * p.row_tiles;
     int64_t parts;
-    p.fits = (p.chunk && !tree) || items <= (tree ? INT32_MAX / 2 : INT32_MAX);
+    p.fits = (p.chunk && !tree) || items <= INT32_MAX;
+    if (tree) {   // an item's workgroup, or its join's, has up to 512 threads, and a launch fewer than 2^32
+        const int least = std::min(p.rm, kChunkRows);
+        p.fits = (int64_t)c->batch * c->kv_heads * ((rows + least - 1) / least) < 1 << 23;
+    }
     const int part_rows = p.rm;
     p.splits = p.shares = 0;
     p.item_bytes = 0;

@@ -197,6 +197,7 @@ extern "C" int tms_kv_compact(const tms_cache* cache, const tms_compact_args* ar
     if (args->dst_tables && (args->dst_table_stride < 1 || args->dst_tables == cache->tables)) return TMS_ERR_INVALID_ARG;
     if (args->new_len && (args->new_len == cache->kv_len || args->new_len == args->n_kept || args->new_len == args->kept))
         return TMS_ERR_INVALID_ARG;
+    if (cache->k == cache->v) return TMS_ERR_INVALID_ARG;
     CompactParams a{};
     a.c = view_of(cache);
     a.kept = args->kept;

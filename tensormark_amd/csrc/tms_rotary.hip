@@ -195,7 +195,7 @@ static int launch_turns(TurnParams& a, int dtype, bool pairs, int64_t tokens, in
     divide(a, piece, pairs, wide, tokens * batch);
     a.copies = a.heads * a.ends + (APPEND ? a.c.kv_heads * (a.head_dim / 8) : 0);
     const int64_t turn_blocks = (tokens * a.groups * a.turned + 255) / 256, blocks = turn_blocks + (tokens * a.copies + 255) / 256;
-    if (blocks > INT32_MAX) return TMS_ERR_CAPACITY;
+    if (blocks >= 1 << 24) return TMS_ERR_CAPACITY;   // a launch has fewer than 2^32 threads
     a.turn_blocks = (int)turn_blocks;
     const dim3 grid((unsigned)blocks, (unsigned)batch);
     if (dtype == TMS_DTYPE_F32) {
@@ -219,6 +219,11 @@ static bool bad_stride(const int64_t* s, int n) {
     return false;
 }
 
+// An output that is the input has its strides.
+static bool bad_output(const void* x, const int64_t* xs, const void* out, const int64_t* os) {
+    return x == out && (xs[0] != os[0] || xs[1] != os[1]);
+}
+
 static bool bad_rotary(int rotary_dim, int head_dim, int interleaved, float scale) {
     return rotary_dim < 2 || rotary_dim % 2 || rotary_dim > head_dim || (interleaved != 0 && interleaved != 1) || !std::isfinite(scale);
 }
@@ -238,6 +243,7 @@ extern "C" int tms_rotary(const tms_rotary_args* args, hipStream_t stream) {
     if (!args->x || !args->out || !aligned16(args->x) || !aligned16(args->out) || !args->positions || !args->freqs ||
         ((uintptr_t)args->positions & 3) || ((uintptr_t)args->freqs & 3))
         return TMS_ERR_INVALID_ARG;
+    if (bad_output(args->x, args->x_stride, args->out, args->out_stride)) return TMS_ERR_INVALID_ARG;
     const int size = args->dtype == TMS_DTYPE_F32 ? 4 : 2;
     TurnParams a{};
     a.x = (const char*)args->x;
@@ -269,6 +275,8 @@ extern "C" int tms_kv_append_rotary(const tms_cache* cache, const tms_append_rot
     if (!args->k_new || !args->v_new || !aligned16(args->k_new) || !aligned16(args->v_new)) return TMS_ERR_INVALID_ARG;
     if (args->q_heads > 0 && (!args->q || !args->out || !aligned16(args->q) || !aligned16(args->out))) return TMS_ERR_INVALID_ARG;
     if (!args->freqs || ((uintptr_t)args->freqs & 3) || ((uintptr_t)args->positions & 3)) return TMS_ERR_INVALID_ARG;
+    if (args->q_heads > 0 && bad_output(args->q, args->q_stride, args->out, args->out_stride)) return TMS_ERR_INVALID_ARG;
+    if (cache->k == cache->v) return TMS_ERR_INVALID_ARG;
     TurnParams a{};
     a.c = view_of(cache);
     a.x = (const char*)args->q;

@@ -45,7 +45,7 @@ def filled(cls, kw):
 
 
 def call(cls, kw=None, c=None):
-    lib, a, c = tree._fns(), filled(cls, kw or {}), C.byref(a_cache(**(c or {})))
+    lib, a, c = tree._fns(), filled(cls, kw or {}), C.byref(a_cache(**{"v": P + (1 << 20), **(c or {})}))
     if cls is tree.RotaryArgs:
         return lib.tms_rotary(C.byref(a), None)
     if cls is tree.AppendRotaryArgs:
@@ -170,12 +170,27 @@ def test_workspaces_do_not_shrink():
             assert sizes == sorted(sizes), (q, kv, sizes)
 
 
-def test_more_items_than_32_bits_count():
+def test_more_threads_than_a_launch_has():
     def call_(batch):
         c = a_cache(batch=batch, kv_heads=1, tokens=512 * 2, max_q=512)
         return tree._fns().tms_tree_attention_workspace(C.byref(c), C.byref(rows_args(cache.AttentionArgs, q_heads=4096)))
 
-    assert call_(1 << 17) == CAPACITY and call_(1 << 15) >= 0
+    assert call_(1 << 17) == CAPACITY and call_(1 << 9) == CAPACITY and call_((1 << 9) - 1) >= 0
+    assert call(tree.RotaryArgs, dict(tokens=1 << 28, heads=64)) == CAPACITY
+    assert call(tree.AppendRotaryArgs, dict(q_heads=65000), dict(tokens=1 << 20, max_q=1 << 20)) == CAPACITY
+
+
+def test_one_pool_for_keys_and_values_is_refused():
+    """Its entries would be moved, or keys and values written, twice at once."""
+    assert call(tree.AppendRotaryArgs, c=dict(v=P)) == INVALID
+    assert call(tree.CompactArgs, c=dict(v=P)) == INVALID
+    assert call(tree.AppendRotaryArgs, c=dict(v=P, tokens=0)) == 0
+
+
+def test_an_output_that_is_the_input_has_its_strides():
+    assert call(tree.RotaryArgs, dict(x_stride=(0, 256))) == INVALID
+    assert call(tree.RotaryArgs, dict(out_stride=(1, 128))) == INVALID
+    assert call(tree.AppendRotaryArgs, dict(q_stride=(0, 512))) == INVALID
 
 
 def test_ctypes_layouts_match_the_c_header(tmp_path):
