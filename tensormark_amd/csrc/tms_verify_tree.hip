@@ -15,7 +15,7 @@
 // wait: one that runs out works the missing part's sum out itself, to the same bits.
 //
 // R stays in registers from refusal to refusal, so a row is read once a node.  32 sequences of 9
-// to 25 drawn nodes over 128256 ids, fp32: 32 to 36 us, some 2.9 a pass (1.4 of them the exchange
+// to 25 drawn nodes over 128256 ids, fp32: 31 to 36 us, some 2.9 a pass (1.4 of them the exchange
 // between XCDs, 1.0 the sum; 90 us with R worked out from the rows at each refusal).  64 of 16 given nodes over 151936
 // ids, bf16: 15 us (3.4 the tree, 4.3 the row, 2.2 the exchange).
 #include <algorithm>
@@ -71,8 +71,9 @@ __device__ __forceinline__ TreeView tree_view(const VerifyParams& a, int b) {
     return s;
 }
 
-// One workgroup where it has few words to clear (on one XCD it takes 1.4 us, on all of them 4).
-__global__ __launch_bounds__(1024) void verify_clear_kernel(VerifyParams a) {
+// One workgroup for few words to clear (1.4 us; workgroups on all XCDs take 4), four for more (32 sequences of
+// 9 to 25 drawn nodes, 13312 words: 36.0 us a call, 37.1 with one).
+__global__ __launch_bounds__(256) void verify_clear_kernel(VerifyParams a) {
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < a.words; i += (int64_t)gridDim.x * blockDim.x)
         st_agent(a.slots + i, (uint64_t)0);
 }
@@ -583,7 +584,7 @@ extern "C" int tms_verify_tree(const tms_verify_tree_args* args, hipStream_t str
     a.passes = p.passes;
     a.words = (int64_t)p.words;
     a.polls = g_polls.load(std::memory_order_relaxed);
-    if (a.parts > 1) hipLaunchKernelGGL(verify_clear_kernel, dim3(a.words <= 1 << 15 ? 1 : 256), dim3(a.words <= 1 << 11 ? 256 : 1024), 0, stream, a);
+    if (a.parts > 1) hipLaunchKernelGGL(verify_clear_kernel, dim3(a.words <= 1 << 11 ? 1 : a.words <= 1 << 15 ? 4 : 256), dim3(256), 0, stream, a);
     switch (args->dtype) {
         case TMS_DTYPE_F32: launch_verify<float>(a, args->batch, stream); break;
         case TMS_DTYPE_F16: launch_verify<_Float16>(a, args->batch, stream); break;
