@@ -248,11 +248,12 @@ __global__ __launch_bounds__(64 * NW, ROWB > 256 ? 1 : 2) void attn_rows_kernel(
             __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): what went before is not counted below
             load(v, kbase, a.c.kp, kslot, koff, lds0);
             load(v, vbase, a.c.vp, vslot, voff, lds0 + KT * ROWB);
+            if (!TREE && v + NW < kend) entries(v + NW);
         }
         if constexpr (TREE) {
             if (lines) sm_tree.find(a, sq, r0 / G, last - r0 / G + 1, parents);
+            if (v + NW < kend) entries(v + NW);
         }
-        if (v + NW < kend) entries(v + NW);
         for (; v < kend; v += NW) {
             const bool more = v + NW < kend;
             const int t0 = tl.key(v);
