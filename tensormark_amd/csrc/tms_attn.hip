@@ -79,10 +79,10 @@ __device__ __forceinline__ void write_row(const AttnParams& a, const SeqView& sq
 
 template <typename T, int ROWB, int KS, int DT, int NW, bool TREE>
 __global__ __launch_bounds__(64 * NW, ROWB > 256 ? 1 : 2) void attn_rows_kernel(AttnParams a) {
-    constexpr int RM = kShareRows, KT = 32, NL = KT * ROWB / 1024, RPI = 1024 / ROWB, PAD = 33;
+    constexpr int RM = kShareRows, KT = 32, NL = KT * ROWB / 1024, RPI = 1024 / ROWB, ROW = DT * 32 + 4;
     // LDS: the waves' pieces, and at an item's end their outputs, maxima and sums.
     constexpr int RING = NW * 2 * KT * ROWB;
-    constexpr int MERGE = NW * DT * 32 * PAD * 4, ML = NW * 32 * 2 * 4;
+    constexpr int MERGE = NW * 32 * ROW * 4, ML = NW * 32 * 2 * 4;
     __shared__ __attribute__((aligned(128))) char sm[MERGE + ML > RING ? MERGE + ML : RING];
     float* const sm_ml = (float*)(sm + MERGE);   // [wave][row][maximum, sum]
     __shared__ std::conditional_t<TREE, TreeRows<RM>, char> sm_tree;
@@ -365,8 +365,9 @@ __global__ __launch_bounds__(64 * NW, ROWB > 256 ? 1 : 2) void attn_rows_kernel(
             if (more) load(v + NW, vbase, a.c.vp, vslot, voff, lds0 + KT * ROWB);
         }
 
-        // The waves' shares of the item's rows, by way of LDS: an array
-        // [dimension][row] a wave.
+        // The waves' shares of the item's rows, by way of LDS: an array [row][dimension] a wave,
+        // 16 bytes at a time (8 tokens of 4 heads over 508 positions: 13.4 us, 14.3 by single values of
+        // [dimension][row]).
         const bool whole = k0 == 0 && k1 == n;
         const int64_t part = 2 * (int64_t)blockIdx.x + (k0 == 0 ? 1 : 0);
         const int item_id = combo * H + h;
@@ -378,11 +379,13 @@ __global__ __launch_bounds__(64 * NW, ROWB > 256 ? 1 : 2) void attn_rows_kernel(
             sm_ml[(wave * 32 + n32) * 2] = m;
             sm_ml[(wave * 32 + n32) * 2 + 1] = l;
         }
-        float* to = (float*)sm + wave * DT * 32 * PAD;
+        float* to = (float*)sm + (wave * 32 + n32) * ROW + 4 * hh;
+        if (in)
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+            for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) to[(32 * dt + 8 * (i / 4) + 4 * hh + (i & 3)) * PAD + n32] = o[dt][i];
+                for (int c = 0; c < 4; ++c)
+                    *(f32x4*)(to + 32 * dt + 8 * c) = (f32x4){o[dt][4 * c], o[dt][4 * c + 1], o[dt][4 * c + 2], o[dt][4 * c + 3]};
         __syncthreads();
         const int quads = D / 4;
         for (int e = t; e < nr * quads; e += 64 * NW) {
@@ -396,9 +399,9 @@ __global__ __launch_bounds__(64 * NW, ROWB > 256 ? 1 : 2) void attn_rows_kernel(
             for (int w = 0; w < NW; ++w) {
                 const float f = __builtin_amdgcn_exp2f(sm_ml[(w * 32 + rr) * 2] - ref);
                 L += sm_ml[(w * 32 + rr) * 2 + 1] * f;
-                const float* from = (const float*)sm + (w * DT * 32 + d) * PAD + rr;
+                const f32x4 from = *(const f32x4*)((const float*)sm + (w * 32 + rr) * ROW + d);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[i] += from[i * PAD] * f;
+                for (int i = 0; i < 4; ++i) acc[i] += from[i] * f;
             }
             if (!whole) {
                 const int64_t row_at = part * RM + rr;
