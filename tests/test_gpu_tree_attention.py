@@ -183,6 +183,21 @@ def test_long_caches(kv, q, kw):
     check(TreeBatch(kv, q, H=1, G=4, D=128, page=64, seed=9), **kw)
 
 
+@pytest.mark.parametrize("D", [64, 80, 128])
+@pytest.mark.parametrize("kw", [{}, dict(window=900, sinks=3)])
+def test_many_rows_over_long_caches(D, kw):
+    check(TreeBatch([3000, 700, 1300], [64, 60, 33], H=2, G=4, D=D, page=32, seed=D), **kw)
+
+
+def test_more_sequences_than_threads():
+    """A long sequence among hundreds of short ones: shares that hold many of them, and none, whole."""
+    rng = np.random.default_rng(14)
+    q = [int(x) for x in rng.integers(0, 41, 300)]
+    kv = [n + int(x) for n, x in zip(q, rng.integers(0, 90, 300))]
+    q[170], kv[170] = 40, 2900
+    check(TreeBatch(kv, q, H=1, G=1, D=64, seed=15))
+
+
 def test_many_sequences_of_any_lengths():
     rng = np.random.default_rng(11)
     q = [int(x) for x in rng.integers(1, 9, 40)]
