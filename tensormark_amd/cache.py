@@ -14,8 +14,9 @@ The calls run on the tensors' device, on its current stream or on ``stream`` (a
 tensor let go before that one has run needs its ``record_stream``), allocate only
 what they return and, for ``paged_attention``, a workspace, with torch's allocator.
 They raise ValueError for tensors that do not fit and RuntimeError for what the
-library refuses; there is no fallback.  None has a backward: where autograd is on, a
-tensor that requires a gradient is refused.
+library refuses; there is no fallback.  None has a derivative: where autograd is on, a
+tensor that requires a gradient is refused, and so is a forward-mode dual tensor with its
+tangent.
 
 The functions here are thin: the checks and the calls are in
 csrc/tms_cache_py.cpp, built beside the library.  The ctypes structures are the C

@@ -3,6 +3,7 @@
 #pragma once
 
 #include <ATen/MemoryOverlap.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/extension.h>
 
@@ -40,11 +41,15 @@ struct OnDeviceOf {
 
 inline const Tensor* of(const MaybeTensor& t) { return t ? &*t : nullptr; }
 
-// No call has a backward: a gradient that would have to go through one is refused.
+// No call has a derivative: a gradient or a forward-mode tangent that would have to go through one is
+// refused.  (Tangents are on without the gradient mode too.)
 inline void want_no_gradient(std::initializer_list<const Tensor*> tensors) {
-    if (!at::GradMode::is_enabled()) return;
-    for (const Tensor* t : tensors)
-        want(!t || !t->requires_grad(), "no gradient goes through this call: detach its tensors, or call it under torch.no_grad()");
+    const bool gradients = at::GradMode::is_enabled(), tangents = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+    for (const Tensor* t : tensors) {
+        if (!t) continue;
+        want(!gradients || !t->requires_grad(), "no gradient goes through this call: detach its tensors, or call it under torch.no_grad()");
+        want(!tangents || !t->_fw_grad(0).defined(), "no tangent goes through this call: unpack its dual tensors");   // (0: the only level)
+    }
 }
 
 // Autograd finds by its version that a tensor it kept has been written (inference tensors have none).

@@ -11,7 +11,8 @@ token, the others are drafts.
 The calls keep the cache calls' rules: they run on the tensors' device, on its current stream or
 on ``stream`` (a tensor let go before that one has run needs its ``record_stream``), allocate
 only what they return and a workspace, raise ValueError for tensors that do not fit and
-RuntimeError for what the library refuses, have no backward and no fallback.
+RuntimeError for what the library refuses, have no derivative (tensors that require a gradient or
+have a forward-mode tangent are refused) and no fallback.
 
 The functions are thin: the checks and the calls are in csrc/tms_tree_py.cpp, built beside the
 library.  The ctypes structures are the C ABI's, for callers without torch.
