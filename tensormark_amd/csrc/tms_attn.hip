@@ -616,14 +616,16 @@ static AttnPlan plan_attention(const tms_cache* c, const tms_attention_args* a, 
         // Shares for as many workgroups as the card holds at once, with 4 tiles each at least; short
         // sequences whole, and the longer ones of many items, which fill the card without shares (25 nodes, 4 heads
         // a key head: 1 sequence of 760 20 us in shares and 24 whole, 16 of 760 28 and 25, 64 of 2000 115 and 108).
-        // The workspace is that of shares in either case past 8 tiles: it does not shrink with more items.
+        // The workspace is that of shares in either case past 8 tiles, and past 128 dimensions always, where fewer
+        // rows have shares at any length: it does not shrink with more items or rows.
         const int kt = chunk_keys(c->head_dim);
         const int64_t tiles = std::max<int64_t>((keys + kt - 1) / kt, 1);
         p.split_tiles = kTreeLeastShare;
         p.shares = (int)std::min<int64_t>(c->head_dim > 128 || wide ? 256 : 512, (tiles + kTreeItemCost) * items / kTreeLeastShare + 1);
-        parts = tiles > 8 ? 2 * (int64_t)p.shares : 0;
+        const bool shared = tiles > 8 || c->head_dim > 128;
+        parts = shared ? 2 * (int64_t)p.shares : 0;
         p.most_parts = (int)std::min<int64_t>(tiles / kTreeLeastShare + 2, p.shares);
-        p.item_bytes = tiles > 8 ? (size_t)(items * 8 + 15) / 16 * 16 : 0;
+        p.item_bytes = shared ? (size_t)(items * 8 + 15) / 16 * 16 : 0;
         p.join = tiles > std::min<int64_t>(8 + items / 16, 40);
         if (!p.join) {
             p.split_tiles = 0;
