@@ -3,9 +3,10 @@
 //
 // At node c, R = p_c and S = 1; child j (token x) is accepted where u_j q_c(x) S < R(x),
 // and refused it leaves R = max(R - S q_c, 0), S = sum R.  R / S is the residual
-// distribution max(R / S - q, 0) over its sum without a division; R - S q is exact or rounded
-// once in fp64, so products with S below 1 shrink but lose nothing.  With given drafts q is a single id, and
-// what is left of S after refusing x is S - R(x): the walk needs two numbers a node and no row.
+// distribution max(R / S - q, 0) over its sum without a division.  R - S q in fp64 is rounded once at a
+// node's first refusal, where S is 1, and past it twice, the product and the difference: by 2^-53 of each.
+// With given drafts q is a single id, and what is left of S after refusing x is S - R(x): the walk
+// needs two numbers a node and no row.
 //
 // Bound by latency: the walk is a chain, and what it reads depends on it.  A refusal
 // of a drawn draft and the last draw are passes over the vocabulary, so a sequence is divided
