@@ -41,8 +41,8 @@ extern "C" {
  *   (x cos a_i - y sin a_i, y cos a_i + x sin a_i) * scale.
  * Pair i is values i and i + rotary_dim / 2, with `interleaved` values 2 i and 2 i + 1;
  * the values from rotary_dim on are copied.  Angles are reduced in fp64, products and sums
- * are fp32, rounded once to dtype.  The call with negative positions undoes it (and is its
- * gradient).
+ * are fp32, rounded once to dtype.  The call with negative positions is its gradient, and with
+ * 1 / scale undoes it.
  */
 typedef struct tms_rotary_args {
     const void* x;            /* device, [tokens][heads][head_dim]; 16-byte aligned */
@@ -96,7 +96,7 @@ int tms_kv_append_rotary(const tms_cache* cache, const tms_append_rotary_args* a
  * tms_paged_attention for trees: a node sees the positions below p0, its
  * ancestors and itself (on mapped pages).  With window > 0 it sees those of them whose
  * position in the text is above its own - window or below `sinks`.  parents: device,
- * [tokens].  Everything else, the workspace too, is as there, with its own call for the
+ * [tokens].  Everything else, what is rounded and the workspace too, is as there, with its own call for the
  * workspace's size; batch times kv_heads times tiles of 128 rows (32, where a page's stride or slots
  * span 2^32 bytes) is below 2^23.
  */
@@ -114,8 +114,9 @@ int tms_tree_attention(const tms_cache* cache, const tms_attention_args* args, c
  * independently.  Without draft rows the drafts are given: q(x) = 1, and after a refusal
  * R(x) = 0 and S loses what R(x) was.  The step's token is then drawn from what is left of
  * R at the last node: the first id v with R(0) + .. + R(v) > u_0 sum(R), u_0 being node
- * 0's number.  So each step's tokens are distributed as the target's.  Where nothing
- * is left the token is drawn from the target row, and is -1 where that holds nothing.
+ * 0's number.  So each step's tokens are distributed as the target's as far as rows sum to 1,
+ * what S is at first: by as much as they do not, as by their rounding to 16 bits, it is off.
+ * Where nothing is left the token is drawn from the target row, and is -1 where that holds nothing.
  * Entries that are not finite numbers above 0 count as 0, as does a draft outside the vocabulary;
  * products and sums are fp64, sums in a fixed order.  Nodes that node 0 is no ancestor of are never tried.
  */

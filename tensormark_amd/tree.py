@@ -150,7 +150,7 @@ def rotary(x, positions, freqs, *, interleaved: bool = False, scale: float = 1.0
     bf16) by its token's position (int32 ``[tokens]``, any numbers): pairs (x, y) of values i and
     i + len(freqs), or 2 i and 2 i + 1 with ``interleaved``, become (x cos a - y sin a, y cos a +
     x sin a) * scale, with a = position * freqs[i]; the other values are copied.  ``out`` may be
-    ``x`` itself.  Negative positions turn back."""
+    ``x`` itself.  Negative positions turn back (with 1 / ``scale``)."""
     if _OPS is None:
         _ready()
     if stream is not None:
@@ -196,6 +196,7 @@ def verify_tree(target, tokens, parents, q_start, uniforms, *, max_q: int, draft
     against ``uniforms`` (float64 ``[tokens]`` in [0, 1)): accepted with the target's probability
     over the draft's, else the rest of the target over what the draft's share leaves is tried
     further; the step's token is drawn from what is left at the last node with node 0's number.
+    So tokens are distributed as the target's, as far as rows sum to 1.
     ``draft`` holds the rows that each node's children were drawn from, independently; without it the drafts are
     given, by whatever rule.  Returns (path, kept, token): the nodes of the walk, node 0 first
     (int32 ``[batch, max_q]``, -1 past them), how many they are, and the token that follows."""
