@@ -195,8 +195,8 @@ __device__ __forceinline__ bool sees(int j, int p, int window, int sinks) {
 
 // Trees in the chunk kernel: all items (sequence, row tile, key head) lie behind each other on
 // one axis of key tiles, and each workgroup takes an equal share of it, as in the rows kernel
-// (8 sequences of 9000 to 16384, trees of 64 nodes: 142 us; 160 with four splits of each sequence, 184 with
-// as many splits as its length asks for, which leaves a second round of workgroups).
+// (8 sequences of 9000 to 16384, trees of 64 nodes, on one card: 142 us; 160 with four splits of each sequence, 184
+// with as many splits as its length asks for, which leaves a second round of workgroups).
 // An item takes kTreeItemCost tiles besides its own.
 constexpr int kTreeItemCost = 4, kTreeLeastShare = 4;
 template <int KT, int RM>
@@ -223,7 +223,9 @@ __device__ __forceinline__ void lds_barrier() {
 
 // Trees: what the tokens of a group of rows see of the new tokens, a bit each, found by
 // climbing from node to parent in LDS (some 100 cycles a step), and their depths.  With a
-// window a node's own line is cut by it here.
+// window a node's own line is cut by it here, and climbed twice.  A workgroup climbs for each item of whose new tokens it
+// has keys, so deep lines show (4 heads a key head of 128, a chain and a tree one deep, 508 positions before it: 64 nodes
+// 34 and 27 us, 512 nodes 99 and 43, with a window of 256 113 and 39; 16 sequences of 512 nodes after 2000 534 and 384).
 constexpr int kTreeWords = TMS_TREE_MAX_NODES / 32;
 template <int TOKENS>
 struct TreeRows {

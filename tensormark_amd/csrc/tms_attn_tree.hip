@@ -8,9 +8,13 @@
 // Few rows over long prefixes (8 nodes and 4 heads a key head are 32 rows): bound by memory, so a
 // key is read once for all rows of its head, 256 of them in 8 waves where there are more than 128.  32 sequences of 257
 // to 8192, 9 to 25 nodes, 8 key heads of 128, 4 heads each, bf16: 129 us, 562 MB, 4.4 TB/s (the card copies
-// at 5.0).  8 of 9000 to 16384 with 64 nodes: 142 us, 106 GFLOP, 740 TFLOP/s (a large product: 1230), where the
-// products take 46 % of a SIMD's cycles and the weights 45 % (153 us with 128 rows a workgroup; 164 with one half of
-// the waves half a tile behind the other; 160 with four tiles on their way).
+// at 5.0).  8 of 9000 to 16384 with 64 nodes: 142 to 155 us by card and clock, 106 GFLOP, 680 to 740 TFLOP/s (a large
+// product: 1230).  Products have 46 % of a SIMD's cycles there and vector instructions 45 %, where the same loop has 60
+// and 54 % for a prompt's chunk, in two workgroups a CU: one workgroup's waves come to the barrier and to the
+// weights of a tile's first half together, and wait a third of their time (22 % there).  At 142 us: 153 with 128 rows a
+// workgroup; 164 with one half of the waves half a tile behind the other; 160 with four tiles on their way.
+// Past 128 dimensions a wave's outputs and queries alone are 192 registers, so a workgroup has 128 rows, and more rows
+// read the keys again: the 32 sequences with heads of 256 288 us, 3.9 TB/s, the 8 365 us, 580 TFLOP/s.
 #include "tms_attn_chunk.h"
 
 namespace tms {

@@ -16,7 +16,7 @@
 // wait: one that runs out works the missing part's sum out itself, to the same bits.
 //
 // R stays in registers from refusal to refusal, so a row is read once a node.  32 sequences of 9
-// to 25 drawn nodes over 128256 ids, fp32: 31 to 36 us, some 2.9 a pass (1.4 of them the exchange
+// to 25 drawn nodes over 128256 ids, fp32: 28 to 36 us, some 2.9 a pass (1.4 of them the exchange
 // between XCDs, 1.0 the sum; 90 us with R worked out from the rows at each refusal).  64 of 16 given nodes over 151936
 // ids, bf16: 15 us (3.4 the tree, 4.3 the row, 2.2 the exchange).
 #include <algorithm>
